@@ -240,7 +240,7 @@ def _own(state):
         q = torch.empty((step.num_tokens, heads * dim), dtype=state["dtype"], device=DEVICE)
         kernels.qkv_norm_write(state["proj"], state["bias"], step, slot, rotary, heads, kv_heads, dim, dim, state["eps"], state["q_weight"],
                                state["k_weight"], None, q)
-        _, read = kernels.kv_read(step, slot)
+        read = kernels.kv_read(step, slot)
         return q, read.k, read.v
     out = torch.empty_like(state["q"])
     kernels.attention(state["q"], out, step, slot, heads, kv_heads, dim, state["window"] or None, state["scale"], None, 0, state["softcap"],
