@@ -1,0 +1,354 @@
+// Rows on their way into the cache and back: queries, keys and values of a step finished from the projection and stored,
+// in the engine's type or as e4m3 numbers with a scale per row (cached_rows.cuh); pages of an 8-bit cache read back.
+#include <cuda_fp16.h>
+
+#include "cached_rows.cuh"
+
+namespace distie {
+
+// ---- write --------------------------------------------------------------------------------------------------------
+// From the projection [q | k | v] (float32, the slices of a split product, or 16-bit) plus bias: every head of q and k
+// optionally divided by its root mean square before or after the rotation, rotated, q also times a temperature; q goes to
+// q_out, k and v to their place in the pages.  A token's place in its request may differ from its position (drafted tokens:
+// siblings share a position).  The value can be the key as projected.  All arithmetic is float32.
+struct RowsInput {
+  const void* q;
+  const void* k;
+  const void* v;      // null: the value is the key with its bias, before anything else is done to it
+  int q_stride, k_stride, v_stride;  // elements between tokens
+  int splits;
+  long long split_stride;  // elements between slices (float32 only)
+  const float* q_bias;
+  const float* k_bias;
+  const float* v_bias;
+};
+struct RowsNorm {
+  int mode;  // 0 none, 1 before the rotation, 2 after it
+  float eps;
+  const float* q_weight;
+  const float* k_weight;
+};
+struct RowsTurn {
+  const float* inv_freq;  // null: nothing is rotated
+  int rotary_dim, interleaved;
+  float factor;
+  float temp_coef, temp_every;  // temp_every > 0: q at position p times 1 + coef ln(floor((p + 1) / every) + 1)
+};
+struct RowsPlace {
+  const int* positions;
+  const int* slots;  // places in the requests; null: the positions
+  const int* token_seq;
+  const int* seq_seat;
+};
+
+// cos and sin of position * frequency as the exact product: the product's rounding error, up to 2^-24 of an angle of many
+// turns, comes back as a small rotation.  (A float32 product alone is off by 4e-3 at position 65,536.)
+__device__ __forceinline__ void exact_angle(int position, float frequency, float& sn, float& cs) {
+  const float p = (float)position, high = __fmul_rn(p, frequency), low = __fmaf_rn(p, frequency, -high);
+  float s, c;
+  sincosf(high, &s, &c);
+  const float half = 0.5f * low * low;
+  sn = s + (c * low - s * half);
+  cs = c - (s * low + c * half);
+}
+
+template <typename IN>
+__device__ __forceinline__ float input_at(const RowsInput& in, const void* rows, size_t at) {
+  const IN* p = reinterpret_cast<const IN*>(rows) + at;
+  float v = to_float(*p);
+  for (int s = 1; s < in.splits; ++s) v += to_float(p[s * in.split_stride]);
+  return v;
+}
+
+// Scale of a row of largest magnitude `most` (bad: some element is not finite).
+__device__ __forceinline__ float row_scale(float most, bool bad) { return bad ? __int_as_float(0x7fc00000) : most / kE4m3Most; }
+
+constexpr int kWriteWarps = 4;
+
+// A warp per row, a row of any size through shared memory.
+template <typename IN, typename T, int CACHE>
+__global__ void __launch_bounds__(kWriteWarps * 32)
+rows_write_kernel(RowsInput in, RowsNorm norm, RowsTurn turn, RowsPlace place, T* __restrict__ q_out, int q_out_stride,
+                  CachePages cache, void* k_out, void* v_out, float* k_scale, float* v_scale, int num_heads, int num_kv_heads,
+                  int write, int* __restrict__ error) {
+  extern __shared__ __align__(16) float rows_s[];  // a piece per warp, then cos and sin of the token
+  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int dim = cache.key_dim, vdim = cache.value_dim, piece = max(dim, vdim);
+  float* row_s = rows_s + (size_t)warp * piece;
+  float* cos_s = rows_s + (size_t)kWriteWarps * piece;
+  const int half = turn.inv_freq ? turn.rotary_dim / 2 : 0;
+  float* sin_s = cos_s + half;
+  const int position = place.positions[t];
+  for (int i = threadIdx.x; i < half; i += blockDim.x) {
+    float sn, cs;
+    exact_angle(position, turn.inv_freq[i], sn, cs);
+    cos_s[i] = cs * turn.factor;
+    sin_s[i] = sn * turn.factor;
+  }
+  long long place_row = -1;  // of kv head 0
+  if (write) {
+    const int seat = place.seq_seat[place.token_seq[t]];
+    const int slot = place.slots ? place.slots[t] : position;
+    place_row = slot < 0 ? -1 : cache.row_of(cache.block_table + (size_t)seat * cache.table_width, slot, 0);
+    if (place_row < 0 && threadIdx.x == 0 && error) atomicExch(error, 2);
+  }
+  const float temperature =
+      turn.temp_every > 0.f ? 1.f + turn.temp_coef * logf(floorf((float)(position + 1) / turn.temp_every) + 1.f) : 1.f;
+  __syncthreads();
+  const int rows_here = num_heads + (write ? 2 * num_kv_heads : 0);
+  for (int index = blockIdx.y * kWriteWarps + warp; index < rows_here; index += gridDim.y * kWriteWarps) {
+    const bool is_query = index < num_heads, is_value = index >= num_heads + num_kv_heads;
+    const int head = is_query ? index : (index - num_heads) % num_kv_heads;
+    const bool from_key = is_value && in.v == nullptr;
+    const int n = is_value ? vdim : dim;
+    const void* rows = is_query ? in.q : (is_value && !from_key) ? in.v : in.k;
+    const int stride = is_query ? in.q_stride : (is_value && !from_key) ? in.v_stride : in.k_stride;
+    const float* bias = is_query ? in.q_bias : (is_value && !from_key) ? in.v_bias : in.k_bias;
+    if (!is_query && place_row < 0) continue;
+    const size_t at = (size_t)t * stride + (size_t)head * n;
+    // A value goes straight to its page; a query or key stays in shared memory between the steps.
+    float squares = 0.f;
+    if (!is_value) {
+      for (int e = lane; e < n; e += 32) {
+        const float x = input_at<IN>(in, rows, at + e) + (bias ? bias[head * n + e] : 0.f);
+        row_s[e] = x;
+        squares += x * x;
+      }
+      const float* weight = is_query ? norm.q_weight : norm.k_weight;
+      if (norm.mode == 1) {
+        const float unit = rsqrtf(warp_sum(squares) / (float)n + norm.eps);
+        for (int e = lane; e < n; e += 32) row_s[e] = row_s[e] * unit * (weight ? weight[e] : 1.f);
+      }
+      __syncwarp();
+      for (int i = lane; i < half; i += 32) {
+        const int a = turn.interleaved ? 2 * i : i, b = turn.interleaved ? 2 * i + 1 : i + half;
+        const float sn = sin_s[i], cs = cos_s[i], u = row_s[a], v = row_s[b];
+        row_s[a] = u * cs - v * sn;
+        row_s[b] = v * cs + u * sn;
+      }
+      __syncwarp();
+      if (norm.mode == 2) {
+        squares = 0.f;
+        for (int e = lane; e < n; e += 32) squares += row_s[e] * row_s[e];
+        const float unit = rsqrtf(warp_sum(squares) / (float)n + norm.eps);
+        for (int e = lane; e < n; e += 32) row_s[e] = row_s[e] * unit * (weight ? weight[e] : 1.f);
+        __syncwarp();
+      }
+    } else {
+      for (int e = lane; e < n; e += 32) row_s[e] = input_at<IN>(in, rows, at + e) + (bias ? bias[head * n + e] : 0.f);
+      __syncwarp();
+    }
+    if (is_query) {
+      for (int e = lane; e < n; e += 32) q_out[(size_t)t * q_out_stride + (size_t)head * n + e] = from_float<T>(row_s[e] * temperature);
+    } else {
+      const size_t to = (size_t)(place_row + (long long)head * cache.page_size) * n;
+      void* out = is_value ? v_out : k_out;
+      if (CACHE == DISTIE_E4M3) {
+        float most = 0.f;
+        bool bad = false;
+        for (int e = lane; e < n; e += 32) {
+          const float size = fabsf(row_s[e]);
+          bad |= !(size <= 3.402823466e38f);
+          most = fmaxf(most, size);
+        }
+        most = warp_max(most);
+        bad = __any_sync(0xffffffffu, bad);
+        const float scale = row_scale(most, bad);
+        if (lane == 0) (is_value ? v_scale : k_scale)[place_row + (long long)head * cache.page_size] = scale;
+        for (int e = lane; e < n; e += 32)
+          reinterpret_cast<uint8_t*>(out)[to + e] =
+              (bad || scale == 0.f) ? (uint8_t)0 : (uint8_t)__nv_cvt_float_to_fp8(row_s[e] / scale, __NV_SATFINITE, __NV_E4M3);
+      } else {
+        for (int e = lane; e < n; e += 32) {
+          if (CACHE == DISTIE_BF16) reinterpret_cast<__nv_bfloat16*>(out)[to + e] = __float2bfloat16_rn(row_s[e]);
+          else reinterpret_cast<float*>(out)[to + e] = row_s[e];
+        }
+      }
+    }
+    __syncwarp();  // before the next row overwrites the piece
+  }
+}
+
+// ---- read back ----------------------------------------------------------------------------------------------------
+// Pages of up to kReadRows requests, one page of the result per block: numbers times scales in the set's type, zeros behind
+// a request's last row.  A page of the cache is one run of memory over all kv heads, and so is a page of the result.
+constexpr int kReadRows = 256;
+struct ReadPlan {
+  int count;
+  int batch_row[kReadRows];    // of the step: its seat is read, and that seat's row of the result's table filled
+  int first_page[kReadRows];   // pages of the result before this request's
+  int first_column[kReadRows]; // its first logical page that is read
+  int hole[kReadRows];         // logical pages hole .. hole_end - 1 are not read: a window has passed them
+  int hole_end[kReadRows];
+  int length[kReadRows];       // its keys
+};
+
+template <typename T>
+__device__ __forceinline__ void store_row16(T* to, const float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float half[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) half[e] = v[8 * i + e];
+    store8(to + 8 * i, half);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void read_rows(const uint8_t* __restrict__ numbers, const float* __restrict__ scales, T* __restrict__ to,
+                                          int rows, int dim, int page_size, int live) {
+  if ((dim & 15) == 0) {
+    const int pieces = rows * (dim / 16);
+    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+      const int row = i / (dim / 16);
+      float v[16];
+      if (row % page_size < live) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(numbers + (size_t)i * 16);
+        const float s = scales[row];
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float f[4];
+          e4m3x4_to_float(w[j], f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * j + e] = f[e] * s;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = 0.f;
+      }
+      store_row16(to + (size_t)i * 16, v);
+    }
+  } else {
+    for (int i = threadIdx.x; i < rows * dim; i += blockDim.x) {
+      const int row = i / dim;
+      to[i] = from_float<T>(row % page_size < live ? e4m3_to_float(numbers[i]) * scales[row] : 0.f);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+rows_read_kernel(const __grid_constant__ ReadPlan plan, CachePages cache, const int* __restrict__ seq_seat, T* __restrict__ k_out,
+                 T* __restrict__ v_out, int* __restrict__ table_out, int page0, int pages, int* __restrict__ error) {
+  if ((int)blockIdx.x >= pages) {  // blocks behind the pages: a row of the result's table each
+    const int i = blockIdx.x - pages;
+    const int columns = (plan.length[i] + cache.page_size - 1) / cache.page_size;
+    int* row = table_out + (size_t)seq_seat[plan.batch_row[i]] * cache.table_width;
+    for (int c = threadIdx.x; c < cache.table_width; c += blockDim.x)
+      row[c] = c >= plan.first_column[i] && c < columns && (c < plan.hole[i] || c >= plan.hole_end[i])
+                   ? plan.first_page[i] + c - plan.first_column[i] : -1;
+    return;
+  }
+  const int page_out = page0 + blockIdx.x;
+  int i = 0;
+  for (int step = kReadRows / 2; step > 0; step >>= 1)
+    if (i + step < plan.count && plan.first_page[i + step] <= page_out) i += step;
+  const int column = plan.first_column[i] + page_out - plan.first_page[i];
+  if (column >= plan.hole[i] && column < plan.hole_end[i]) return;  // (no table entry names this page of the result)
+  const int seat = seq_seat[plan.batch_row[i]];
+  const int page = column < cache.table_width ? cache.block_table[(size_t)seat * cache.table_width + column] : -1;
+  int live = min(cache.page_size, plan.length[i] - column * cache.page_size);
+  if (page < 0 || page >= cache.num_pages) {
+    if (threadIdx.x == 0 && error) atomicExch(error, 5);
+    live = 0;
+  }
+  const int rows = cache.num_kv_heads * cache.page_size;
+  const size_t from = (size_t)max(page, 0) * rows, to = (size_t)page_out * rows;
+  read_rows(reinterpret_cast<const uint8_t*>(cache.k) + from * cache.key_dim, cache.k_scale + from, k_out + to * cache.key_dim, rows,
+            cache.key_dim, cache.page_size, live);
+  read_rows(reinterpret_cast<const uint8_t*>(cache.v) + from * cache.value_dim, cache.v_scale + from, v_out + to * cache.value_dim, rows,
+            cache.value_dim, cache.page_size, live);
+}
+
+template <typename IN, typename T, int CACHE>
+static int launch_write(const RowsInput& in, const RowsNorm& norm, const RowsTurn& turn, const RowsPlace& place, void* q_out,
+                        int q_out_stride, const CachePages& cache, void* k_out, void* v_out, float* k_scale, float* v_scale,
+                        int tokens, int num_heads, int num_kv_heads, int write, int* error, cudaStream_t stream) {
+  const int rows = num_heads + (write ? 2 * num_kv_heads : 0);
+  const dim3 grid(tokens, tokens < 512 ? (rows + kWriteWarps - 1) / kWriteWarps : 1);
+  const size_t shared = ((size_t)kWriteWarps * max(cache.key_dim, cache.value_dim) + turn.rotary_dim) * sizeof(float);
+  rows_write_kernel<IN, T, CACHE><<<grid, kWriteWarps * 32, shared, stream>>>(in, norm, turn, place, (T*)q_out, q_out_stride, cache, k_out,
+                                                                              v_out, k_scale, v_scale, num_heads, num_kv_heads, write, error);
+  DISTIE_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace distie
+
+using namespace distie;
+
+// in_type: DISTIE_F32 or DISTIE_BF16 (one slice).  out_type: of q_out.  cache_type: DISTIE_F32, DISTIE_BF16 or DISTIE_E4M3
+// (with scales).  num_heads 0: there are no queries.  write 0: only the queries are made.
+extern "C" int distie_rows_write(const void* q, int q_stride, const void* k, int k_stride, const void* v, int v_stride, int in_type,
+                                 int splits, long long split_stride, const float* q_bias, const float* k_bias, const float* v_bias,
+                                 int norm_mode, float norm_eps, const float* q_weight, const float* k_weight, const float* inv_freq,
+                                 int rotary_dim, int interleaved, float factor, float temp_coef, float temp_every,
+                                 const int* positions, const int* slots, const int* token_seq, const int* seq_seat,
+                                 const int* block_table, int table_width, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                                 int tokens, int num_heads, int num_kv_heads, int key_dim, int value_dim, int page_size, int num_pages,
+                                 int write, void* q_out, int q_out_stride, int out_type, int cache_type, int* error,
+                                 cudaStream_t stream) {
+  if (tokens <= 0) return 0;
+  if (num_heads < 0 || num_kv_heads < 1 || key_dim < 1 || key_dim > 1024 || value_dim < 1 || value_dim > 1024 || rotary_dim < 0 ||
+      rotary_dim > key_dim || (rotary_dim & 1) || splits < 1 || page_size < 1 || table_width < 1 || num_heads + 2 * num_kv_heads > 65535 ||
+      (in_type == DISTIE_BF16 && splits != 1) || (num_heads > 0 && (q == nullptr || q_out == nullptr)) ||
+      (write && (k == nullptr || k_cache == nullptr || v_cache == nullptr || block_table == nullptr)) ||
+      (write && v == nullptr && value_dim != key_dim) || (write && cache_type == DISTIE_E4M3 && (k_scale == nullptr || v_scale == nullptr)) ||
+      norm_mode < 0 || norm_mode > 2)
+    return DISTIE_ERR_ARG;
+  const RowsInput in{q, k, v, q_stride, k_stride, v_stride, splits, split_stride, q_bias, k_bias, v_bias};
+  const RowsNorm norm{norm_mode, norm_eps, q_weight, k_weight};
+  const RowsTurn turn{rotary_dim > 0 ? inv_freq : nullptr, rotary_dim, interleaved, factor, temp_coef, temp_every};
+  const RowsPlace place{positions, slots, token_seq, seq_seat};
+  const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, key_dim, value_dim,
+                                      page_size, num_pages);
+#define DISTIE_ROWS_WRITE(IN, T, CACHE)                                                                                     \
+  return launch_write<IN, T, CACHE>(in, norm, turn, place, q_out, q_out_stride, cache, k_cache, v_cache, k_scale, v_scale,   \
+                                    tokens, num_heads, num_kv_heads, write, error, stream)
+  if (in_type == DISTIE_F32 && out_type == DISTIE_BF16) {
+    if (cache_type == DISTIE_E4M3) DISTIE_ROWS_WRITE(float, __nv_bfloat16, DISTIE_E4M3);
+    if (cache_type == DISTIE_BF16) DISTIE_ROWS_WRITE(float, __nv_bfloat16, DISTIE_BF16);
+  } else if (in_type == DISTIE_BF16 && out_type == DISTIE_BF16) {
+    if (cache_type == DISTIE_E4M3) DISTIE_ROWS_WRITE(__nv_bfloat16, __nv_bfloat16, DISTIE_E4M3);
+    if (cache_type == DISTIE_BF16) DISTIE_ROWS_WRITE(__nv_bfloat16, __nv_bfloat16, DISTIE_BF16);
+  } else if (in_type == DISTIE_F32 && out_type == DISTIE_F32) {
+    if (cache_type == DISTIE_E4M3) DISTIE_ROWS_WRITE(float, float, DISTIE_E4M3);
+    if (cache_type == DISTIE_F32) DISTIE_ROWS_WRITE(float, float, DISTIE_F32);
+  }
+#undef DISTIE_ROWS_WRITE
+  return DISTIE_ERR_UNSUPPORTED;
+}
+
+// plan: `count` rows (batch row, first page of the result, first logical page, hole, end of the hole, keys) on the host; their
+// pages of the result are page0 .. page0 + pages - 1.  table_out: of the shape of block_table.
+extern "C" int distie_rows_read(const int* plan, int count, const void* k_cache, const void* v_cache, const float* k_scale,
+                                const float* v_scale, const int* block_table, int table_width, const int* seq_seat, int num_kv_heads,
+                                int key_dim, int value_dim, int page_size, int num_pages, void* k_out, void* v_out, int* table_out,
+                                int page0, int pages, int out_type, int* error, cudaStream_t stream) {
+  if (count <= 0 || pages <= 0) return 0;
+  if (count > kReadRows || num_kv_heads < 1 || key_dim < 1 || value_dim < 1 || page_size < 1 || table_width < 1 || k_scale == nullptr || v_scale == nullptr)
+    return DISTIE_ERR_ARG;
+  ReadPlan p;
+  p.count = count;
+  for (int i = 0; i < count; ++i) {
+    p.batch_row[i] = plan[6 * i];
+    p.first_page[i] = plan[6 * i + 1];
+    p.first_column[i] = plan[6 * i + 2];
+    p.hole[i] = plan[6 * i + 3];
+    p.hole_end[i] = plan[6 * i + 4];
+    p.length[i] = plan[6 * i + 5];
+  }
+  const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, key_dim, value_dim,
+                                      page_size, num_pages);
+  if (out_type == DISTIE_BF16)
+    rows_read_kernel<<<pages + count, 256, 0, stream>>>(p, cache, seq_seat, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, table_out,
+                                                        page0, pages, error);
+  else if (out_type == DISTIE_F32)
+    rows_read_kernel<<<pages + count, 256, 0, stream>>>(p, cache, seq_seat, (float*)k_out, (float*)v_out, table_out, page0, pages,
+                                                        error);
+  else
+    return DISTIE_ERR_UNSUPPORTED;
+  DISTIE_LAUNCH_CHECK();
+  return 0;
+}

@@ -1,8 +1,8 @@
 """Kernel sets: the interface parts are written against and the CUDA implementation."""
 
-from .interface import KernelSet, KvSlot, RotaryTable, StepTensors
+from .interface import DraftTree, KernelSet, KvSlot, RotaryTable, StepTensors
 
-__all__ = ["KernelSet", "KvSlot", "RotaryTable", "StepTensors", "make_kernels"]
+__all__ = ["DraftTree", "KernelSet", "KvSlot", "RotaryTable", "StepTensors", "make_kernels"]
 
 
 def make_kernels(dtype, device="cuda:0") -> KernelSet:

@@ -21,9 +21,11 @@ import torch
 
 import ctypes
 import math
+from contextlib import nullcontext
 from dataclasses import replace
 
 from . import library
+from .cached import CachedRows
 from .interface import KernelSet, Normed, StepTensors, Terms
 from .library import KernelError, check, function
 
@@ -52,6 +54,7 @@ _ERROR_TEXT = {
     6: "a kernel gave up waiting for its own copies or instructions",
     7: "a router chose an expert that does not exist",
     5: "a block table does not cover the keys a portion of a prompt attends to",
+    8: "a block table does not cover the keys a drafted token attends to",
 }
 
 
@@ -160,7 +163,10 @@ def pairs_pay(portions: list, heads: int, kv_heads: int, window: int, longest: i
     return two < 0.9 * one
 
 
-class DeviceKernels(KernelSet):
+_NOTHING = nullcontext()
+
+
+class DeviceKernels(CachedRows, KernelSet):
     def __init__(self, dtype: torch.dtype, device: torch.device | str = "cuda:0") -> None:
         if dtype not in _CODE:
             raise KernelError(f"no kernel set for dtype {dtype}; the engine runs bfloat16 or float32")
@@ -191,6 +197,10 @@ class DeviceKernels(KernelSet):
     def _stream(self) -> int:
         # The handle alone: torch.cuda.current_stream() builds an object around it, 3 us a launch on the host.
         return torch._C._cuda_getCurrentRawStream(self._index)
+
+    def _here(self):
+        """The set's device as the current one while a kernel is launched (a stream belongs to its device)."""
+        return _NOTHING if torch._C._cuda_getDevice() == self._index else torch.cuda.device(self._index)
 
     def _ran(self, name: str, kernels: int = 1) -> None:
         self.launches += kernels
@@ -411,6 +421,15 @@ class DeviceKernels(KernelSet):
         self._ran("swiglu")
 
     def rope_kv_write(self, qkv, step, kv, rotary, num_heads, num_kv_heads, head_dim, bias=None, q_out=None) -> None:
+        if self._apart(step, kv):
+            if qkv.dim() == 3 and q_out is None:
+                raise KernelError("rope_kv_write: slices of a projection need a q_out buffer")
+            turned = q_out if qkv.dim() == 3 else qkv[:, : num_heads * head_dim]  # (a finished projection is rotated in place)
+            self._write_projection("rope_kv_write", qkv, bias if qkv.dim() == 3 else None, step, kv, rotary, num_heads, num_kv_heads,
+                                   head_dim, head_dim, turned)
+            if q_out is not None and turned is not q_out:
+                q_out.copy_(turned)
+            return
         write = kv is not None
         table = kv.block_table if write else step.seq_seat  # any valid pointer when nothing is written
         tail = [
@@ -461,7 +480,7 @@ class DeviceKernels(KernelSet):
         epilogue of the tcgen05 product, which reads the step's angles and cache rows from a table made once
         per step.  Everything else: the product's float32 slices into the rotation kernel."""
         fused = (
-            self._tensor_core(x, weight) and head_dim in (64, 128)
+            not self._apart(step, kv) and self._tensor_core(x, weight) and head_dim in (64, 128)
             and weight.shape[0] == (num_heads + 2 * num_kv_heads) * head_dim
             and (rotary is None or (rotary.rotary_dim == head_dim and not rotary.interleaved))
             and (bias is None or bias.dtype == torch.float32)
@@ -524,7 +543,7 @@ class DeviceKernels(KernelSet):
         projection's float32 slices itself (bias, rotation, the token's key and value into the cache and into
         its own tile), so the kernel between the projection and the attention is not launched."""
         merged = (
-            step.num_decode_tokens == step.num_tokens and self.dtype == torch.bfloat16 and head_dim in _PREFILL_HEAD_DIMS
+            step.tree is None and kv.k_scale is None and step.slots is None and step.num_decode_tokens == step.num_tokens and self.dtype == torch.bfloat16 and head_dim in _PREFILL_HEAD_DIMS
             and self._skinny(x, weight) and weight.shape[0] == (num_heads + 2 * num_kv_heads) * head_dim
             and (rotary is None or (rotary.rotary_dim == head_dim and not rotary.interleaved))
             and (bias is None or bias.dtype == torch.float32) and kv.k.dtype == torch.bfloat16
@@ -570,6 +589,19 @@ class DeviceKernels(KernelSet):
         sink_ptr = sink.data_ptr() if sink is not None else None
         if sink is not None and (sink.dtype != torch.float32 or sink.numel() != num_heads or not sink.is_contiguous()):
             raise KernelError("attention: the sink is one float32 per head")
+        if step.tree is not None:
+            self._attention_rows(qkv, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first, softcap, sink,
+                                 step.num_tokens, step.num_seqs)
+            return
+        portions_only = kv.k_scale is not None
+        if portions_only:  # single tokens attend to the numbers as they are, portions to the pages read back
+            singles = step.num_decode_tokens
+            if singles > 0:
+                self._attention_rows(qkv, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first, softcap,
+                                     sink, singles, singles)
+            if singles == step.num_tokens:
+                return
+            kv = self.kv_read(step, kv, window, chunk, keep_first)
         extras = softcap > 0.0 or sink is not None
         value_dim = kv.v.shape[-1]
         same = value_dim == head_dim
@@ -579,9 +611,9 @@ class DeviceKernels(KernelSet):
                   and value_dim % 8 == 0 and _RAGGED_FROM <= max(head_dim, value_dim) <= max(_PREFILL_HEAD_DIMS)
                   and qkv.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and kv.k.is_contiguous() and kv.v.is_contiguous())
         tile_dim = (64 if max(head_dim, value_dim) <= 64 else 128) if ragged else (head_dim if same else 0)  # 0: no tiles
-        n_dec = step.num_decode_tokens if ragged or (head_dim in _DECODE_HEAD_DIMS and same) else 0
+        n_dec = step.num_decode_tokens if ragged or portions_only or (head_dim in _DECODE_HEAD_DIMS and same) else 0
         element = qkv.element_size()
-        if n_dec > 0:
+        if n_dec > 0 and not portions_only:
             splits = self.plan_splits(n_dec, num_heads, num_kv_heads, step.max_kv_len)
             tensor_cores = self.dtype == torch.bfloat16 and tile_dim in _PREFILL_HEAD_DIMS
             if tensor_cores and splits <= 2 * _CLUSTER_SPLITS:
@@ -776,6 +808,9 @@ class DeviceKernels(KernelSet):
         return x.data_ptr(), x.stride(0), 1, 0
 
     def kv_write(self, k, v, step, kv) -> None:
+        if self._apart(step, kv):
+            self._rows_write("kv_write", None, k, v, (None, None, None), step, kv, None, 0, kv.k.shape[1], kv.k.shape[-1], kv.v.shape[-1], None)
+            return
         if k.dtype != v.dtype or k.dtype not in _CODE or k.stride(1) != 1 or v.stride(1) != 1:
             raise KernelError("kv_write: keys and values of one float type with unit column stride are expected")
         check(
@@ -1126,6 +1161,11 @@ class DeviceKernels(KernelSet):
         self._ran("average_add_rmsnorm")
 
     def qk_rope_norm_write(self, qk, bias, step, kv, rotary, num_heads, num_kv_heads, head_dim, norm_eps, q_out) -> None:
+        if self._apart(step, kv):
+            norm = (0, 0.0, None, None) if norm_eps is None else (2, float(norm_eps), None, None)
+            self._write_projection("qk_rope_norm_write", self._rows32(qk, "qk_rope_norm_write"), bias, step, kv, rotary, num_heads,
+                                   num_kv_heads, head_dim, head_dim, q_out, norm, values=False)
+            return
         write = kv is not None
         if write and kv.k.dtype != q_out.dtype:
             raise KernelError("qk_rope_norm_write: the cache and q are of one type")
@@ -1148,6 +1188,11 @@ class DeviceKernels(KernelSet):
 
     def qkv_norm_write(self, qkv, bias, step, kv, rotary, num_heads, num_kv_heads, head_dim, value_dim, norm_eps,
                        q_weight, k_weight, q_temp, q_out) -> None:
+        if self._apart(step, kv):
+            norm = (0, 0.0, None, None) if norm_eps is None else (1, float(norm_eps), q_weight, k_weight)
+            self._write_projection("qkv_norm_write", self._rows32(qkv, "qkv_norm_write"), bias, step, kv, rotary, num_heads, num_kv_heads,
+                                   head_dim, value_dim, q_out, norm, q_temp)
+            return
         write = kv is not None
         if write and (kv.k.dtype != q_out.dtype or kv.v.shape[-1] != value_dim or kv.k.shape[-1] != head_dim):
             raise KernelError("qkv_norm_write: the cache holds keys of head_dim and values of value_dim, of q's type")

@@ -17,6 +17,11 @@ Shapes (``T`` tokens of this step, ``B`` requests of this step):
     block_table [seats, width] int32.  In a group whose values lie inside its keys (attention through
     a latent) ``v`` is a view of the first ``value_dim`` columns of ``k``.
 
+    A slot in eight bits holds e4m3 numbers (``torch.float8_e4m3fn``) and ``k_scale``, ``v_scale [pages, kv_heads,
+    page_size]`` float32: the row of a token and kv head stands for its numbers times its scale, the largest magnitude
+    of the row as it was stored over 448.  A row that held a number that is not finite reads back as NaN throughout.
+``DraftTree``     drafted tokens: every entry of the step is a tree of new tokens behind its cached ones (see there).
+
 Which keys a token sees: all keys up to its own position (``first_visible``), the last
 ``window`` of them, or those of its own ``chunk`` (positions ``chunk * n .. chunk * (n + 1) - 1``);
 beside a window, the request's first ``keep_first`` positions when a layer keeps them.
@@ -33,6 +38,22 @@ import torch
 Q_TILE = 128  # tokens per tile of StepTensors.q_tiles
 
 
+MOST_DRAFTED = 256  # new tokens of one request that a step of drafted tokens takes
+
+
+@dataclass
+class DraftTree:
+    """The new tokens of a step of drafted tokens.  Request b brings ``nodes`` of them, tokens ``first .. first + nodes - 1``
+    of the step, behind ``past`` cached ones; new token j stands in the cache's place ``past + j`` (``StepTensors.slots``)
+    whatever its position, ``past`` plus its depth.  A new token sees the cached keys that its window or chunk allows, and of
+    its request's new tokens those whose bits are set in its mask: itself and its ancestors, or any others; a token whose
+    mask is empty and that has no cached key gets zeros.  Windows and chunks count positions, not places."""
+
+    bits: torch.Tensor  # [T, words] int32: bit j % 32 of word j / 32 is new token j of the same request
+    seqs: torch.Tensor  # [B, 3] int32: first, nodes, past
+    most_nodes: int     # of a request, at most MOST_DRAFTED
+
+
 @dataclass
 class StepTensors:
     token_ids: torch.Tensor
@@ -46,6 +67,8 @@ class StepTensors:
     q_tiles: torch.Tensor | None = None  # [n, 2] int32: (first token, rows <= Q_TILE) of each tile of the
     num_q_tiles: int = 0                 # multi-token entries; a tile holds consecutive tokens of one request
     portions: list | None = None         # (cached tokens, new tokens) of the multi-token entries, where the host knows them
+    slots: torch.Tensor | None = None    # [T] int32: each token's place in the cache where that is not its position
+    tree: DraftTree | None = None        # a step of drafted tokens
     derived: dict = field(default_factory=dict)  # what a kernel set made of this step once and its layers share
 
 
@@ -56,6 +79,8 @@ class KvSlot:
     block_table: torch.Tensor
     page_size: int
     num_pages: int
+    k_scale: torch.Tensor | None = None  # of a cache in eight bits: a float32 per row
+    v_scale: torch.Tensor | None = None
 
 
 def first_visible(position: int, window: int | None = None, chunk: int | None = None) -> int:
@@ -231,7 +256,17 @@ class KernelSet(ABC):
         The size of a value is the last dimension of ``kv.v`` and may differ from ``head_dim``; ``out`` is
         ``[T, heads * value size]``.  ``softcap > 0``: a score ``s = q . k * scale`` becomes ``softcap * tanh(s /
         softcap)``.  ``sink [heads]`` (float32): the softmax's denominator also holds ``exp(sink_h)``, a term with
-        no key and no value that is neither scaled nor capped."""
+        no key and no value that is neither scaled nor capped.  A step of drafted tokens (``step.tree``) sees what
+        :class:`DraftTree` says; a cache in eight bits serves every step."""
+
+    def kv_read(self, step: StepTensors, kv: KvSlot, window: int | None = None, chunk: int | None = None,
+                keep_first: int = 0) -> KvSlot:
+        """What the requests of the step's portions hold in a cache in eight bits, read back to the set's dtype: a slot
+        with pages of its own, one request's behind the other's in the order of the step, rows behind a request's last
+        token zeros, and a block table of the cache's shape, of which the rows of these requests' seats are set.  Pages
+        that no token of a portion sees (``window``, ``chunk``, ``keep_first`` as in :meth:`attention`) are left out.  Needs
+        ``step.portions``."""
+        raise NotImplementedError
 
     def qkv_norm_write(self, qkv, bias, step: StepTensors, kv: KvSlot | None, rotary: RotaryTable | None,
                        num_heads: int, num_kv_heads: int, head_dim: int, value_dim: int, norm_eps: float | None,

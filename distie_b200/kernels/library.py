@@ -124,6 +124,15 @@ _SIGNATURES: dict[str, tuple[str, list]] = {
     "distie_latent_attention_tiles": ("latent", [P, P, P, I, I, I, I, P, I, P, P, P, P, I, P, I, I, F, I, P, P, P]),
     "distie_latent_gate": ("latent", [P, I, I, I, P, I, I, L, P, I, I, P]),
     "distie_glu_act": ("latent", [P, I, I, L, I, I, I, F, F, F, P, I, I, L, P, I, I, P]),
+    "distie_rows_write": (
+        "cached", [P, I, P, I, P, I, I, I, L, P, P, P, I, F, P, P, P, I, I, F, F, F, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I,
+                   P, I, I, I, P, P]
+    ),
+    "distie_rows_read": ("cached", [P, I, P, P, P, P, P, I, P, I, I, I, I, I, P, P, P, I, I, I, P, P]),
+    "distie_attention_rows_scratch_floats": ("cached", [I, I, I, I]),
+    "distie_attention_rows": (
+        "cached", [P, I, P, I, P, P, P, P, P, P, I, I, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, F, P, I, I, I, P, P]
+    ),
     "distie_gated_rmsnorm": ("state", [P, I, P, I, I, L, P, I, P, I, I, I, I, F, I, I, P]),
     "distie_gemm_tcgen05": ("bf16", [P, I, P, P, I, I, I, I, I, I, I, P, P]),
     "distie_gemm_tcgen05_act": ("bf16", [P, I, P, P, I, I, I, I, I, I, I, F, F, I, P, P]),
@@ -138,7 +147,7 @@ _SIGNATURES: dict[str, tuple[str, list]] = {
 _RESULT = {"distie_gemm_float32_scratch_floats": c_longlong, "distie_attention_prefill_pairs_scratch_floats": c_longlong, "distie_retention_scratch_floats": c_longlong, "distie_recurrence_chunks_scratch_floats": c_longlong,
            "distie_exp_gate_scratch_floats": c_longlong, "distie_attention_decode_scratch_floats": c_longlong, "distie_route_plan_words": c_longlong,
            "distie_latent_attention_scratch_floats": c_longlong, "distie_selective_scan_scratch_floats": c_longlong,
-           "distie_channel_delta_scratch_floats": c_longlong}
+           "distie_channel_delta_scratch_floats": c_longlong, "distie_attention_rows_scratch_floats": c_longlong}
 
 _libraries: dict[str, ctypes.CDLL] = {}
 _functions: dict[str, object] = {}
