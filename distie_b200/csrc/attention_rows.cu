@@ -186,28 +186,71 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   }
 }
 
-// Joins the parts of a (token, head): a block each, a thread per column; the order of the additions is that of the splits.
+// Joins the parts of a (token, head): a block each.  A row of parts takes a group of threads, four columns a thread, and
+// the groups share out the splits, so that the loads of many of them are in flight together; the order of the additions
+// follows from the number of splits alone.
+constexpr int kMergeThreads = 256;
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-attention_rows_merge_kernel(Partials parts, T* __restrict__ out, int out_stride, int num_heads, int value_dim,
-                            const float* __restrict__ sink) {
-  const int token = blockIdx.x, head = blockIdx.y;
-  const size_t row0 = ((size_t)token * num_heads + head) * parts.splits;
+__global__ void __launch_bounds__(kMergeThreads)
+attention_rows_merge_kernel(Partials parts, T* __restrict__ out, int out_stride, int value_dim, const float* __restrict__ sink) {
+  __shared__ float sh_acc[kMergeThreads][4];
+  __shared__ float sh_l[kMergeThreads];
+  __shared__ float sh_max[kMergeThreads / 32];
+  grid_dependency_release();
+  grid_dependency_wait();
+  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const size_t row0 = ((size_t)token * gridDim.y + head) * parts.splits;
+  const int per_row = (value_dim + 3) / 4, groups = kMergeThreads / per_row;  // up to 64 threads, at least 4 groups
+  const int mine = threadIdx.x / per_row, column = threadIdx.x % per_row * 4;
   float m_all = -INFINITY;
-  for (int s = 0; s < parts.splits; ++s) m_all = fmaxf(m_all, parts.ml[(row0 + s) * 2]);
-  float l_all = 0.f, acc = 0.f;
-  for (int s = 0; s < parts.splits; ++s) {
-    const float m = parts.ml[(row0 + s) * 2];
-    // (a part without a key has m = -inf and l = 0; one whose scores are all NaN has m = -inf and l = NaN)
-    const float l = parts.ml[(row0 + s) * 2 + 1];
-    const float weight = m == -INFINITY ? (l == 0.f ? 0.f : l) : exp2f(m - m_all);
-    l_all += l * weight;
-    if ((int)threadIdx.x < value_dim && l != 0.f) acc += parts.o[(row0 + s) * value_dim + threadIdx.x] * weight;
+  for (int s = threadIdx.x; s < parts.splits; s += kMergeThreads) m_all = fmaxf(m_all, __ldcg(parts.ml + (row0 + s) * 2));
+  m_all = warp_max(m_all);
+  if (lane == 0) sh_max[warp] = m_all;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; ++w) m_all = fmaxf(m_all, sh_max[w]);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l_mine = 0.f;
+  if (mine < groups) {
+#pragma unroll 4
+    for (int s = mine; s < parts.splits; s += groups) {
+      const float m = __ldcg(parts.ml + (row0 + s) * 2), l = __ldcg(parts.ml + (row0 + s) * 2 + 1);
+      // (a part without a key has a sum of 0, one whose scores are all NaN a sum of NaN; both have no maximum)
+      const float weight = m == -INFINITY ? l : exp2f(m - m_all);
+      l_mine += l * weight;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (column + e < value_dim) acc[e] += __ldcg(parts.o + (row0 + s) * value_dim + column + e) * weight;
+    }
   }
-  if ((int)threadIdx.x < value_dim) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sh_acc[threadIdx.x][e] = acc[e];
+  if (column == 0) sh_l[mine] = l_mine;
+  __syncthreads();
+  if (threadIdx.x < per_row) {
+    float l_all = 0.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < groups; ++r) {
+      l_all += sh_l[r];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += sh_acc[r * per_row + threadIdx.x][e];
+    }
     const float inv = sink ? sink_inverse_log2(m_all, l_all, sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
-    out[(size_t)token * out_stride + (size_t)head * value_dim + threadIdx.x] = from_float<T>(acc * inv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (column + e < value_dim) out[(size_t)token * out_stride + (size_t)head * value_dim + column + e] = from_float<T>(sum[e] * inv);
   }
+}
+
+template <typename T>
+static int rows_merge(const Partials& parts, void* out, int out_stride, int tokens, int num_heads, int value_dim, const float* sink,
+                      cudaStream_t stream) {
+  return (int)launch_dependent(attention_rows_merge_kernel<T>, dim3(tokens, num_heads), dim3(kMergeThreads), 0, stream, parts, (T*)out, out_stride,
+                               value_dim, sink);
+}
+
+int rows_merge_bf16(const Partials& parts, void* out, int out_stride, int tokens, int num_heads, int value_dim, const float* sink,
+                    cudaStream_t stream) {
+  return rows_merge<__nv_bfloat16>(parts, out, out_stride, tokens, num_heads, value_dim, sink, stream);
 }
 
 }  // namespace distie
@@ -250,10 +293,7 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
     attention_rows_kernel<T, CACHE><<<grid, kRowsThreads, shared, stream>>>((const T*)q, q_stride, (T*)out, out_stride, rows, cache,   \
                                                                             parts, error);                                          \
     DISTIE_LAUNCH_CHECK();                                                                                                          \
-    if (splits > 1)                                                                                                                 \
-      attention_rows_merge_kernel<T><<<dim3(tokens, num_heads), 256, 0, stream>>>(parts, (T*)out, out_stride, num_heads, value_dim,    \
-                                                                                  sink);                                            \
-    DISTIE_LAUNCH_CHECK();                                                                                                          \
+    if (splits > 1) return rows_merge<T>(parts, out, out_stride, tokens, num_heads, value_dim, sink, stream);                          \
     return 0;                                                                                                                       \
   }
   if (dtype == DISTIE_BF16 && cache_type == DISTIE_E4M3) DISTIE_ROWS(__nv_bfloat16, DISTIE_E4M3)

@@ -129,4 +129,8 @@ struct Partials {
   int splits;
 };
 
+// Joins the parts of every (token, head) into 16-bit rows (attention_rows.cu).
+int rows_merge_bf16(const Partials& parts, void* out, int out_stride, int tokens, int num_heads, int value_dim, const float* sink,
+                    cudaStream_t stream);
+
 }  // namespace distie

@@ -151,6 +151,9 @@ class CachedRows:
                 raise KernelError(f"attention: a tree of 1 to {MOST_DRAFTED} new tokens a request with int32 masks [tokens, words] and "
                                   f"rows [{requests}, 3] is expected")
         group = num_heads // num_kv_heads
+        if tree is None and self._decode_e4m3(q, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first, softcap,
+                                              sink, tokens):
+            return
         blocks = requests * num_kv_heads * -(-most * group // 16)
         splits = max(1, min(4 * self.sm_count // blocks, step.max_kv_len // 64, 64))
         scratch = None
@@ -171,3 +174,31 @@ class CachedRows:
                 "attention_rows",
             )
         self._ran("attention_rows", 1 if splits == 1 else 2)
+
+    def _decode_e4m3(self, q, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first, softcap, sink,
+                     tokens: int) -> bool:
+        """Single tokens on the tensor cores (attention_decode_e4m3.cu); False for sizes and alignments that the kernel does not take."""
+        if self.dtype != torch.bfloat16 or head_dim not in (64, 128) or kv.v.shape[-1] != head_dim:
+            return False
+        blocks = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 16)
+        seen = min(step.max_kv_len, window or chunk or step.max_kv_len)
+        splits = max(1, min(3 * self.sm_count // blocks, seen // 256, 64))
+        if splits <= 12:
+            splits = min(splits, 8)  # joined inside the kernel, by a cluster of CTAs
+        scratch = None
+        if splits > 8:
+            floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, head_dim, splits)
+            scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        with self._here():
+            code = function("distie_attention_decode_e4m3")(
+                q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
+                step.token_seq.data_ptr(), step.seq_seat.data_ptr(), tokens, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(),
+                kv.v_scale.data_ptr(), kv.block_table.data_ptr(), kv.block_table.shape[-1], num_heads, num_kv_heads, head_dim,
+                kv.page_size, kv.num_pages, window, chunk, keep_first, float(scale), softcap, _ptr(sink), splits,
+                self.error_flag.data_ptr(), self._stream(),
+            )
+        if code == -2:
+            return False
+        check(code, "attention_decode_e4m3")
+        self._ran("attention_decode_e4m3", 1 if splits <= 8 else 2)
+        return True

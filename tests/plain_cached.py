@@ -121,6 +121,16 @@ class Case:
             first = torch.maximum(first, mine // chunk * chunk)
         return seen & ((place[None, :] >= first[:, None]) | (place[None, :] < (keep_first if window else 0)))
 
+    def reach(self, q, heads, scale):
+        """The largest sum of magnitudes behind any score, [tokens, heads * value size]: what its float32 sum is rounded relative to."""
+        out = []
+        for r in range(len(self.news)):
+            k = self.held("k", r).repeat_interleave(heads // self.kv_heads, 0).abs()
+            mine = q[self.starts[r] : self.starts[r] + self.news[r], : heads * self.dim].double().cpu().abs()
+            s = mine.reshape(self.news[r], heads, self.dim).transpose(0, 1) @ k.transpose(1, 2) * scale
+            out.append(s.amax(-1).transpose(0, 1).repeat_interleave(self.value_dim, 1))
+        return torch.cat(out)
+
     def attention(self, q, heads, scale, window=None, chunk=None, keep_first=0, softcap=0.0, sink=None):
         """(output, sum of weight times magnitude of the values), 64 bits, both [tokens, heads * value size]."""
         outs, sizes = [], []
