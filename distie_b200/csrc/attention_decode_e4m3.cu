@@ -496,7 +496,7 @@ extern "C" int distie_attention_decode_e4m3(const void* q, int q_stride, void* o
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, head_dim, head_dim,
                                       page_size, num_pages);
   const int group = num_heads / num_kv_heads, chunks = (group + 15) / 16;
-  const QueryRows rows{positions, token_seq, seq_seat, nullptr, nullptr, 1, group, num_heads, window, chunk, keep_first,
+  const QueryRows rows{positions, token_seq, seq_seat, nullptr, nullptr, 1, tokens, group, num_heads, window, chunk, keep_first,
                        scale * 1.4426950408889634f, make_score_extras(scale, softcap, sink)};
   const Partials parts{scratch, scratch ? scratch + (size_t)tokens * num_heads * splits * head_dim : nullptr, splits};
   const int cluster_merge = splits > 1 && splits <= kDecClusterSplits;

@@ -278,7 +278,7 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
     return DISTIE_ERR_ARG;
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, key_dim, value_dim,
                                       page_size, num_pages);
-  const QueryRows rows{positions, token_seq, seq_seat, seqs, bits, words, num_heads / num_kv_heads, num_heads, window, chunk, keep_first,
+  const QueryRows rows{positions, token_seq, seq_seat, seqs, bits, words, tokens, num_heads / num_kv_heads, num_heads, window, chunk, keep_first,
                        scale * 1.4426950408889634f, make_score_extras(scale, softcap, sink)};
   const Partials parts{scratch, scratch ? scratch + (size_t)tokens * num_heads * splits * value_dim : nullptr, splits};
   const int tiles = (most_nodes * rows.group + kRowsTile - 1) / kRowsTile;

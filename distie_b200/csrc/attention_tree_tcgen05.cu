@@ -1,0 +1,673 @@
+// Attention of drafted tokens over the paged cache on the 5th-generation tensor cores: 16-bit queries, a cache in 16 or 8
+// bits, heads of 64 and 128.
+//
+// The new tokens of a request see the same cached keys, so their rows share one pass over them: row r of a request and kv
+// head is head r % group of new token r / group, and a CTA takes up to 128 rows and a share of the keys in blocks of 128.
+//
+//   S = Q K^T        tcgen05.mma, M = 128 rows, N = 128 keys; S in tensor memory, two buffers of 128 columns
+//   P = softmax      eight warps in two groups of four: group 0 owns keys 0..63 of every block, group 1 keys 64..127, a thread
+//                    per row in each, two softmax streams that meet at the end.  P goes back over the group's columns of S
+//                    as 16-bit numbers, two keys to a column.  Warps whose rows are all empty take no part.
+//   O_g += P_g V_g   tcgen05.mma with P as the A operand straight from tensor memory
+//
+// Loaders bring K and V through registers (seven warps, 16 bytes a thread and load; V of a block is requested while its K is
+// stored, and the next K while V is): pages of any size, rows in any order of
+// pages.  Of a 16-bit cache they store what they loaded; of an 8-bit one they turn e4m3 numbers into float16, which holds
+// them exactly, so that Q (times a power of two a row, float16), K, P and V are float16 there and bfloat16 here.  The
+// scales of the rows go beside the tiles: s^k multiplies the finished score, and p s^v is one exponential,
+// exp2(score + log2 s^v - m'), with a running maximum m' of its own (attention_decode_e4m3.cu says why).
+//
+// Masks: a block that lies before every row's new tokens and inside every row's window needs none; the others get 64 bits a
+// row and group.  A masked weight is 0, and 0 * (what is not finite) is not 0: in blocks that need masks, values that are not
+// finite are stored as zeros, and the rows that see them get them back at the end, element by element (8-bit rows carry
+// NaN in their scales, which masks reach).  Rows of keys that belong to nobody are zeros.
+//
+// Running maxima are raised only when exceeded by more than 8 (base 2), so O is read, scaled and written back rarely.
+// With several shares of the keys, the parts go to scratch in float32 and attention_rows.cu joins them.
+//
+//   warps 0..7    softmax, end        warp 8   tensor memory, MMA issue        warps 9..15   loaders
+//
+// Every wait on an mbarrier is bounded; when one runs out the CTA sets the error word to 6 and every role stops at its
+// next wait.
+#include <cuda_fp16.h>
+
+#include "cached_rows.cuh"
+#include "softmax_pairs.cuh"
+#include "tcgen05.cuh"
+
+namespace distie {
+
+constexpr int kTreeRows = 128;
+constexpr int kTreeKeys = 128;
+constexpr int kTreeGroupKeys = 64;
+constexpr int kTreeMmaWarp = 8;
+constexpr int kTreeLoadWarp = 9;
+constexpr int kTreeLoaders = 7 * 32;  // threads
+constexpr int kTreeThreads = 32 * 16;
+constexpr int kTreeKStages = 2, kTreeVStages = 3, kTreeScaleSlots = 4;
+constexpr int kTreeHalf = kTreeRows * 128;  // bytes of one [128 rows x 64 elements] swizzled half tile
+constexpr int kTreeMostNodes = 256;
+constexpr float kTreeRaise = 8.f;
+
+template <int D>
+struct TreeShared {
+  alignas(1024) unsigned char q[kTreeRows * D * 2];
+  alignas(1024) unsigned char k[kTreeKStages][kTreeKeys * D * 2];
+  alignas(1024) unsigned char v[kTreeVStages][kTreeKeys * D * 2];
+  float k_scale[kTreeScaleSlots][kTreeKeys];  // of the keys of a block
+  float v_log[kTreeScaleSlots][kTreeKeys];    // log2 of the values' scales
+  float q_times[kTreeRows];                   // what turns a row's raw products into scores, before the keys' scales
+  int node_position[kTreeMostNodes];
+  uint64_t q_full;
+  uint64_t k_full[kTreeKStages], k_empty[kTreeKStages];
+  uint64_t v_full[kTreeVStages], v_empty[kTreeVStages];
+  uint64_t scale_full[kTreeScaleSlots];
+  uint64_t s_full[2];
+  uint64_t p_full[2][2];  // [group][S buffer]
+  uint64_t pv_done[2];    // [group]
+  uint64_t merge_ready;
+  float row_max[2][kTreeRows], row_sum[2][kTreeRows], row_out[2][kTreeRows];
+  uint32_t tmem_base;
+  uint32_t failed;
+  uint32_t bad;  // a masked block holds a value that is not finite
+};
+
+// The blocks of 128 keys that a tile of rows walks: those of the kept first keys, then those from the window's start on.
+struct TreeSpan {
+  int past, keys;       // cached keys, and all of them
+  int oldest, newest;   // oldest key that any row's window holds; oldest one that every row's window holds
+  int kept;             // first keys that stay visible before `oldest`
+  int kept_blocks, start, blocks;
+
+  __device__ __forceinline__ int key0(int j) const { return j < kept_blocks ? j * kTreeKeys : start + (j - kept_blocks) * kTreeKeys; }
+  __device__ __forceinline__ int key_end(int j) const { return j < kept_blocks ? min(kept, start) : keys; }
+  // Whether every row of the tile sees every key of the block.
+  __device__ __forceinline__ bool whole(int j) const {
+    return j >= kept_blocks && key0(j) >= newest && key0(j) + kTreeKeys <= past;
+  }
+};
+
+__device__ __forceinline__ uint32_t tree_offset(int row, int piece) {  // of 8 elements of a row in a tile of swizzled halves
+  return (uint32_t)((piece >> 3) * kTreeHalf + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float tree_log2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two 16-bit bfloat16 numbers of which some are not finite: those become zeros.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t x, bool& bad) {
+  uint32_t keep = 0xffffffffu;
+  if ((x & 0x7f80u) == 0x7f80u) keep &= 0xffff0000u;
+  if ((x & 0x7f800000u) == 0x7f800000u) keep &= 0x0000ffffu;
+  bad |= keep != 0xffffffffu;
+  return x & keep;
+}
+
+template <int D, bool E4M3>
+__global__ void __launch_bounds__(kTreeThreads, 1)
+attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride, QueryRows rows,
+                              CachePages cache, Partials parts, int* __restrict__ error) {
+  extern __shared__ unsigned char raw_shared[];
+  auto& sm = *reinterpret_cast<TreeShared<D>*>((reinterpret_cast<uintptr_t>(raw_shared) + 1023) & ~uintptr_t(1023));
+  constexpr uint32_t TMEM_COLS = D == 128 ? 512 : 512, O_COL = 256;  // S0 | S1 | O of group 0 | O of group 1
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile uint32_t* failed = &sm.failed;
+
+  const int split = blockIdx.z;
+  const int kv_head = blockIdx.x % cache.num_kv_heads, tile = blockIdx.x / cache.num_kv_heads;
+  const Request request = request_of(rows, blockIdx.y);
+  const int row0 = tile * kTreeRows, count = min(kTreeRows, request.nodes * rows.group - row0);
+  if (count <= 0) return;
+  const int active = (count + 31) / 32;  // warps of a softmax group that have rows
+  const int* table = cache.block_table + (size_t)request.seat * cache.table_width;
+
+  grid_dependency_release();
+  TreeSpan span;
+  {
+    int low = 0x7fffffff, high = 0;
+    const int node0 = row0 / rows.group, node1 = (row0 + count - 1) / rows.group;
+    for (int n = node0 + lane; n <= node1; n += 32) {
+      const int first = first_visible_key(rows.positions[request.first + n], rows.window, rows.chunk);
+      low = min(low, first);
+      high = max(high, first);
+    }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+      low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
+      high = max(high, __shfl_xor_sync(0xffffffffu, high, d));
+    }
+    span.past = request.past;
+    span.keys = request.past + request.nodes;
+    span.oldest = min(low, request.past);  // (all new tokens' keys are walked)
+    span.newest = high;
+    span.kept = min(rows.keep_first, span.oldest);
+    span.kept_blocks = (span.kept + kTreeKeys - 1) / kTreeKeys;
+    span.start = span.oldest / kTreeKeys * kTreeKeys;
+    span.blocks = span.kept_blocks + (span.keys - span.start + kTreeKeys - 1) / kTreeKeys;
+  }
+  const int share = (span.blocks + parts.splits - 1) / parts.splits;
+  const int block0 = min(span.blocks, split * share), block1 = min(span.blocks, block0 + share);
+  const int blocks = block1 - block0;
+  if (blocks == 0) {  // a share without keys: its parts count nothing
+    grid_dependency_wait();
+    for (int r = warp; r < count; r += kTreeThreads / 32) {
+      const int token = request.first + (row0 + r) / rows.group, head = kv_head * rows.group + (row0 + r) % rows.group;
+      const size_t at = ((size_t)token * rows.num_heads + head) * parts.splits + split;
+      for (int e = lane; e < D; e += 32) parts.o[at * D + e] = 0.f;
+      if (lane == 0) {
+        parts.ml[2 * at] = -INFINITY;
+        parts.ml[2 * at + 1] = 0.f;
+      }
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.q_full, kTreeMmaWarp);
+    for (int s = 0; s < kTreeKStages; ++s) {
+      mbar_init(&sm.k_full[s], kTreeLoaders / 32);
+      mbar_init(&sm.k_empty[s], 1);
+    }
+    for (int s = 0; s < kTreeVStages; ++s) {
+      mbar_init(&sm.v_full[s], kTreeLoaders / 32);
+      mbar_init(&sm.v_empty[s], 1);
+    }
+    for (int s = 0; s < kTreeScaleSlots; ++s) mbar_init(&sm.scale_full[s], kTreeLoaders / 32);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sm.s_full[b], 1);
+      mbar_init(&sm.p_full[0][b], active);
+      mbar_init(&sm.p_full[1][b], active);
+      mbar_init(&sm.pv_done[b], 1);
+    }
+    mbar_init(&sm.merge_ready, 2 * active);
+    sm.failed = 0;
+    sm.bad = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kTreeMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  for (int n = threadIdx.x; n < request.nodes && n < kTreeMostNodes; n += kTreeThreads)
+    sm.node_position[n] = rows.positions[request.first + n];
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = sm.tmem_base;
+  grid_dependency_wait();  // q and the newest rows come from the kernels before this one
+
+  if (warp >= kTreeLoadWarp) {
+    // ---- loaders: 16 bytes of a row per thread and load --------------------------------------------------------------
+    constexpr int PPR = E4M3 ? D / 16 : D / 8;  // pieces of a row
+    constexpr int ALL = kTreeKeys * PPR;        // of a tile
+    constexpr int PIECES = (ALL + kTreeLoaders - 1) / kTreeLoaders;  // of a tile, per thread
+    const int thread = threadIdx.x - kTreeLoadWarp * 32;
+    auto fetch = [&](uint4 (&raw)[PIECES], float (&scale)[PIECES], const void* rows_at, const float* scales_at, int j) {
+      if (j >= block1) return;
+      const int key0 = span.key0(j), key_end = span.key_end(j);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int p = thread + i * kTreeLoaders, key = key0 + p / PPR;
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        scale[i] = 0.f;
+        if (p < ALL && key < key_end && (key >= span.oldest || key < span.kept)) {
+          const long long at = cache.row_of(table, key, kv_head);
+          if (at < 0) {
+            if (error) atomicExch(error, 8);
+          } else {
+            raw[i] = load16_cg(reinterpret_cast<const unsigned char*>(rows_at) + (size_t)at * (PPR * 16) + p % PPR * 16);
+            if (E4M3 && p % PPR == 0) scale[i] = __ldcg(scales_at + at);
+          }
+        }
+      }
+    };
+    auto put = [&](unsigned char* tile_at, const uint4 (&raw)[PIECES]) {
+      const uint32_t base = smem_u32(tile_at);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int p = thread + i * kTreeLoaders, row = p / PPR, piece = p % PPR;
+        if (p >= ALL) break;
+        const uint4& x = raw[i];
+        if (E4M3) {
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            h[2 * e] = e4m3x2_to_half2((uint16_t)(w[e] & 0xffffu));
+            h[2 * e + 1] = e4m3x2_to_half2((uint16_t)(w[e] >> 16));
+          }
+          store_shared16(base + tree_offset(row, 2 * piece), h[0], h[1], h[2], h[3]);
+          store_shared16(base + tree_offset(row, 2 * piece + 1), h[4], h[5], h[6], h[7]);
+        } else {
+          store_shared16(base + tree_offset(row, piece), x.x, x.y, x.z, x.w);
+        }
+      }
+    };
+    auto put_scales = [&](float* scales_at, const float (&scale)[PIECES], bool as_log) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int p = thread + i * kTreeLoaders;
+        if (p < ALL && p % PPR == 0) scales_at[p / PPR] = as_log ? tree_log2(scale[i]) : scale[i];
+      }
+    };
+    auto ready = [&](uint64_t* bar) {  // this warp's stores are in shared memory, for the tensor cores and for other warps
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_unless(bar, parity, failed)) != 0; };
+    uint4 k_raw[PIECES], v_raw[PIECES];
+    float k_scale[PIECES], v_scale[PIECES];
+    bool ok = true;
+    fetch(k_raw, k_scale, cache.k, cache.k_scale, block0);
+    fetch(v_raw, v_scale, cache.v, cache.v_scale, block0);
+    for (int j = block0; j < block1; ++j) {
+      const int n = j - block0, ks = n % kTreeKStages, vs = n % kTreeVStages, slot = n % kTreeScaleSlots;
+      // The slot's last scales are read: the S of two blocks ago, whose K this stage held, was issued behind their P.
+      if (!wait(&sm.k_empty[ks], ((n / kTreeKStages) & 1) ^ 1)) { ok = false; break; }
+      put(sm.k[ks], k_raw);
+      if (E4M3) put_scales(sm.k_scale[slot], k_scale, false);
+      ready(&sm.k_full[ks]);
+      fetch(k_raw, k_scale, cache.k, cache.k_scale, j + 1);
+      if (E4M3) {
+        put_scales(sm.v_log[slot], v_scale, true);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.scale_full[slot]);
+      }
+      if (!wait(&sm.v_empty[vs], ((n / kTreeVStages) & 1) ^ 1)) { ok = false; break; }
+      if (!E4M3 && !span.whole(j)) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          v_raw[i].x = finite_pair(v_raw[i].x, bad);
+          v_raw[i].y = finite_pair(v_raw[i].y, bad);
+          v_raw[i].z = finite_pair(v_raw[i].z, bad);
+          v_raw[i].w = finite_pair(v_raw[i].w, bad);
+        }
+        if (bad) atomicExch(&sm.bad, 1u);
+      }
+      put(sm.v[vs], v_raw);
+      ready(&sm.v_full[vs]);
+      fetch(v_raw, v_scale, cache.v, cache.v_scale, j + 1);
+    }
+    if (!ok) atomicExch(&sm.failed, 1u);
+  } else if (warp == kTreeMmaWarp) {
+    // ---- MMA issuer ----------------------------------------------------------------------------------------------------
+    if (lane == 0) {
+      constexpr uint32_t type = E4M3 ? 0u : (1u << 7) | (1u << 10);  // float16 or bfloat16 operands
+      constexpr uint32_t idesc_s = (1u << 4) | type | ((uint32_t)(kTreeKeys >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+      const uint64_t q_desc = smem_desc(sm.q);
+      bool ok = mbar_wait_unless(&sm.q_full, 0, failed);
+      auto issue_s = [&](int n) {
+        const int s = n & 1, ks = n % kTreeKStages;
+        if (!mbar_wait_unless(&sm.k_full[ks], (n / kTreeKStages) & 1, failed)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t k_desc = smem_desc(sm.k[ks]);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t step = (uint64_t)(((kk >> 2) * kTreeHalf + (kk & 3) * 32) >> 4);
+          umma_bf16(tmem + s * kTreeKeys, q_desc + step, k_desc + step, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        umma_commit(&sm.k_empty[ks]);
+        umma_commit(&sm.s_full[s]);
+        return true;
+      };
+      ok = ok && issue_s(0);
+      if (ok && blocks > 1) ok = issue_s(1);
+      for (int n = 0; n < blocks && ok; ++n) {
+        const int s = n & 1, vs = n % kTreeVStages;
+        if (!mbar_wait_unless(&sm.v_full[vs], (n / kTreeVStages) & 1, failed)) { ok = false; break; }
+        const uint64_t v_desc = smem_desc_mn(sm.v[vs], kTreeHalf, 1024);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (!mbar_wait_unless(&sm.p_full[g][s], (n >> 1) & 1, failed)) { ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+          for (int kk = 0; kk < kTreeGroupKeys / 16; ++kk) {
+            const uint64_t v_step = (uint64_t)(((g * kTreeGroupKeys + kk * 16) * 128) >> 4);
+            umma_bf16_ts(tmem + O_COL + g * D, tmem + s * kTreeKeys + g * kTreeGroupKeys + kk * 8, v_desc + v_step, idesc_o,
+                         (n > 0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&sm.pv_done[g]);
+        }
+        if (!ok) break;
+        umma_commit(&sm.v_empty[vs]);
+        if (n + 2 < blocks) ok = issue_s(n + 2);
+      }
+      if (!ok) atomicExch(&sm.failed, 1u);
+    }
+  } else {
+    // ---- queries into shared memory: a warp takes 16 rows ---------------------------------------------------------------
+    {
+      constexpr int PER_LANE = D / 32;  // 4 or 2 elements
+      const float unit_times = rows.extras.cap > 0.f ? rows.extras.cap_pre : rows.scale_log2;
+      uint2 x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = warp * 16 + i;
+        x[i] = make_uint2(0u, 0u);
+        if (r < count) {
+          const int token = request.first + (row0 + r) / rows.group, head = kv_head * rows.group + (row0 + r) % rows.group;
+          const __nv_bfloat16* from = q + (size_t)token * q_stride + (size_t)head * D + lane * PER_LANE;
+          if (PER_LANE == 4) x[i] = __ldcg(reinterpret_cast<const uint2*>(from));
+          else x[i].x = __ldcg(reinterpret_cast<const unsigned int*>(from));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = warp * 16 + i;
+        uint32_t a = x[i].x, b = x[i].y;
+        if (E4M3) {  // times a power of two that brings the row's largest element to [1, 2): float16 then holds it
+          const float f[4] = {__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)};
+          const float most = warp_max(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))));
+          const int exponent = most > 0.f ? min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126) : 0;
+          const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
+          const __half2 lo = __floats2half2_rn(f[0] * down, f[1] * down), hi = __floats2half2_rn(f[2] * down, f[3] * down);
+          a = *reinterpret_cast<const uint32_t*>(&lo);
+          b = *reinterpret_cast<const uint32_t*>(&hi);
+          if (lane == 0) sm.q_times[r] = __uint_as_float((uint32_t)(127 + exponent) << 23) * unit_times;
+        }
+        const uint32_t at = smem_u32(sm.q) + tree_offset(r, lane * PER_LANE / 8) + (lane * PER_LANE % 8) * 2;
+        if (PER_LANE == 4) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
+        else asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(a) : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full);
+    }
+    // ---- softmax, correction of O, end: group g owns 64 keys of every block, thread = row ---------------------------------
+    const int quadrant = warp & 3, g = warp >> 2, r = quadrant * 32 + lane;
+    if (quadrant < active) {
+      const uint32_t lane_base = tmem + ((uint32_t)(quadrant * 32) << 16);
+      const uint32_t o_addr = lane_base + O_COL + g * D;
+      bool ok = true;
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) {  // one lane polls
+        int done = 1;
+        if (lane == 0) done = mbar_wait_unless(bar, parity, failed) ? 1 : 0;
+        done = __shfl_sync(0xffffffffu, done, 0);
+        __syncwarp();
+        return done != 0;
+      };
+      const bool live = r < count;
+      const int node = live ? (row0 + r) / rows.group : 0, head = kv_head * rows.group + (live ? (row0 + r) % rows.group : 0);
+      const int token = request.first + node;
+      const int first = first_visible_key(rows.positions[token], rows.window, rows.chunk);
+      const int* bits = rows.bits + (size_t)token * rows.words;
+      auto seen = [&](int key, int key_end) {
+        if (!live || key >= key_end) return false;
+        int place = key;
+        if (key >= span.past) {
+          const int n = key - span.past;
+          if (!((__ldg(bits + (n >> 5)) >> (n & 31)) & 1)) return false;
+          place = sm.node_position[n];
+        }
+        return place >= first || place < rows.keep_first;
+      };
+      // The keys of [key0, key0 + 64) that the row sees, a bit each.
+      auto seen64 = [&](int key0, int key_end) {
+        uint64_t mask = 0;
+        if (!live) return mask;
+        if (first == 0) {  // no window has moved: cached keys, then the row's mask
+          const int cached = min(max(span.past - key0, 0), 64);
+          if (cached > 0) mask = cached == 64 ? ~0ull : (1ull << cached) - 1;
+          const int skip = max(key0 - span.past, 0);  // new tokens before key0
+          const int there = min(64 - cached, key_end - max(key0, span.past));
+          if (there > 0) {
+            const int word = skip >> 5, shift = skip & 31;
+            auto load = [&](int w) { return w < rows.words ? (uint32_t)__ldg(bits + w) : 0u; };
+            const uint32_t w0 = load(word), w1 = load(word + 1), w2 = load(word + 2);
+            uint64_t draft = (uint64_t)__funnelshift_r(w0, w1, shift) | ((uint64_t)__funnelshift_r(w1, w2, shift) << 32);
+            if (there < 64) draft &= (1ull << there) - 1;
+            mask |= draft << cached;  // (cached < 64 here)
+          }
+        } else {
+          for (int i = 0; i < 64; ++i)
+            if (seen(key0 + i, key_end)) mask |= 1ull << i;
+        }
+        return mask;
+      };
+      ok = wait_all(&sm.q_full, 0);
+      const float times = E4M3 ? sm.q_times[r] : (rows.extras.cap > 0.f ? rows.extras.cap_pre : rows.scale_log2);
+      const float cap = rows.extras.cap * 1.4426950408889634f;
+      float m_used = -INFINITY, o_used = -INFINITY, l = 0.f;  // o_used: the maximum that P is taken with, of scores with the values' scales
+      for (int n = 0; n < blocks && ok; ++n) {
+        const int j = block0 + n, s = n & 1, slot = n % kTreeScaleSlots;
+        const int key0 = span.key0(j) + g * kTreeGroupKeys;
+        const uint32_t s_addr = lane_base + s * kTreeKeys + g * kTreeGroupKeys;
+        const bool whole = span.whole(j);
+        const uint64_t mask = whole ? ~0ull : seen64(key0, span.key_end(j));
+        if (E4M3 && !wait_all(&sm.scale_full[slot], (n / kTreeScaleSlots) & 1)) { ok = false; break; }
+        if (!wait_all(&sm.s_full[s], (n >> 1) & 1)) { ok = false; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        uint32_t sv[kTreeGroupKeys];
+        tmem_load_64(s_addr, sv);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        const float* k_scale = &sm.k_scale[slot][g * kTreeGroupKeys];
+        const float* v_log = &sm.v_log[slot][g * kTreeGroupKeys];
+        float mx = -INFINITY, ox = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kTreeGroupKeys; i += 4) {
+          float4 ks = make_float4(1.f, 1.f, 1.f, 1.f), vl = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (E4M3) {
+            ks = *reinterpret_cast<const float4*>(k_scale + i);
+            vl = *reinterpret_cast<const float4*>(v_log + i);
+          }
+          const float kk[4] = {ks.x, ks.y, ks.z, ks.w}, vv[4] = {vl.x, vl.y, vl.z, vl.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = __uint_as_float(sv[i + e]) * (E4M3 ? times * kk[e] : times);
+            if (rows.extras.cap > 0.f) x = cap * (1.f - __fdividef(2.f, exp2_approx(x * 2.8853900817779268f) + 1.f));
+            if (!whole && !((mask >> (i + e)) & 1)) x = -INFINITY;
+            sv[i + e] = __float_as_uint(x);
+            mx = fmaxf(mx, x);
+            if (E4M3) ox = fmaxf(ox, x == -INFINITY ? x : x + vv[e]);
+          }
+        }
+        // The maximum in use for the sum, and the one for O (of a 16-bit cache they are one).
+        const float m_new = fmaxf(m_used, mx);
+        const bool raise_sum = m_new > m_used + kTreeRaise || (m_used == -INFINITY && m_new > -INFINITY);
+        float corr = 1.f;
+        if (raise_sum) {
+          corr = exp2_approx(m_used - m_new);
+          l *= corr;
+          m_used = m_new;
+        }
+        bool raise = raise_sum;
+        if (E4M3) {
+          const float o_new = fmaxf(o_used, ox);
+          raise = o_new > o_used + kTreeRaise || (o_used == -INFINITY && o_new > -INFINITY);
+          corr = 1.f;
+          if (raise) {
+            corr = exp2_approx(o_used - o_new);
+            o_used = o_new;
+          }
+        }
+        // The group's O is in use by its product of the block before this one until that has completed.
+        if (n > 0 && __any_sync(0xffffffffu, raise)) {
+          if (!wait_all(&sm.pv_done[g], (n - 1) & 1)) { ok = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+          for (int c0 = 0; c0 < D; c0 += 32) {
+            uint32_t v[32];
+            tmem_load_32(o_addr + c0, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+            tmem_store_32(o_addr + c0, v);
+          }
+        }
+        const float shift = m_used == -INFINITY ? 0.f : m_used, out_shift = o_used == -INFINITY ? 0.f : o_used;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float4 vl = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (E4M3) vl = *reinterpret_cast<const float4*>(v_log + half * 32 + i);
+            const float vv[4] = {vl.x, vl.y, vl.z, vl.w};
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = __uint_as_float(sv[half * 32 + i + e]);
+              const float p = exp2_approx(x - shift);
+              if (E4M3) {
+                sum[e & 1] += p;
+                w[e] = x == -INFINITY ? 0.f : exp2_approx(x + vv[e] - out_shift);
+              } else {
+                w[e] = p;
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              if (E4M3) {
+                const __half2 pair = __floats2half2_rn(w[e], w[e + 1]);
+                packed[(i + e) >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
+              } else {  // the sum is that of the weights as the product takes them
+                const __nv_bfloat162 pair = __floats2bfloat162_rn(w[e], w[e + 1]);
+                const uint32_t both = *reinterpret_cast<const uint32_t*>(&pair);
+                packed[(i + e) >> 1] = both;
+                sum[0] += __uint_as_float(both << 16);
+                sum[1] += __uint_as_float(both & 0xffff0000u);
+              }
+            }
+          }
+          tmem_store_16(s_addr + half * 16, packed);
+        }
+        l += sum[0] + sum[1];
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[g][s]);
+      }
+      if (!ok) atomicExch(&sm.failed, 1u);
+      // ---- end: the two groups' parts of a row at a common maximum -------------------------------------------------------
+      sm.row_max[g][r] = m_used;
+      sm.row_sum[g][r] = l;
+      sm.row_out[g][r] = E4M3 ? o_used : m_used;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.merge_ready);
+      if (ok && wait_all(&sm.merge_ready, 0) && wait_all(&sm.pv_done[0], (blocks - 1) & 1) && wait_all(&sm.pv_done[1], (blocks - 1) & 1)) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const float m_all = fmaxf(sm.row_max[0][r], sm.row_max[1][r]), at_most = m_all == -INFINITY ? 0.f : m_all;
+        float l_all = 0.f, f[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          // (no maximum: a sum of 0 without a key, of NaN where every score is NaN)
+          const float sum = sm.row_sum[u][r], weight = sm.row_max[u][r] == -INFINITY ? sum : exp2_approx(sm.row_max[u][r] - at_most);
+          l_all += sum * weight;
+          f[u] = sm.row_out[u][r] == -INFINITY ? sum - sum : exp2_approx(sm.row_out[u][r] - at_most);
+        }
+        const bool alone = parts.splits == 1;
+        float inv = 1.f;
+        if (alone) inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
+        const float f0 = f[0] * inv, f1 = f[1] * inv;
+        constexpr int SIDE = D / 2;  // group g writes columns g * D / 2 ... of the row, from both accumulators
+        const size_t part_row = ((size_t)token * rows.num_heads + head) * parts.splits + split;
+#pragma unroll 1
+        for (int c0 = 0; c0 < SIDE; c0 += 16) {
+          uint32_t a[16], b[16];
+          tmem_load_16(lane_base + O_COL + g * SIDE + c0, a);
+          tmem_load_16(lane_base + O_COL + D + g * SIDE + c0, b);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          float y[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(a[i]) * f0 + __uint_as_float(b[i]) * f1;
+          if (!E4M3 && sm.bad) {  // values that are not finite, for the rows that see them
+            for (int j = block0; j < block1; ++j) {
+              if (span.whole(j)) continue;
+              for (int key = span.key0(j); key < span.key0(j) + kTreeKeys; ++key) {
+                if (!seen(key, span.key_end(j))) continue;
+                const long long at = cache.row_of(table, key, kv_head);
+                if (at < 0) continue;
+                const __nv_bfloat16* value = reinterpret_cast<const __nv_bfloat16*>(cache.v) + (size_t)at * D + g * SIDE + c0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float v = __bfloat162float(value[i]);
+                  if (!(fabsf(v) <= 3.402823466e38f)) y[i] += v;
+                }
+              }
+            }
+          }
+          if (live && alone) {
+            __nv_bfloat16* to = out + (size_t)token * out_stride + (size_t)head * D + g * SIDE + c0;
+#pragma unroll
+            for (int i = 0; i < 16; i += 8) {
+              const float part[8] = {y[i], y[i + 1], y[i + 2], y[i + 3], y[i + 4], y[i + 5], y[i + 6], y[i + 7]};
+              store8(to + i, part);
+            }
+          } else if (live) {
+            float* to = parts.o + part_row * D + g * SIDE + c0;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) store4(to + i, make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
+          }
+        }
+        if (live && !alone && g == 0) {
+          parts.ml[2 * part_row] = m_all;
+          parts.ml[2 * part_row + 1] = l_all;
+        }
+      } else {
+        atomicExch(&sm.failed, 1u);
+      }
+    }
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == kTreeMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+  if (threadIdx.x == 0 && sm.failed && error) atomicCAS(error, 0, 6);
+}
+
+template <int D, bool E4M3>
+static int launch_tree(const dim3& grid, const __nv_bfloat16* q, int q_stride, __nv_bfloat16* out, int out_stride, const QueryRows& rows,
+                       const CachePages& cache, const Partials& parts, int* error, cudaStream_t stream) {
+  const size_t shared = sizeof(TreeShared<D>) + 1024;
+  auto kernel = attention_tree_tcgen05_kernel<D, E4M3>;
+  cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+  if (err != cudaSuccess) return (int)err;
+  return (int)launch_dependent(kernel, grid, dim3(kTreeThreads), shared, stream, q, q_stride, out, out_stride, rows, cache, parts, error);
+}
+
+}  // namespace distie
+
+using namespace distie;
+
+// Drafted tokens: q [tokens, >= heads * head_dim] and out [tokens, heads * head_dim] bfloat16, a cache of bfloat16 or (with
+// scales) e4m3, heads of 64 or 128 (else DISTIE_ERR_UNSUPPORTED, like rows that are not aligned to what a thread moves), at most
+// 256 new tokens a request.  seqs [requests, 3], bits [tokens, words].  scratch: distie_attention_rows_scratch_floats.
+extern "C" int distie_attention_tree_tcgen05(const void* q, int q_stride, void* out, int out_stride, float* scratch, const int* positions,
+                                             const int* seq_seat, const int* seqs, const int* bits, int words, int requests, int tokens,
+                                             int most_nodes, const void* k_cache, const void* v_cache, const float* k_scale,
+                                             const float* v_scale, const int* block_table, int table_width, int num_heads, int num_kv_heads,
+                                             int head_dim, int page_size, int num_pages, int window, int chunk, int keep_first, float scale,
+                                             float softcap, const float* sink, int splits, int* error, cudaStream_t stream) {
+  if (tokens <= 0 || requests <= 0) return 0;
+  if (num_heads < 1 || num_kv_heads < 1 || num_heads % num_kv_heads != 0 || page_size < 1 || table_width < 1 || keep_first < 0 || splits < 1 ||
+      splits > 65535 || requests > 65535 || most_nodes < 1 || most_nodes > kTreeMostNodes || words > kTreeMostNodes / 32 || words * 32 < most_nodes || seqs == nullptr ||
+      bits == nullptr || (splits > 1 && scratch == nullptr) || (k_scale == nullptr) != (v_scale == nullptr))
+    return DISTIE_ERR_ARG;
+  if ((head_dim != 64 && head_dim != 128) || (q_stride & 3) || ((uintptr_t)q & 7) || (out_stride & 7) || ((uintptr_t)out & 15) ||
+      (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15))
+    return DISTIE_ERR_UNSUPPORTED;
+  const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, head_dim, head_dim,
+                                      page_size, num_pages);
+  const int group = num_heads / num_kv_heads;
+  const QueryRows rows{positions, nullptr, seq_seat, seqs, bits, words, tokens, group, num_heads, window, chunk, keep_first,
+                       scale * 1.4426950408889634f, make_score_extras(scale, softcap, sink)};
+  const Partials parts{scratch, scratch ? scratch + (size_t)tokens * num_heads * splits * head_dim : nullptr, splits};
+  const dim3 grid((unsigned)(((long long)most_nodes * group + kTreeRows - 1) / kTreeRows * num_kv_heads), requests, splits);
+  int status;
+  if (head_dim == 64)
+    status = k_scale ? launch_tree<64, true>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts, error, stream)
+                     : launch_tree<64, false>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts, error, stream);
+  else
+    status = k_scale ? launch_tree<128, true>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts, error, stream)
+                     : launch_tree<128, false>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts, error, stream);
+  if (status != 0 || splits == 1) return status;
+  return rows_merge_bf16(parts, out, out_stride, tokens, num_heads, head_dim, sink, stream);
+}

@@ -58,7 +58,7 @@ CUDA_UNITS: dict[str, list[str]] = {
     # models whose attention reads one latent row per token; gated and squared-ReLU activations on float32 products
     "latent": ["latent.cu", "latent_attention_mma.cu"],
     # caches in eight bits, trees of drafted tokens (both dtypes)
-    "cached": ["cached_rows.cu", "attention_rows.cu", "attention_decode_e4m3.cu"],
+    "cached": ["cached_rows.cu", "attention_rows.cu", "attention_decode_e4m3.cu", "attention_tree_tcgen05.cu"],
 }
 _HEADERS = ["common.cuh", "recurrent.cuh", "cached_rows.cuh", "tcgen05.cuh", "softmax_pairs.cuh", "no_alloc.h"]
 

@@ -61,6 +61,7 @@ struct QueryRows {
   const int* seqs;        // [requests, 3]: first, nodes, past; or null
   const int* bits;        // [tokens, words]
   int words;
+  int tokens;             // of the step
   int group;              // query heads per kv head
   int num_heads;
   int window, chunk, keep_first;
@@ -75,9 +76,10 @@ struct Request {
 __device__ __forceinline__ Request request_of(const QueryRows& rows, int b) {
   Request r;
   if (rows.seqs) {
-    r.first = rows.seqs[3 * b];
-    r.nodes = rows.seqs[3 * b + 1];
-    r.past = rows.seqs[3 * b + 2];
+    // (held to the step's tokens and to the masks' words, whatever the rows say)
+    r.first = min(max(rows.seqs[3 * b], 0), rows.tokens);
+    r.nodes = min(min(max(rows.seqs[3 * b + 1], 0), rows.words * 32), rows.tokens - r.first);
+    r.past = max(rows.seqs[3 * b + 2], 0);
     r.seat = rows.seq_seat[b];
   } else {
     r.first = b;

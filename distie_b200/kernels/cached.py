@@ -25,6 +25,18 @@ def _ptr(x):
     return x.data_ptr() if x is not None else None
 
 
+def tree_splits(tiles: int, blocks: int, sms: int) -> int:
+    """Shares that the keys of ``tiles`` tiles of rows, ``blocks`` blocks of 128 keys each, are cut into
+    (attention_tree_tcgen05.cu): the number for which whole waves of CTAs take the least time, a CTA the time of its blocks
+    and of two more for its start and end; joining the parts takes another two."""
+    best, least = 1, None
+    for splits in range(1, max(1, min(blocks, 64)) + 1):
+        cost = -(-tiles * splits // sms) * (-(-blocks // splits) + 2) + (2 if splits > 1 else 0)
+        if least is None or cost < least:
+            best, least = splits, cost
+    return best
+
+
 class CachedRows:
     @staticmethod
     def _apart(step, kv) -> bool:
@@ -146,13 +158,16 @@ class CachedRows:
         if tree is not None:
             most = int(tree.most_nodes)
             if not 1 <= most <= MOST_DRAFTED or tree.bits.dtype != torch.int32 or tree.seqs.dtype != torch.int32 \
-                    or tree.bits.shape[0] < tokens or tree.bits.shape[1] * 32 < most or not tree.bits.is_contiguous() \
+                    or tree.bits.shape[0] < tokens or not most <= 32 * tree.bits.shape[1] <= MOST_DRAFTED or not tree.bits.is_contiguous() \
                     or tuple(tree.seqs.shape) != (requests, 3) or not tree.seqs.is_contiguous():
                 raise KernelError(f"attention: a tree of 1 to {MOST_DRAFTED} new tokens a request with int32 masks [tokens, words] and "
                                   f"rows [{requests}, 3] is expected")
         group = num_heads // num_kv_heads
         if tree is None and self._decode_e4m3(q, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first, softcap,
                                               sink, tokens):
+            return
+        if tree is not None and self._tree_tcgen05(q, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first,
+                                                   softcap, sink, tokens, requests, most):
             return
         blocks = requests * num_kv_heads * -(-most * group // 16)
         splits = max(1, min(4 * self.sm_count // blocks, step.max_kv_len // 64, 64))
@@ -201,4 +216,30 @@ class CachedRows:
             return False
         check(code, "attention_decode_e4m3")
         self._ran("attention_decode_e4m3", 1 if splits <= 8 else 2)
+        return True
+
+    def _tree_tcgen05(self, q, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first, softcap, sink,
+                      tokens: int, requests: int, most: int) -> bool:
+        """Drafted tokens on the tensor cores (attention_tree_tcgen05.cu); False for sizes and alignments that the kernel does not take."""
+        if self.dtype != torch.bfloat16 or head_dim not in (64, 128) or kv.v.shape[-1] != head_dim:
+            return False
+        tree, group = step.tree, num_heads // num_kv_heads
+        seen = min(step.max_kv_len, (window or chunk or step.max_kv_len) + most + 128)
+        splits = tree_splits(requests * num_kv_heads * -(-most * group // 128), -(-seen // 128), self.sm_count)
+        scratch = None
+        if splits > 1:
+            floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, head_dim, splits)
+            scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        with self._here():
+            code = function("distie_attention_tree_tcgen05")(
+                q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
+                step.seq_seat.data_ptr(), tree.seqs.data_ptr(), tree.bits.data_ptr(), tree.bits.shape[1], requests, tokens, most,
+                kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.k_scale), _ptr(kv.v_scale), kv.block_table.data_ptr(),
+                kv.block_table.shape[-1], num_heads, num_kv_heads, head_dim, kv.page_size, kv.num_pages, window, chunk, keep_first,
+                float(scale), softcap, _ptr(sink), splits, self.error_flag.data_ptr(), self._stream(),
+            )
+        if code == -2:
+            return False
+        check(code, "attention_tree_tcgen05")
+        self._ran("attention_tree_tcgen05", 1 if splits == 1 else 2)
         return True

@@ -132,8 +132,11 @@ class Case:
         return torch.cat(out)
 
     def attention(self, q, heads, scale, window=None, chunk=None, keep_first=0, softcap=0.0, sink=None):
-        """(output, sum of weight times magnitude of the values), 64 bits, both [tokens, heads * value size]."""
-        outs, sizes = [], []
+        """(output, sum of weight times magnitude of the values), 64 bits, both [tokens, heads * value size].  ``least`` then holds
+        what weights in float16 may miss of an 8-bit cache's output: below 2^-14 float16 has steps of 2^-24, so every weight
+        (times its value's scale, over the largest such product) may be off by 2^-25, and an element by as much of the sum of
+        its numbers' magnitudes."""
+        outs, sizes, least = [], [], []
         for r in range(len(self.news)):
             k, v = self.held("k", r).repeat_interleave(heads // self.kv_heads, 0), self.held("v", r).repeat_interleave(heads // self.kv_heads, 0)
             mine = q[self.starts[r] : self.starts[r] + self.news[r], : heads * self.dim].double().cpu()
@@ -152,8 +155,17 @@ class Case:
                 out, size = w @ v, w @ v.abs()
             else:  # a value that is not finite counts for the rows that see it
                 out, size = (w.unsqueeze(-1) * clean(v)).sum(2), (w.unsqueeze(-1) * clean(v.abs())).sum(2)
+            small = torch.zeros_like(out)
+            if self.kv.v_scale is not None:
+                need = -(-(self.pasts[r] + self.news[r]) // self.page)
+                ids = self.table[self.seats[r], :need].long()
+                flat = lambda x: x[ids].transpose(0, 1).flatten(1, 2)[:, : v.shape[1]].repeat_interleave(heads // self.kv_heads, 0)  # noqa: E731
+                most = (w * flat(self.kv.v_scale.double().cpu())[:, None]).nan_to_num(0.0).amax(-1, keepdim=True)
+                small = 2.0**-25 * most * flat(self.kv.v.double().cpu()).abs().sum(1)[:, None]
+            least.append(small.transpose(0, 1).reshape(self.news[r], -1))
             outs.append(out.transpose(0, 1).reshape(self.news[r], -1))
             sizes.append(size.transpose(0, 1).reshape(self.news[r], -1))
+        self.least = torch.cat(least)
         return torch.cat(outs), torch.cat(sizes)
 
 

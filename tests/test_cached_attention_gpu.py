@@ -42,6 +42,8 @@ def check(k, case, heads, q=None, large=False, **what):
     # (relative to the sum of weight times magnitude; the sum that divides them is not rounded), and float32 sums and exponentials: scores
     # of up to 50 are off by 50 * 2^-22 or so, and so are their exponentials.
     slack = half_step(dtype) * want.abs() + ((half_step(BF16) if dtype == BF16 else 0.0) + 2.0**-15) * size
+    if dtype == BF16:
+        slack = slack + case.least
     if large:
         # A score is summed in float32: head_dim / 16 steps of the tensor cores, each off by 2^-23 of the sum of magnitudes at
         # most (or head_dim roundings of 2^-24 that go either way): 2^-20 of that sum for 128 dims.  An error e of the scores
