@@ -196,8 +196,8 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
     float x[MT][4], most = 0.f;
 #pragma unroll
     for (int ks = 0; ks < MT; ++ks) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (hd < heads_here) v = load4_cg(q + (size_t)t * q_stride + (size_t)(head0 + hd) * D + 16 * ks + 4 * c);
+      // (columns behind the last head are nobody's: copies of it, so that no load hangs on a branch)
+      const float4 v = load4_cg(q + (size_t)t * q_stride + (size_t)(head0 + min(hd, heads_here - 1)) * D + 16 * ks + 4 * c);
       x[ks][0] = v.x; x[ks][1] = v.y; x[ks][2] = v.z; x[ks][3] = v.w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[ks][e]));

@@ -10,12 +10,13 @@
 //                    as 16-bit numbers, two keys to a column.  Warps whose rows are all empty take no part.
 //   O_g += P_g V_g   tcgen05.mma with P as the A operand straight from tensor memory
 //
-// Loaders bring K and V through registers (seven warps, 16 bytes a thread and load; V of a block is requested while its K is
-// stored, and the next K while V is): pages of any size, rows in any order of
-// pages.  Of a 16-bit cache they store what they loaded; of an 8-bit one they turn e4m3 numbers into float16, which holds
-// them exactly, so that Q (times a power of two a row, float16), K, P and V are float16 there and bfloat16 here.  The
-// scales of the rows go beside the tiles: s^k multiplies the finished score, and p s^v is one exponential,
-// exp2(score + log2 s^v - m'), with a running maximum m' of its own (attention_decode_e4m3.cu says why).
+// Loaders (four warps, 32 keys each) copy K and V asynchronously, three tiles in flight, pages of any size: a lane looks up
+// the row of its key, and the warp takes the rows from its lanes, 16 bytes a lane and copy.  Rows of a 16-bit cache land
+// where the product reads them; those of an 8-bit one land packed where their warp's rows will be, are read into registers
+// and written back as float16, which holds every e4m3 number exactly, so that Q (times a power of two a row, float16), K, P and V are float16 there and bfloat16 here.  The
+// scales of the rows go beside the tiles: s^k multiplies the finished score; the weights of the second product are p s^v over
+// a running maximum m' of their own, p (s^v 2^(m - m')), so that float16 holds the largest of a row near 1 whatever
+// the scales.
 //
 // Masks: a block that lies before every row's new tokens and inside every row's window needs none; the others get 64 bits a
 // row and group.  A masked weight is 0, and 0 * (what is not finite) is not 0: in blocks that need masks, values that are not
@@ -25,7 +26,7 @@
 // Running maxima are raised only when exceeded by more than 8 (base 2), so O is read, scaled and written back rarely.
 // With several shares of the keys, the parts go to scratch in float32 and attention_rows.cu joins them.
 //
-//   warps 0..7    softmax, end        warp 8   tensor memory, MMA issue        warps 9..15   loaders
+//   warps 0..7    softmax, end        warp 8   tensor memory, MMA issue        warps 9..12   loaders
 //
 // Every wait on an mbarrier is bounded; when one runs out the CTA sets the error word to 6 and every role stops at its
 // next wait.
@@ -42,11 +43,12 @@ constexpr int kTreeKeys = 128;
 constexpr int kTreeGroupKeys = 64;
 constexpr int kTreeMmaWarp = 8;
 constexpr int kTreeLoadWarp = 9;
-constexpr int kTreeLoaders = 7 * 32;  // threads
-constexpr int kTreeThreads = 32 * 16;
+constexpr int kTreeLoaders = 4;    // warps
+constexpr int kTreeThreads = 32 * 13;
 constexpr int kTreeKStages = 2, kTreeVStages = 3, kTreeScaleSlots = 4;
 constexpr int kTreeHalf = kTreeRows * 128;  // bytes of one [128 rows x 64 elements] swizzled half tile
 constexpr int kTreeMostNodes = 256;
+constexpr int kTreePages = 2048;   // page ids of a CTA's share that are kept in shared memory
 constexpr float kTreeRaise = 8.f;
 
 template <int D>
@@ -55,9 +57,11 @@ struct TreeShared {
   alignas(1024) unsigned char k[kTreeKStages][kTreeKeys * D * 2];
   alignas(1024) unsigned char v[kTreeVStages][kTreeKeys * D * 2];
   float k_scale[kTreeScaleSlots][kTreeKeys];  // of the keys of a block
-  float v_log[kTreeScaleSlots][kTreeKeys];    // log2 of the values' scales
+  float v_scale[kTreeScaleSlots][kTreeKeys];
+  float v_log[kTreeScaleSlots][kTreeKeys];    // log2 of it
   float q_times[kTreeRows];                   // what turns a row's raw products into scores, before the keys' scales
   int node_position[kTreeMostNodes];
+  int pages[kTreePages];
   uint64_t q_full;
   uint64_t k_full[kTreeKStages], k_empty[kTreeKStages];
   uint64_t v_full[kTreeVStages], v_empty[kTreeVStages];
@@ -169,14 +173,14 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, kTreeMmaWarp);
     for (int s = 0; s < kTreeKStages; ++s) {
-      mbar_init(&sm.k_full[s], kTreeLoaders / 32);
+      mbar_init(&sm.k_full[s], kTreeLoaders);
       mbar_init(&sm.k_empty[s], 1);
     }
     for (int s = 0; s < kTreeVStages; ++s) {
-      mbar_init(&sm.v_full[s], kTreeLoaders / 32);
+      mbar_init(&sm.v_full[s], kTreeLoaders);
       mbar_init(&sm.v_empty[s], 1);
     }
-    for (int s = 0; s < kTreeScaleSlots; ++s) mbar_init(&sm.scale_full[s], kTreeLoaders / 32);
+    for (int s = 0; s < kTreeScaleSlots; ++s) mbar_init(&sm.scale_full[s], kTreeLoaders);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.s_full[b], 1);
       mbar_init(&sm.p_full[0][b], active);
@@ -194,6 +198,10 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
   }
   for (int n = threadIdx.x; n < request.nodes && n < kTreeMostNodes; n += kTreeThreads)
     sm.node_position[n] = rows.positions[request.first + n];
+  // The page ids of the share's keys from its window's first block on.
+  const int column0 = cache.column_of(span.key0(max(block0, span.kept_blocks)));
+  const int columns = block1 > span.kept_blocks ? min(kTreePages, cache.column_of(min(span.keys - 1, span.key0(block1 - 1) + kTreeKeys - 1)) - column0 + 1) : 0;
+  for (int i = threadIdx.x; i < columns; i += kTreeThreads) sm.pages[i] = column0 + i < cache.table_width ? table[column0 + i] : -1;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -202,38 +210,48 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
 
   if (warp >= kTreeLoadWarp) {
     // ---- loaders: 16 bytes of a row per thread and load --------------------------------------------------------------
-    constexpr int PPR = E4M3 ? D / 16 : D / 8;  // pieces of a row
-    constexpr int ALL = kTreeKeys * PPR;        // of a tile
-    constexpr int PIECES = (ALL + kTreeLoaders - 1) / kTreeLoaders;  // of a tile, per thread
-    const int thread = threadIdx.x - kTreeLoadWarp * 32;
-    auto fetch = [&](uint4 (&raw)[PIECES], float (&scale)[PIECES], const void* rows_at, const float* scales_at, int j) {
-      if (j >= block1) return;
-      const int key0 = span.key0(j), key_end = span.key_end(j);
+    constexpr int PPR = E4M3 ? D / 16 : D / 8;  // 16-byte pieces of a row
+    constexpr int RPI = 32 / PPR;               // rows that one copy of the warp covers
+    constexpr int PIECES = 32 / RPI;            // copies of a tile, per lane
+    constexpr int LAG = 3;                      // tiles in flight
+    const int row0_mine = (warp - kTreeLoadWarp) * 32;  // the warp's keys of a block
+    const int sub_row = lane / PPR, piece = lane % PPR;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_unless(bar, parity, failed)) != 0; };
+    auto find = [&](int j) {  // the row of this lane's key of block j among the slot's rows, -1: none
+      const int key = span.key0(j) + row0_mine + lane;
+      int at = -1;
+      if (key < span.key_end(j) && (key >= span.oldest || key < span.kept)) {
+        const int column = cache.column_of(key), index = column - column0;
+        const int page = index >= 0 && index < columns ? sm.pages[index] : column < cache.table_width ? __ldg(table + column) : -1;
+        if (page >= 0 && page < cache.num_pages) at = (page * cache.num_kv_heads + kv_head) * cache.page_size + cache.within(key);
+        else if (error) atomicExch(error, 8);
+      }
+      __syncwarp();
+      return at;
+    };
+    auto copy = [&](unsigned char* stage, const void* rows_at, int at) {
+      const uint32_t base = smem_u32(stage) + (E4M3 ? row0_mine * 128 + lane * 16 : 0);
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int p = thread + i * kTreeLoaders, key = key0 + p / PPR;
-        raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        scale[i] = 0.f;
-        if (p < ALL && key < key_end && (key >= span.oldest || key < span.kept)) {
-          const long long at = cache.row_of(table, key, kv_head);
-          if (at < 0) {
-            if (error) atomicExch(error, 8);
-          } else {
-            raw[i] = load16_cg(reinterpret_cast<const unsigned char*>(rows_at) + (size_t)at * (PPR * 16) + p % PPR * 16);
-            if (E4M3 && p % PPR == 0) scale[i] = __ldcg(scales_at + at);
-          }
-        }
+        const int row = i * RPI + sub_row, from_row = __shfl_sync(0xffffffffu, at, row);
+        const unsigned char* from = reinterpret_cast<const unsigned char*>(rows_at) + (size_t)max(from_row, 0) * (PPR * 16) + piece * 16;
+        const uint32_t to = E4M3 ? base + i * 512 : base + tree_offset(row0_mine + row, piece);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(from_row >= 0 ? 16 : 0) : "memory");
       }
     };
-    auto put = [&](unsigned char* tile_at, const uint4 (&raw)[PIECES]) {
-      const uint32_t base = smem_u32(tile_at);
+    // A tile whose copies have landed (this warp's of them): made what the product reads.
+    auto finish = [&](unsigned char* stage, bool check) {
+      if (E4M3) {
+        uint4 raw[PIECES];
+        __syncwarp();
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int p = thread + i * kTreeLoaders, row = p / PPR, piece = p % PPR;
-        if (p >= ALL) break;
-        const uint4& x = raw[i];
-        if (E4M3) {
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        for (int i = 0; i < PIECES; ++i) raw[i] = *reinterpret_cast<const uint4*>(stage + row0_mine * 128 + i * 512 + lane * 16);
+        __syncwarp();
+        const uint32_t base = smem_u32(stage);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int row = row0_mine + i * RPI + sub_row;
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
           uint32_t h[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -242,16 +260,21 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
           }
           store_shared16(base + tree_offset(row, 2 * piece), h[0], h[1], h[2], h[3]);
           store_shared16(base + tree_offset(row, 2 * piece + 1), h[4], h[5], h[6], h[7]);
-        } else {
-          store_shared16(base + tree_offset(row, piece), x.x, x.y, x.z, x.w);
         }
-      }
-    };
-    auto put_scales = [&](float* scales_at, const float (&scale)[PIECES], bool as_log) {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int p = thread + i * kTreeLoaders;
-        if (p < ALL && p % PPR == 0) scales_at[p / PPR] = as_log ? tree_log2(scale[i]) : scale[i];
+      } else if (check) {
+        bool bad = false;
+        for (int i = 0; i < PIECES; ++i) {  // (the lane's own copies)
+          uint4* at = reinterpret_cast<uint4*>(stage + tree_offset(row0_mine + i * RPI + sub_row, piece));
+          uint4 x = *at;
+          bool here = false;
+          x.x = finite_pair(x.x, here);
+          x.y = finite_pair(x.y, here);
+          x.z = finite_pair(x.z, here);
+          x.w = finite_pair(x.w, here);
+          if (here) *at = x;
+          bad |= here;
+        }
+        if (bad) atomicExch(&sm.bad, 1u);
       }
     };
     auto ready = [&](uint64_t* bar) {  // this warp's stores are in shared memory, for the tensor cores and for other warps
@@ -259,45 +282,54 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_unless(bar, parity, failed)) != 0; };
-    uint4 k_raw[PIECES], v_raw[PIECES];
-    float k_scale[PIECES], v_scale[PIECES];
+    // Tile 2 n is K of the share's block n, tile 2 n + 1 its V: requested when its stage is free, finished LAG tiles later.
     bool ok = true;
-    fetch(k_raw, k_scale, cache.k, cache.k_scale, block0);
-    fetch(v_raw, v_scale, cache.v, cache.v_scale, block0);
-    for (int j = block0; j < block1; ++j) {
-      const int n = j - block0, ks = n % kTreeKStages, vs = n % kTreeVStages, slot = n % kTreeScaleSlots;
-      // The slot's last scales are read: the S of two blocks ago, whose K this stage held, was issued behind their P.
-      if (!wait(&sm.k_empty[ks], ((n / kTreeKStages) & 1) ^ 1)) { ok = false; break; }
-      put(sm.k[ks], k_raw);
-      if (E4M3) put_scales(sm.k_scale[slot], k_scale, false);
-      ready(&sm.k_full[ks]);
-      fetch(k_raw, k_scale, cache.k, cache.k_scale, j + 1);
-      if (E4M3) {
-        put_scales(sm.v_log[slot], v_scale, true);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.scale_full[slot]);
+    float ks_ahead = 0.f, vs_ahead = 0.f;
+    int at = -1;
+    for (int i = 0; i < 2 * blocks + LAG && ok; ++i) {
+      const int n = i >> 1;
+      if (i < 2 * blocks) {
+        const bool is_k = !(i & 1);
+        if (is_k) at = find(block0 + n);
+        uint64_t* empty = is_k ? &sm.k_empty[n % kTreeKStages] : &sm.v_empty[n % kTreeVStages];
+        const int use = is_k ? n / kTreeKStages : n / kTreeVStages;
+        if (!wait(empty, (use & 1) ^ 1)) { ok = false; break; }
+        copy(is_k ? sm.k[n % kTreeKStages] : sm.v[n % kTreeVStages], is_k ? cache.k : cache.v, at);
       }
-      if (!wait(&sm.v_empty[vs], ((n / kTreeVStages) & 1) ^ 1)) { ok = false; break; }
-      if (!E4M3 && !span.whole(j)) {
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-          v_raw[i].x = finite_pair(v_raw[i].x, bad);
-          v_raw[i].y = finite_pair(v_raw[i].y, bad);
-          v_raw[i].z = finite_pair(v_raw[i].z, bad);
-          v_raw[i].w = finite_pair(v_raw[i].w, bad);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (E4M3 && !(i & 1)) {
+        // Scales, a lane per key, one block ahead in registers.  The slot's last ones have been read: the S of two blocks
+        // ago, whose stage K has just taken, was issued behind the P before it.
+        if (n >= 1 && n <= blocks) {
+          const int slot = (n - 1) % kTreeScaleSlots;
+          sm.k_scale[slot][row0_mine + lane] = ks_ahead;
+          sm.v_scale[slot][row0_mine + lane] = vs_ahead;
+          sm.v_log[slot][row0_mine + lane] = tree_log2(vs_ahead);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.scale_full[slot]);
         }
-        if (bad) atomicExch(&sm.bad, 1u);
+        if (n < blocks) {
+          ks_ahead = __ldcg(cache.k_scale + max(at, 0));  // (of no key: never read behind the mask)
+          vs_ahead = __ldcg(cache.v_scale + max(at, 0));
+        }
       }
-      put(sm.v[vs], v_raw);
-      ready(&sm.v_full[vs]);
-      fetch(v_raw, v_scale, cache.v, cache.v_scale, j + 1);
+      if (i >= LAG) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
+        const int done = i - LAG, m = done >> 1;
+        if (!(done & 1)) {
+          finish(sm.k[m % kTreeKStages], false);
+          ready(&sm.k_full[m % kTreeKStages]);
+        } else {
+          finish(sm.v[m % kTreeVStages], !span.whole(block0 + m));
+          ready(&sm.v_full[m % kTreeVStages]);
+        }
+      }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (!ok) atomicExch(&sm.failed, 1u);
   } else if (warp == kTreeMmaWarp) {
     // ---- MMA issuer ----------------------------------------------------------------------------------------------------
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t type = E4M3 ? 0u : (1u << 7) | (1u << 10);  // float16 or bfloat16 operands
       constexpr uint32_t idesc_s = (1u << 4) | type | ((uint32_t)(kTreeKeys >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       constexpr uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -349,14 +381,11 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
       uint2 x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int r = warp * 16 + i;
-        x[i] = make_uint2(0u, 0u);
-        if (r < count) {
-          const int token = request.first + (row0 + r) / rows.group, head = kv_head * rows.group + (row0 + r) % rows.group;
-          const __nv_bfloat16* from = q + (size_t)token * q_stride + (size_t)head * D + lane * PER_LANE;
-          if (PER_LANE == 4) x[i] = __ldcg(reinterpret_cast<const uint2*>(from));
-          else x[i].x = __ldcg(reinterpret_cast<const unsigned int*>(from));
-        }
+        const int r = min(warp * 16 + i, count - 1);  // (rows behind the last one are nobody's: copies of it)
+        const int token = request.first + (row0 + r) / rows.group, head = kv_head * rows.group + (row0 + r) % rows.group;
+        const __nv_bfloat16* from = q + (size_t)token * q_stride + (size_t)head * D + lane * PER_LANE;
+        if (PER_LANE == 4) x[i] = __ldcg(reinterpret_cast<const uint2*>(from));
+        else x[i] = make_uint2(__ldcg(reinterpret_cast<const unsigned int*>(from)), 0u);
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -449,25 +478,45 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         const float* k_scale = &sm.k_scale[slot][g * kTreeGroupKeys];
         const float* v_log = &sm.v_log[slot][g * kTreeGroupKeys];
-        float mx = -INFINITY, ox = -INFINITY;
+        const float* v_scale = &sm.v_scale[slot][g * kTreeGroupKeys];
+        // Scores in base-2 units, on pairs of values.
+        const uint64_t times2 = pair_of(times, times);
 #pragma unroll
-        for (int i = 0; i < kTreeGroupKeys; i += 4) {
-          float4 ks = make_float4(1.f, 1.f, 1.f, 1.f), vl = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (E4M3) {
-            ks = *reinterpret_cast<const float4*>(k_scale + i);
-            vl = *reinterpret_cast<const float4*>(v_log + i);
-          }
-          const float kk[4] = {ks.x, ks.y, ks.z, ks.w}, vv[4] = {vl.x, vl.y, vl.z, vl.w};
+        for (int i = 0; i < kTreeGroupKeys; i += 2) {
+          uint64_t x = pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+          if (E4M3) x = mul_pairs(x, *reinterpret_cast<const uint64_t*>(k_scale + i));
+          x = mul_pairs(x, times2);
+          float x0, x1;
+          halves_of(x, x0, x1);
+          sv[i] = __float_as_uint(x0);
+          sv[i + 1] = __float_as_uint(x1);
+        }
+        if (rows.extras.cap > 0.f) {  // cap * tanh, by its exponential: off by 2^-22 of the cap
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = __uint_as_float(sv[i + e]) * (E4M3 ? times * kk[e] : times);
-            if (rows.extras.cap > 0.f) x = cap * (1.f - __fdividef(2.f, exp2_approx(x * 2.8853900817779268f) + 1.f));
-            if (!whole && !((mask >> (i + e)) & 1)) x = -INFINITY;
-            sv[i + e] = __float_as_uint(x);
-            mx = fmaxf(mx, x);
-            if (E4M3) ox = fmaxf(ox, x == -INFINITY ? x : x + vv[e]);
+          for (int i = 0; i < kTreeGroupKeys; ++i)
+            sv[i] = __float_as_uint(cap * (1.f - __fdividef(2.f, exp2_approx(__uint_as_float(sv[i]) * 2.8853900817779268f) + 1.f)));
+        }
+        if (!whole) {
+          const uint32_t low = (uint32_t)mask, high = (uint32_t)(mask >> 32);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (!((low >> i) & 1)) sv[i] = 0xff800000u;  // -inf
+            if (!((high >> i) & 1)) sv[32 + i] = 0xff800000u;
           }
         }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ox4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kTreeGroupKeys; i += 2) {
+          float& m = mx4[(i >> 1) & 3];
+          m = max3(m, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+          if (E4M3) {
+            float z0, z1;
+            halves_of(add_pairs(pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), *reinterpret_cast<const uint64_t*>(v_log + i)), z0, z1);
+            float& o = ox4[(i >> 1) & 3];
+            o = max3(o, z0, z1);
+          }
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), ox = fmaxf(fmaxf(ox4[0], ox4[1]), fmaxf(ox4[2], ox4[3]));
         // The maximum in use for the sum, and the one for O (of a 16-bit cache they are one).
         const float m_new = fmaxf(m_used, mx);
         const bool raise_sum = m_new > m_used + kTreeRaise || (m_used == -INFINITY && m_new > -INFINITY);
@@ -501,45 +550,46 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             tmem_store_32(o_addr + c0, v);
           }
         }
-        const float shift = m_used == -INFINITY ? 0.f : m_used, out_shift = o_used == -INFINITY ? 0.f : o_used;
-        float sum[2] = {0.f, 0.f};
+        const float shift = m_used == -INFINITY ? 0.f : m_used;
+        // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0)
+        const float units = E4M3 && o_used != -INFINITY ? exp2_approx(fminf(shift - o_used, 126.f)) : 0.f;
+        const uint64_t shift2 = pair_of(-shift, -shift), units2 = pair_of(units, units);
+        uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t packed[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float4 vl = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (E4M3) vl = *reinterpret_cast<const float4*>(v_log + half * 32 + i);
-            const float vv[4] = {vl.x, vl.y, vl.z, vl.w};
-            float w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = __uint_as_float(sv[half * 32 + i + e]);
-              const float p = exp2_approx(x - shift);
-              if (E4M3) {
-                sum[e & 1] += p;
-                w[e] = x == -INFINITY ? 0.f : exp2_approx(x + vv[e] - out_shift);
-              } else {
-                w[e] = p;
+          for (int i = 0; i < 32; i += 2) {
+            const int at = half * 32 + i;
+            float x0, x1;
+            halves_of(add_pairs(pair_of(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), shift2), x0, x1);
+            const uint64_t p = pair_of(exp2_approx(x0), exp2_approx(x1));
+            uint64_t& sum = sum4[(i >> 1) & 3];
+            float w0, w1;
+            if (E4M3) {
+              sum = add_pairs(sum, p);
+              halves_of(mul_pairs(p, mul_pairs(*reinterpret_cast<const uint64_t*>(v_scale + at), units2)), w0, w1);
+              if (!whole) {  // (0 times the scale of a row that is not finite, or of nobody's, is not 0)
+                w0 = sv[at] == 0xff800000u ? 0.f : w0;
+                w1 = sv[at + 1] == 0xff800000u ? 0.f : w1;
               }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              if (E4M3) {
-                const __half2 pair = __floats2half2_rn(w[e], w[e + 1]);
-                packed[(i + e) >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
-              } else {  // the sum is that of the weights as the product takes them
-                const __nv_bfloat162 pair = __floats2bfloat162_rn(w[e], w[e + 1]);
-                const uint32_t both = *reinterpret_cast<const uint32_t*>(&pair);
-                packed[(i + e) >> 1] = both;
-                sum[0] += __uint_as_float(both << 16);
-                sum[1] += __uint_as_float(both & 0xffff0000u);
-              }
+              const __half2 pair = __floats2half2_rn(w0, w1);
+              packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
+            } else {  // the sum is that of the weights as the product takes them
+              halves_of(p, w0, w1);
+              const __nv_bfloat162 pair = __floats2bfloat162_rn(w0, w1);
+              const uint32_t both = *reinterpret_cast<const uint32_t*>(&pair);
+              packed[i >> 1] = both;
+              sum = add_pairs(sum, pair_of(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)));
             }
           }
           tmem_store_16(s_addr + half * 16, packed);
         }
-        l += sum[0] + sum[1];
+        {
+          float even, odd;
+          halves_of(add_pairs(add_pairs(sum4[0], sum4[1]), add_pairs(sum4[2], sum4[3])), even, odd);
+          l += even + odd;
+        }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -652,7 +702,7 @@ extern "C" int distie_attention_tree_tcgen05(const void* q, int q_stride, void* 
       bits == nullptr || (splits > 1 && scratch == nullptr) || (k_scale == nullptr) != (v_scale == nullptr))
     return DISTIE_ERR_ARG;
   if ((head_dim != 64 && head_dim != 128) || (q_stride & 3) || ((uintptr_t)q & 7) || (out_stride & 7) || ((uintptr_t)out & 15) ||
-      (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15))
+      (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15) || (long long)num_pages * num_kv_heads * page_size > 0x7fffffffLL)
     return DISTIE_ERR_UNSUPPORTED;
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, head_dim, head_dim,
                                       page_size, num_pages);
