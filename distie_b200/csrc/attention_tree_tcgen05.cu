@@ -51,6 +51,21 @@ constexpr int kTreeMostNodes = 256;
 constexpr int kTreePages = 2048;   // page ids of a CTA's share that are kept in shared memory
 constexpr float kTreeRaise = 8.f;
 
+// The blocks of 128 keys that a tile of rows walks: those of the kept first keys, then those from the window's start on.
+struct TreeSpan {
+  int past, keys;       // cached keys, and all of them
+  int oldest, newest;   // oldest key that any row's window holds; oldest one that every row's window holds
+  int kept;             // first keys that stay visible before `oldest`
+  int kept_blocks, start, blocks;
+
+  __device__ __forceinline__ int key0(int j) const { return j < kept_blocks ? j * kTreeKeys : start + (j - kept_blocks) * kTreeKeys; }
+  __device__ __forceinline__ int key_end(int j) const { return j < kept_blocks ? min(kept, start) : keys; }
+  // Whether every row of the tile sees every key of the block.
+  __device__ __forceinline__ bool whole(int j) const {
+    return j >= kept_blocks && key0(j) >= newest && key0(j) + kTreeKeys <= past;
+  }
+};
+
 template <int D>
 struct TreeShared {
   alignas(1024) unsigned char q[kTreeRows * D * 2];
@@ -60,6 +75,9 @@ struct TreeShared {
   float v_scale[kTreeScaleSlots][kTreeKeys];
   float v_log[kTreeScaleSlots][kTreeKeys];    // log2 of it
   float q_times[kTreeRows];                   // what turns a row's raw products into scores, before the keys' scales
+  TreeSpan span;              // (here and not in registers: the softmax warps need theirs)
+  int row_token[kTreeRows];   // token of a row, -1: no row
+  int row_first[kTreeRows];   // its oldest visible key
   int node_position[kTreeMostNodes];
   int pages[kTreePages];
   uint64_t q_full;
@@ -74,21 +92,6 @@ struct TreeShared {
   uint32_t tmem_base;
   uint32_t failed;
   uint32_t bad;  // a masked block holds a value that is not finite
-};
-
-// The blocks of 128 keys that a tile of rows walks: those of the kept first keys, then those from the window's start on.
-struct TreeSpan {
-  int past, keys;       // cached keys, and all of them
-  int oldest, newest;   // oldest key that any row's window holds; oldest one that every row's window holds
-  int kept;             // first keys that stay visible before `oldest`
-  int kept_blocks, start, blocks;
-
-  __device__ __forceinline__ int key0(int j) const { return j < kept_blocks ? j * kTreeKeys : start + (j - kept_blocks) * kTreeKeys; }
-  __device__ __forceinline__ int key_end(int j) const { return j < kept_blocks ? min(kept, start) : keys; }
-  // Whether every row of the tile sees every key of the block.
-  __device__ __forceinline__ bool whole(int j) const {
-    return j >= kept_blocks && key0(j) >= newest && key0(j) + kTreeKeys <= past;
-  }
 };
 
 __device__ __forceinline__ uint32_t tree_offset(int row, int piece) {  // of 8 elements of a row in a tile of swizzled halves
@@ -111,6 +114,62 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t x, bool& bad) {
   return x & keep;
 }
 
+// Whether the row sees a key.  (Functions of their own, called where a block needs masks: what they look at takes no registers
+// elsewhere.)
+template <int D>
+__device__ __forceinline__ bool tree_seen(const TreeShared<D>& sm, int r, int key, int key_end, const int* bits, int words, int keep_first) {
+  const int token = sm.row_token[r];
+  if (token < 0 || key >= key_end) return false;
+  int place = key;
+  if (key >= sm.span.past) {
+    const int n = key - sm.span.past;
+    if (!((__ldg(bits + (size_t)token * words + (n >> 5)) >> (n & 31)) & 1)) return false;
+    place = sm.node_position[n];
+  }
+  return place >= sm.row_first[r] || place < keep_first;
+}
+// The keys of [key0, key0 + 64) that the row sees, a bit each.
+template <int D>
+__device__ __noinline__ uint64_t tree_seen64(const TreeShared<D>& sm, int r, int key0, int key_end, const int* bits, int words, int keep_first) {
+  uint64_t mask = 0;
+  const int token = sm.row_token[r], past = sm.span.past;
+  if (token < 0) return mask;
+  if (sm.row_first[r] == 0) {  // no window has moved: cached keys, then the row's mask
+    const int cached = min(max(past - key0, 0), 64);
+    if (cached > 0) mask = cached == 64 ? ~0ull : (1ull << cached) - 1;
+    const int there = min(64 - cached, key_end - max(key0, past));
+    if (there > 0) {
+      const int skip = max(key0 - past, 0), word = skip >> 5, shift = skip & 31;  // new tokens before key0
+      auto load = [&](int w) { return w < words ? (uint32_t)__ldg(bits + (size_t)token * words + w) : 0u; };
+      const uint32_t w0 = load(word), w1 = load(word + 1), w2 = load(word + 2);
+      uint64_t draft = (uint64_t)__funnelshift_r(w0, w1, shift) | ((uint64_t)__funnelshift_r(w1, w2, shift) << 32);
+      if (there < 64) draft &= (1ull << there) - 1;
+      mask |= draft << cached;  // (cached < 64 here)
+    }
+  } else {
+    for (int i = 0; i < 64; ++i)
+      if (tree_seen(sm, r, key0 + i, key_end, bits, words, keep_first)) mask |= 1ull << i;
+  }
+  return mask;
+}
+// What the values that are not finite, in blocks block0 .. block1 - 1 that need masks, add to element e of the row's sum.
+template <int D>
+__device__ __noinline__ float tree_not_finite(const TreeShared<D>& sm, int r, int e, int block0, int block1, const __nv_bfloat16* values,
+                                              const CachePages& cache, const int* table, int kv_head, const int* bits, int words, int keep_first) {
+  float sum = 0.f;
+  for (int j = block0; j < block1; ++j) {
+    if (sm.span.whole(j)) continue;
+    for (int key = sm.span.key0(j); key < sm.span.key0(j) + kTreeKeys; ++key) {
+      if (!tree_seen(sm, r, key, sm.span.key_end(j), bits, words, keep_first)) continue;
+      const long long at = cache.row_of(table, key, kv_head);
+      if (at < 0) continue;
+      const float v = __bfloat162float(values[(size_t)at * D + e]);
+      if (!(fabsf(v) <= 3.402823466e38f)) sum += v;
+    }
+  }
+  return sum;
+}
+
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(kTreeThreads, 1)
 attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride, QueryRows rows,
@@ -130,8 +189,9 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
   const int* table = cache.block_table + (size_t)request.seat * cache.table_width;
 
   grid_dependency_release();
-  TreeSpan span;
+  int block0, blocks;
   {
+    TreeSpan span;
     int low = 0x7fffffff, high = 0;
     const int node0 = row0 / rows.group, node1 = (row0 + count - 1) / rows.group;
     for (int n = node0 + lane; n <= node1; n += 32) {
@@ -152,10 +212,11 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     span.kept_blocks = (span.kept + kTreeKeys - 1) / kTreeKeys;
     span.start = span.oldest / kTreeKeys * kTreeKeys;
     span.blocks = span.kept_blocks + (span.keys - span.start + kTreeKeys - 1) / kTreeKeys;
+    const int share = (span.blocks + parts.splits - 1) / parts.splits;
+    block0 = min(span.blocks, split * share);
+    blocks = min(span.blocks, block0 + share) - block0;
+    if (threadIdx.x == 0) sm.span = span;
   }
-  const int share = (span.blocks + parts.splits - 1) / parts.splits;
-  const int block0 = min(span.blocks, split * share), block1 = min(span.blocks, block0 + share);
-  const int blocks = block1 - block0;
   if (blocks == 0) {  // a share without keys: its parts count nothing
     grid_dependency_wait();
     for (int r = warp; r < count; r += kTreeThreads / 32) {
@@ -198,18 +259,28 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
   }
   for (int n = threadIdx.x; n < request.nodes && n < kTreeMostNodes; n += kTreeThreads)
     sm.node_position[n] = rows.positions[request.first + n];
-  // The page ids of the share's keys from its window's first block on.
-  const int column0 = cache.column_of(span.key0(max(block0, span.kept_blocks)));
-  const int columns = block1 > span.kept_blocks ? min(kTreePages, cache.column_of(min(span.keys - 1, span.key0(block1 - 1) + kTreeKeys - 1)) - column0 + 1) : 0;
-  for (int i = threadIdx.x; i < columns; i += kTreeThreads) sm.pages[i] = column0 + i < cache.table_width ? table[column0 + i] : -1;
+  for (int r = threadIdx.x; r < kTreeRows; r += kTreeThreads) {
+    const int token = r < count ? request.first + (row0 + r) / rows.group : -1;
+    sm.row_token[r] = token;
+    sm.row_first[r] = token < 0 ? 0 : first_visible_key(rows.positions[token], rows.window, rows.chunk);
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const TreeSpan& span = sm.span;
+  const int block1 = block0 + blocks;
+  // The page ids of the share's keys from its window's first block on.
+  const int column0 = cache.column_of(span.key0(max(block0, span.kept_blocks)));
+  const int columns = block1 > span.kept_blocks ? min(kTreePages, cache.column_of(min(span.keys - 1, span.key0(block1 - 1) + kTreeKeys - 1)) - column0 + 1) : 0;
+  if (warp >= kTreeLoadWarp)  // (the loaders alone look at them)
+    for (int i = threadIdx.x - kTreeLoadWarp * 32; i < columns; i += kTreeLoaders * 32)
+      sm.pages[i] = column0 + i < cache.table_width ? table[column0 + i] : -1;
   const uint32_t tmem = sm.tmem_base;
   grid_dependency_wait();  // q and the newest rows come from the kernels before this one
 
   if (warp >= kTreeLoadWarp) {
-    // ---- loaders: 16 bytes of a row per thread and load --------------------------------------------------------------
+    // ---- loaders: 16 bytes of a row per lane and copy ------------------------------------------------------------------
+    asm volatile("bar.sync 1, %0;" ::"n"(kTreeLoaders * 32) : "memory");  // the page ids are there
     constexpr int PPR = E4M3 ? D / 16 : D / 8;  // 16-byte pieces of a row
     constexpr int RPI = 32 / PPR;               // rows that one copy of the warp covers
     constexpr int PIECES = 32 / RPI;            // copies of a tile, per lane
@@ -422,44 +493,6 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         __syncwarp();
         return done != 0;
       };
-      const bool live = r < count;
-      const int node = live ? (row0 + r) / rows.group : 0, head = kv_head * rows.group + (live ? (row0 + r) % rows.group : 0);
-      const int token = request.first + node;
-      const int first = first_visible_key(rows.positions[token], rows.window, rows.chunk);
-      const int* bits = rows.bits + (size_t)token * rows.words;
-      auto seen = [&](int key, int key_end) {
-        if (!live || key >= key_end) return false;
-        int place = key;
-        if (key >= span.past) {
-          const int n = key - span.past;
-          if (!((__ldg(bits + (n >> 5)) >> (n & 31)) & 1)) return false;
-          place = sm.node_position[n];
-        }
-        return place >= first || place < rows.keep_first;
-      };
-      // The keys of [key0, key0 + 64) that the row sees, a bit each.
-      auto seen64 = [&](int key0, int key_end) {
-        uint64_t mask = 0;
-        if (!live) return mask;
-        if (first == 0) {  // no window has moved: cached keys, then the row's mask
-          const int cached = min(max(span.past - key0, 0), 64);
-          if (cached > 0) mask = cached == 64 ? ~0ull : (1ull << cached) - 1;
-          const int skip = max(key0 - span.past, 0);  // new tokens before key0
-          const int there = min(64 - cached, key_end - max(key0, span.past));
-          if (there > 0) {
-            const int word = skip >> 5, shift = skip & 31;
-            auto load = [&](int w) { return w < rows.words ? (uint32_t)__ldg(bits + w) : 0u; };
-            const uint32_t w0 = load(word), w1 = load(word + 1), w2 = load(word + 2);
-            uint64_t draft = (uint64_t)__funnelshift_r(w0, w1, shift) | ((uint64_t)__funnelshift_r(w1, w2, shift) << 32);
-            if (there < 64) draft &= (1ull << there) - 1;
-            mask |= draft << cached;  // (cached < 64 here)
-          }
-        } else {
-          for (int i = 0; i < 64; ++i)
-            if (seen(key0 + i, key_end)) mask |= 1ull << i;
-        }
-        return mask;
-      };
       ok = wait_all(&sm.q_full, 0);
       const float times = E4M3 ? sm.q_times[r] : (rows.extras.cap > 0.f ? rows.extras.cap_pre : rows.scale_log2);
       const float cap = rows.extras.cap * 1.4426950408889634f;
@@ -469,7 +502,7 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         const int key0 = span.key0(j) + g * kTreeGroupKeys;
         const uint32_t s_addr = lane_base + s * kTreeKeys + g * kTreeGroupKeys;
         const bool whole = span.whole(j);
-        const uint64_t mask = whole ? ~0ull : seen64(key0, span.key_end(j));
+        const uint64_t mask = whole ? ~0ull : tree_seen64(sm, r, key0, span.key_end(j), rows.bits, rows.words, rows.keep_first);
         if (E4M3 && !wait_all(&sm.scale_full[slot], (n / kTreeScaleSlots) & 1)) { ok = false; break; }
         if (!wait_all(&sm.s_full[s], (n >> 1) & 1)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -613,9 +646,10 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
           l_all += sum * weight;
           f[u] = sm.row_out[u][r] == -INFINITY ? sum - sum : exp2_approx(sm.row_out[u][r] - at_most);
         }
-        const bool alone = parts.splits == 1;
+        const bool alone = parts.splits == 1, live = r < count;
+        const int token = max(sm.row_token[r], 0), head = kv_head * rows.group + (row0 + r) % rows.group;
         float inv = 1.f;
-        if (alone) inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
+        if (alone && live) inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
         const float f0 = f[0] * inv, f1 = f[1] * inv;
         constexpr int SIDE = D / 2;  // group g writes columns g * D / 2 ... of the row, from both accumulators
         const size_t part_row = ((size_t)token * rows.num_heads + head) * parts.splits + split;
@@ -628,21 +662,11 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
           float y[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(a[i]) * f0 + __uint_as_float(b[i]) * f1;
-          if (!E4M3 && sm.bad) {  // values that are not finite, for the rows that see them
-            for (int j = block0; j < block1; ++j) {
-              if (span.whole(j)) continue;
-              for (int key = span.key0(j); key < span.key0(j) + kTreeKeys; ++key) {
-                if (!seen(key, span.key_end(j))) continue;
-                const long long at = cache.row_of(table, key, kv_head);
-                if (at < 0) continue;
-                const __nv_bfloat16* value = reinterpret_cast<const __nv_bfloat16*>(cache.v) + (size_t)at * D + g * SIDE + c0;
+          if (!E4M3 && sm.bad && live) {  // values that are not finite, for the rows that see them
+            const __nv_bfloat16* values = reinterpret_cast<const __nv_bfloat16*>(cache.v);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float v = __bfloat162float(value[i]);
-                  if (!(fabsf(v) <= 3.402823466e38f)) y[i] += v;
-                }
-              }
-            }
+            for (int i = 0; i < 16; ++i)
+              y[i] += tree_not_finite(sm, r, g * SIDE + c0 + i, block0, block1, values, cache, table, kv_head, rows.bits, rows.words, rows.keep_first);
           }
           if (live && alone) {
             __nv_bfloat16* to = out + (size_t)token * out_stride + (size_t)head * D + g * SIDE + c0;
