@@ -33,6 +33,11 @@ values live in one device slab per group, indexed by those ids.
   inside its keys (``values_in_keys``: the latent rows of an attention through a latent) keeps
   keys only, and ``KvSlot.v`` is a view of their first columns.
 
+* A cache in eight bits (``cache_dtype=torch.float8_e4m3fn``) holds e4m3 numbers in its slabs and beside
+  them, per row of a token and kv head, a float32 scale: ``[slot, 2 (k|v), page, kv_head, page_size]``.
+* ``keep_places`` makes the rows of some of a request's newest places its next ones: what is left of a
+  tree of drafted tokens once a path of it has been accepted.
+
 With ``device=None`` the manager keeps only the bookkeeping (no slabs), which is
 what the scheduler tests and sizing estimates use.
 """
@@ -45,7 +50,7 @@ from typing import Callable, Mapping
 import numpy as np
 import torch
 
-from ..kernels.interface import KvSlot
+from ..kernels.interface import E4M3, KvSlot
 from ..parts.base import CacheNeed, StateNeed
 
 
@@ -59,10 +64,14 @@ def pages_needed(tokens: int, page_size: int) -> int:
     return 0 if tokens <= 0 else (tokens + page_size - 1) // page_size
 
 
-def pages_that_fit(cache_needs, page_size: int, element_size: int, budget_bytes: int) -> int:
+SCALE_BYTES = 8  # of a token and kv head in a cache in eight bits: a float32 for its key and one for its value
+
+
+def pages_that_fit(cache_needs, page_size: int, element_size: int, budget_bytes: int, row_bytes: int = 0) -> int:
     """How many pages per group ``budget_bytes`` of device memory hold (the spare page of every slab included
-    in the budget, not in the count): every cache slot keeps keys and values of its own for each page id."""
-    per_page = sum(need.num_kv_heads * need.row_elements * element_size * page_size for need in cache_needs.values())
+    in the budget, not in the count): every cache slot keeps keys and values of its own for each page id, and
+    ``row_bytes`` more for each token and kv head."""
+    per_page = sum(need.num_kv_heads * (need.row_elements * element_size + row_bytes) * page_size for need in cache_needs.values())
     if per_page <= 0:
         raise ValueError("the model declares no cache to size")
     return int(budget_bytes // per_page) - 1
@@ -100,8 +109,8 @@ class KvGroup:
         self._views: dict[int, KvSlot] = {}
         self._uploaded = None  # CUDA event after the last upload: the pinned table waits for it before it changes
 
-    def bytes_per_token(self, element_size: int) -> int:
-        return len(self.slots) * self.need.num_kv_heads * self.need.row_elements * element_size
+    def bytes_per_token(self, element_size: int, row_bytes: int = 0) -> int:
+        return len(self.slots) * self.need.num_kv_heads * (self.need.row_elements * element_size + row_bytes)
 
     # -- bookkeeping --------------------------------------------------------
     def first_needed_page(self, cached: int) -> int:
@@ -181,6 +190,12 @@ class KvGroup:
     # -- device side --------------------------------------------------------
     def allocate_device(self, dtype: torch.dtype, device: torch.device) -> None:
         rows = (self.num_pages + 1, self.need.num_kv_heads, self.page_size)
+        self._scales = None
+        if dtype == E4M3:
+            if self.need.values_in_keys:
+                raise ValueError("a cache in eight bits holds keys and values of their own: rows that are both (attention through a latent) "
+                                 "stay in the engine's type")
+            self._scales = torch.zeros((len(self.slots), 2, *rows), dtype=torch.float32, device=device)
         if self.need.values_in_keys:  # one row per token; a value is the head of its key's row
             self._keys = torch.zeros((len(self.slots), *rows, self.need.head_dim), dtype=dtype, device=device)
             self._values = self._keys[..., : self.need.v_dim]
@@ -212,11 +227,29 @@ class KvGroup:
                 self._uploaded = torch.cuda.Event()
             self._uploaded.record()
 
+    def move_rows(self, seat: int, sources: list[int], targets: list[int]) -> None:
+        """The rows of places ``sources`` of a seat, in every slot, to ``targets`` (all are read before any is written)."""
+        if self.device_table is None:
+            return
+        place = np.asarray([sources, targets], dtype=np.int64)
+        pages = self.host_table[seat, place // self.page_size].astype(np.int64)
+        if bool((pages < 0).any()):
+            raise ValueError(f"seat {seat} holds no page for some of the places {sources} and {targets}")
+        index = torch.from_numpy(np.stack([pages, place % self.page_size])).to(self.device_table.device)
+        (from_page, to_page), (from_row, to_row) = index[0], index[1]
+        held = [self._keys] if self.need.values_in_keys else [self._keys, self._values]
+        held = [t.view(torch.uint8) if t.dtype == E4M3 else t for t in held]  # (numbers of eight bits move as bytes)
+        if self._scales is not None:
+            held += [self._scales[:, 0], self._scales[:, 1]]
+        for rows in held:
+            rows[:, to_page, :, to_row] = rows[:, from_page, :, from_row]
+
     def slot_view(self, slot: int) -> KvSlot:
         view = self._views.get(slot)
         if view is None:
             index = self.slots.index(slot)
-            view = KvSlot(self._keys[index], self._values[index], self.device_table, self.page_size, self.num_pages + 1)
+            scales = (None, None) if self._scales is None else (self._scales[index, 0], self._scales[index, 1])
+            view = KvSlot(self._keys[index], self._values[index], self.device_table, self.page_size, self.num_pages + 1, *scales)
             self._views[slot] = view
         return view
 
@@ -233,6 +266,7 @@ class CacheManager:
         max_tokens_per_request: int,
         dtype: torch.dtype = torch.bfloat16,
         device=None,
+        cache_dtype: torch.dtype | None = None,  # None: ``dtype``; torch.float8_e4m3fn: eight bits and a scale per row
         pool_factory: Callable[[int], object] | None = None,
     ) -> None:
         if num_pages < 1 or page_size < 1 or max_seats < 1 or max_tokens_per_request < 1:
@@ -244,6 +278,9 @@ class CacheManager:
         self.pad_seat = max_seats
         self.max_tokens_per_request = max_tokens_per_request
         self.dtype = dtype
+        self.cache_dtype = cache_dtype if cache_dtype is not None else dtype
+        if self.cache_dtype not in (dtype, E4M3):
+            raise ValueError(f"a cache holds {dtype} or {E4M3}, not {cache_dtype}")
         self.device = torch.device(device) if device is not None else None
         width = pages_needed(max_tokens_per_request, page_size)
         by_need: dict[CacheNeed, list[int]] = {}
@@ -260,7 +297,7 @@ class CacheManager:
         self._open: set[int] = set()
         if self.device is not None:
             for group in self.groups:
-                group.allocate_device(dtype, self.device)
+                group.allocate_device(self.cache_dtype, self.device)
             def make(need: StateNeed) -> torch.Tensor:
                 return torch.zeros((max_seats + 1, *need.shape), dtype=need.dtype, device=self.device)
 
@@ -345,8 +382,27 @@ class CacheManager:
         return {i: g.pages_of(seat) for i, g in enumerate(self.groups)}
 
     def bytes_per_token(self) -> int:
-        size = torch.empty((), dtype=self.dtype).element_size()
-        return sum(g.bytes_per_token(size) for g in self.groups)
+        extra = SCALE_BYTES if self.cache_dtype == E4M3 else 0
+        return sum(g.bytes_per_token(self.cache_dtype.itemsize, extra) for g in self.groups)
+
+    def keep_places(self, seat: int, cached: int, places) -> int:
+        """Of the new tokens of a seat behind its first ``cached`` places, those at ``cached + place`` for the given places
+        (rising) stay, one behind the other from ``cached`` on; the others' rows may be written over.  Returns how many
+        tokens the seat holds then.  The work runs on the current stream, behind the step that wrote the rows."""
+        places = [int(p) for p in places]
+        if seat not in self._open:
+            raise ValueError(f"seat {seat} is not open")
+        if cached < 0 or any(p < 0 for p in places) or any(a >= b for a, b in zip(places, places[1:])):
+            raise ValueError(f"places to keep are rising numbers from 0 on, got {places} behind {cached}")
+        moved = [(cached + p, cached + i) for i, p in enumerate(places) if p != i]
+        if moved and cached + places[-1] >= self.max_tokens_per_request:
+            raise ValueError(f"place {cached + places[-1]} lies behind the longest request the tables hold ({self.max_tokens_per_request})")
+        if moved:
+            if self.state_needs:
+                raise ValueError("layers with per-request state cannot take back some of a step's tokens")
+            for group in self.groups:
+                group.move_rows(seat, *map(list, zip(*moved)))
+        return cached + len(places)
 
     # -- what a step sees -----------------------------------------------------
     def upload_tables(self, seats) -> None:

@@ -59,6 +59,8 @@ def _engine_options(parser: argparse.ArgumentParser) -> None:
     parser.add_argument("--max-seqs", type=int, default=None, help="requests running at once (default WORKER_MAX_SEQS or 32)")
     parser.add_argument("--token-budget", type=int, default=None, help="tokens per scheduler step (default WORKER_TOKEN_BUDGET or 2048)")
     parser.add_argument("--prefill-chunk", type=int, default=None, help="largest portion of a prompt in one step")
+    parser.add_argument("--cache-dtype", default="auto", choices=["auto", "float8_e4m3"],
+                        help="keys and values in the engine's dtype, or in eight bits with a scale per row")
     parser.add_argument("--max-model-len", type=int, default=None, help="longest request the block tables hold")
     parser.add_argument("--no-decode-graphs", action="store_true", help="keep pure-decode steps eager (WORKER_DECODE_GRAPHS=0)")
     parser.add_argument("--step-stats", type=int, default=None, help="log where step time goes every N steps (WORKER_STEP_STATS)")
@@ -72,7 +74,7 @@ def _load(args):
     knobs = dict(
         num_blocks=args.num_blocks, page_size=args.page_size, max_seqs=args.max_seqs, token_budget=args.token_budget,
         prefill_chunk=args.prefill_chunk, max_model_len=args.max_model_len, step_stats=args.step_stats,
-        gpu_mem_fraction=args.gpu_mem_fraction,
+        gpu_mem_fraction=args.gpu_mem_fraction, cache_dtype=args.cache_dtype,
     )
     if args.no_decode_graphs:
         knobs["decode_graphs"] = False

@@ -22,6 +22,8 @@ DEFAULT_MAX_SEQS = 32
 DEFAULT_TOKEN_BUDGET = 2048
 DEFAULT_PAGE_SIZE = 16
 
+CACHE_DTYPES = ("auto", "float8_e4m3")
+
 _DTYPE_NAMES = {
     "bf16": "bfloat16",
     "bfloat16": "bfloat16",
@@ -54,6 +56,7 @@ class EngineConfig:
     step_stats: int = 0
     device: str = "cuda:0"
     float32_weights: str = "auto"  # matrices stored in 32-bit under a 16-bit engine: "auto" | "keep" | "cast"
+    cache_dtype: str = "auto"  # keys and values: "auto" (the engine's dtype) or "float8_e4m3" (8 bits and a scale per row)
     gpu_mem_fraction: float | None = None  # size the cache from free device memory instead of num_blocks
 
     def __post_init__(self) -> None:
@@ -68,6 +71,8 @@ class EngineConfig:
             raise ValueError("gpu_mem_fraction must lie in (0, 1]")
         if self.float32_weights not in ("auto", "keep", "cast"):
             raise ValueError("float32_weights must be one of 'auto', 'keep', 'cast'")
+        if self.cache_dtype not in CACHE_DTYPES:
+            raise ValueError(f"cache_dtype must be one of {', '.join(CACHE_DTYPES)}; got {self.cache_dtype!r}")
         object.__setattr__(self, "dtype", resolve_dtype_name(self.dtype))
 
     @classmethod

@@ -20,6 +20,7 @@ from __future__ import annotations
 import fcntl
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -60,7 +61,6 @@ CUDA_UNITS: dict[str, list[str]] = {
     # caches in eight bits, trees of drafted tokens (both dtypes)
     "cached": ["cached_rows.cu", "attention_rows.cu", "attention_decode_e4m3.cu", "attention_tree_tcgen05.cu"],
 }
-_HEADERS = ["common.cuh", "recurrent.cuh", "cached_rows.cuh", "tcgen05.cuh", "softmax_pairs.cuh", "no_alloc.h"]
 
 
 class BuildError(RuntimeError):
@@ -114,6 +114,20 @@ def _digest(paths: list[str], flags: list[str]) -> str:
     return h.hexdigest()
 
 
+def _headers_of(paths: list[str]) -> list[str]:
+    """The headers of this folder that the files include, and those that these include, in the order they are met."""
+    found: list[str] = []
+    todo = list(paths)
+    while todo:
+        with open(todo.pop(0), encoding="utf-8") as handle:
+            for name in re.findall(r'^\s*#include "([^"]+)"', handle.read(), flags=re.MULTILINE):
+                path = os.path.join(HERE, name)
+                if path not in found and os.path.exists(path):
+                    found.append(path)
+                    todo.append(path)
+    return found
+
+
 def find_nvcc() -> str:
     for candidate in (os.environ.get("NVCC"), shutil.which("nvcc"), "/usr/local/cuda/bin/nvcc"):
         if candidate and os.path.exists(candidate):
@@ -154,7 +168,7 @@ def build_cuda_unit(name: str, verbose_ptxas: bool = False) -> str:
         raise BuildError(f"unknown kernel unit {name!r}")
     out_dir = build_dir()
     sources = [os.path.join(HERE, s) for s in CUDA_UNITS[name]]
-    headers = [os.path.join(HERE, h) for h in _HEADERS]
+    headers = _headers_of(sources)
     flags = NVCC_FLAGS + (["-Xptxas", "-v"] if verbose_ptxas else [])
     digest = _digest(sources + headers, flags)
     lib = os.path.join(out_dir, f"libdistie_{name}.so")

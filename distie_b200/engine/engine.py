@@ -24,10 +24,11 @@ from typing import Callable, Sequence
 
 import torch
 
-from ..cache.manager import CacheExhausted, CacheManager, pages_that_fit
+from ..cache.manager import SCALE_BYTES, CacheExhausted, CacheManager, pages_that_fit
 from ..config.engine_config import EngineConfig
 from ..config.registry import read_config
 from ..kernels import make_kernels
+from ..kernels.interface import E4M3, MOST_DRAFTED
 from ..models.decoder import DecoderModel, model_tensor_specs, slot_needs
 from ..weights.loader import open_weights
 from .batch import BatchEntry
@@ -60,6 +61,17 @@ class GenerationResult:
     time_to_first_token_ms: float = 0.0
     total_latency_ms: float = 0.0
     preemptions: int = 0
+
+
+@dataclass
+class DraftedGeneration:
+    """What :meth:`Engine.generate_drafted` made: the tokens, and how many steps and drafted tokens it took."""
+
+    token_ids: list[int] = field(default_factory=list)
+    finish_reason: str | None = None  # "eos" | "length"
+    steps: int = 0      # steps that checked drafted tokens (the prompt's are not counted)
+    drafted: int = 0    # drafted tokens that were checked
+    accepted: int = 0   # and those that became output
 
 
 @dataclass(frozen=True)
@@ -97,7 +109,7 @@ class Engine:
 
         ``knobs``: ``num_blocks`` or ``gpu_mem_fraction``, ``page_size``, ``max_seqs``, ``token_budget``,
         ``prefill_chunk``, ``max_model_len``, ``decode_graphs``, ``decode_ahead``, ``step_stats``,
-        ``float32_weights``; the reference's ``WORKER_*`` environment variables give the defaults.
+        ``float32_weights``, ``cache_dtype`` (``"float8_e4m3"``: keys and values in eight bits with a scale per row); the reference's ``WORKER_*`` environment variables give the defaults.
         """
         if device == "cuda":
             device = "cuda:0"
@@ -112,6 +124,8 @@ class Engine:
         (a model folder or a dict of tensors by checkpoint name) and a kernel set."""
         spec = arch.recipe(model_config)
         started = time.perf_counter()
+        if config.cache_dtype != "auto" and not getattr(kernels, "caches_in_8_bits", False):
+            raise ValueError(f"this kernel set serves no cache of {config.cache_dtype}")
         weights = open_weights(source, model_tensor_specs(spec), spec.tolerated, kernels.dtype, kernels.device,
                                config.float32_weights)
         decoder = DecoderModel(spec, kernels, weights)
@@ -329,6 +343,79 @@ class Engine:
         if on_token is not None:
             on_token(emission.seq.request_id, emission.token_id, emission.finished)
 
+    # -- drafted tokens -------------------------------------------------------
+    def generate_drafted(self, prompt_ids: Sequence[int], drafter: Callable[[list[int]], tuple[Sequence[int], Sequence[int]]],
+                         max_new_tokens: int = DEFAULT_MAX_TOKENS, eos_id: int | None | str = "config") -> DraftedGeneration:
+        """Greedy generation of one request that checks drafted tokens, several a step.
+
+        ``drafter(ids)`` is given all tokens so far and returns ``(tokens, parents)``: a tree of guesses at what follows,
+        ``parents[i]`` the index of token i's parent among them or -1 for a guess at the very next token (two empty lists:
+        no guess).  One step gives the arg-max behind the last token and behind every guess; the guesses that agree with it
+        become output, and what follows the last of them is the next token.  The output is the one that
+        :meth:`generate` gives at temperature 0, as far as the arithmetic of larger steps leaves the arg-max alone.
+        """
+        if not prompt_ids:
+            raise ValueError("prompt_ids must be non-empty")
+        limit = clamp_max_tokens(max_new_tokens)
+        longest = self.cache.max_tokens_per_request
+        if len(prompt_ids) + limit > longest:
+            raise CacheExhausted(f"{len(prompt_ids)} prompt tokens and {limit} new ones exceed the longest request ({longest})")
+        if eos_id == "config":
+            eos_id = getattr(self.model_config, "eos_token_id", None)
+        ids, made, seat = [int(t) for t in prompt_ids], DraftedGeneration(), self.cache.open_seat()
+        try:
+            cached, pick = 0, None
+            for at in range(0, len(ids), self.runner.max_step_tokens):
+                part = ids[at : at + self.runner.max_step_tokens]
+                if not self.cache.grow(seat, at + len(part)):
+                    raise CacheExhausted("out of KV blocks for the prompt")
+                logits = self.runner.step([BatchEntry(seat, part, at, (len(part) - 1,))])
+                cached = at + len(part)
+            pick = int(torch.argmax(logits[0]))
+            self.runner.finish_step()
+            while True:
+                ids.append(pick)
+                made.token_ids.append(pick)
+                if eos_id is not None and pick == eos_id:
+                    made.finish_reason = "eos"
+                elif len(made.token_ids) >= limit:
+                    made.finish_reason = "length"
+                if made.finish_reason:
+                    return made
+                tokens, parents = drafter(list(ids))
+                if len(tokens) != len(parents):
+                    raise ValueError(f"{len(tokens)} drafted tokens with {len(parents)} parents")
+                # No more than a step takes, the tables hold or the request still wants behind the token it has.
+                room = min(MOST_DRAFTED, self.runner.max_step_tokens, longest - cached) - 1
+                tokens, parents = [pick, *map(int, tokens[:room])], [-1, *(int(p) + 1 for p in parents[:room])]
+                if not self.cache.grow(seat, cached + len(tokens)):
+                    tokens, parents = tokens[:1], parents[:1]
+                    if not self.cache.grow(seat, cached + 1):
+                        raise CacheExhausted("out of KV blocks for the drafted tokens")
+                logits = self.runner.step([BatchEntry(seat, tokens, cached, tuple(range(len(tokens))), parents)])
+                picks = torch.argmax(logits, dim=-1).tolist()
+                self.runner.finish_step()
+                made.steps += 1
+                made.drafted += len(tokens) - 1
+                children: dict[tuple[int, int], int] = {}
+                for node in range(len(tokens) - 1, 0, -1):  # (of equal guesses the first one)
+                    children[parents[node], tokens[node]] = node
+                path = [0]
+                while len(made.token_ids) < limit - 1 and (path[-1], picks[path[-1]]) in children:
+                    node = children[path[-1], picks[path[-1]]]
+                    path.append(node)
+                    ids.append(tokens[node])
+                    made.token_ids.append(tokens[node])
+                    made.accepted += 1
+                    if tokens[node] == eos_id:
+                        made.finish_reason = "eos"
+                        return made
+                cached = self.cache.keep_places(seat, cached, path)
+                self.cache.trim(seat, cached)
+                pick = picks[path[-1]]
+        finally:
+            self.cache.close_seat(seat)
+
     # -- trace ----------------------------------------------------------------
     def trace(self, prompt_ids: Sequence[int], max_new_tokens: int, forced_ids: Sequence[int] | None = None) -> Trace:
         """One request through the step function, synchronously (torch_engine.py:295-338).
@@ -370,6 +457,10 @@ class Engine:
         return Trace(token_ids=picks, logits=torch.stack(rows))
 
 
+def cache_type(config: EngineConfig, torch_dtype: torch.dtype) -> torch.dtype:
+    return E4M3 if config.cache_dtype == "float8_e4m3" else torch_dtype
+
+
 def pages_from_free_memory(spec, config: EngineConfig, torch_dtype, device) -> int:
     """Pages that ``config.gpu_mem_fraction`` of the device memory free right now (the weights are loaded)
     holds, keys and values of every cache slot counted.  What is left over serves activations, the captured
@@ -380,8 +471,9 @@ def pages_from_free_memory(spec, config: EngineConfig, torch_dtype, device) -> i
         raise ValueError("gpu_mem_fraction sizes the cache from a CUDA device's free memory; give num_blocks on other devices")
     torch.cuda.empty_cache()
     free, _total = torch.cuda.mem_get_info(device)
-    element = torch.empty((), dtype=torch_dtype).element_size()
-    pages = pages_that_fit(cache_needs, config.page_size, element, int(free * float(config.gpu_mem_fraction)))
+    cache_dtype = cache_type(config, torch_dtype)
+    pages = pages_that_fit(cache_needs, config.page_size, cache_dtype.itemsize, int(free * float(config.gpu_mem_fraction)),
+                           SCALE_BYTES if cache_dtype == E4M3 else 0)
     if pages < 1:
         raise CacheExhausted(f"{config.gpu_mem_fraction} of the {free >> 20} MiB that are free hold not one page of cache")
     _log.info("cache sized from free memory free_mib=%s fraction=%s pages=%s", free >> 20, config.gpu_mem_fraction, pages)
@@ -402,4 +494,5 @@ def build_cache(spec, config: EngineConfig, torch_dtype, device) -> CacheManager
         max_tokens_per_request=longest,
         dtype=torch_dtype,
         device=device,
+        cache_dtype=cache_type(config, torch_dtype),
     )

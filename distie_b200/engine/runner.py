@@ -23,6 +23,7 @@ from typing import Sequence
 import numpy as np
 import torch
 
+from ..kernels.interface import MOST_DRAFTED
 from ..sampling.sampler import Sampler, uniform
 from .batch import BatchEntry, StepLayout, StepStaging, lay_out, views
 
@@ -84,7 +85,9 @@ class ModelRunner:
         self.sampler = Sampler(self.kernels)
         self.max_step_tokens = max_step_tokens
         self.max_seqs = max_seqs
-        self.staging = StepStaging(5 * max_step_tokens + 3 * max_seqs, self.device)
+        # (a step of drafted tokens: a place and up to MOST_DRAFTED bits more a token, three numbers more a request)
+        self.staging = StepStaging((6 + MOST_DRAFTED // 32) * max_step_tokens + 6 * max_seqs, self.device)
+        self._takes_trees = getattr(self.kernels, "drafted_tokens", False) and all(getattr(block, "tree_safe", False) for block in model.blocks)
         self._floats_host = [
             torch.zeros(2 * max_seqs, dtype=torch.float32, pin_memory=self.device.type == "cuda") for _ in range(2)
         ]
@@ -101,7 +104,13 @@ class ModelRunner:
     # -- the step function ----------------------------------------------------
     @torch.inference_mode()
     def step(self, entries: Sequence[BatchEntry]) -> torch.Tensor | None:
-        if self.use_graphs and len(entries) <= self._sizes[-1] and all(len(e.tokens) == 1 for e in entries):
+        """Logits at the wanted places, in the order of entries and of ``want``.  Entries with ``parents`` make it a step of
+        drafted tokens, for models all of whose layers are plain attention: the rows of all their tokens are in
+        the cache afterwards, at the places behind the request's cached ones (``CacheManager.keep_places`` takes the accepted ones)."""
+        drafted = any(entry.parents is not None for entry in entries)
+        if drafted and not self._takes_trees:
+            raise ValueError("drafted tokens branch: layers with per-request state and attention through a latent do not take them")
+        if not drafted and self.use_graphs and len(entries) <= self._sizes[-1] and all(len(e.tokens) == 1 for e in entries):
             logits = self._graph_logits(entries)
             if logits is not NotImplemented:
                 return logits

@@ -13,10 +13,9 @@ import ctypes
 
 import torch
 
-from .interface import MOST_DRAFTED, KvSlot, first_visible
+from .interface import E4M3, MOST_DRAFTED, KvSlot, first_visible
 from .library import KernelError, check, function
 
-E4M3 = torch.float8_e4m3fn
 _CACHE_CODE = {torch.float32: 0, torch.bfloat16: 1, E4M3: 2}
 _READ_ROWS = 256  # requests that one launch reads back
 
@@ -38,6 +37,9 @@ def tree_splits(tiles: int, blocks: int, sms: int) -> int:
 
 
 class CachedRows:
+    caches_in_8_bits = True
+    drafted_tokens = True
+
     @staticmethod
     def _apart(step, kv) -> bool:
         """Whether new rows go to their places by the kernel here: an 8-bit slot, or places that are not the positions."""

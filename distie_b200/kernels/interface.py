@@ -39,6 +39,7 @@ Q_TILE = 128  # tokens per tile of StepTensors.q_tiles
 
 
 MOST_DRAFTED = 256  # new tokens of one request that a step of drafted tokens takes
+E4M3 = torch.float8_e4m3fn  # the numbers of a cache in eight bits
 
 
 @dataclass
@@ -178,6 +179,8 @@ class RotaryTable:
 class KernelSet(ABC):
     dtype: torch.dtype
     device: torch.device
+    caches_in_8_bits = False  # whether the set writes and reads slots in eight bits
+    drafted_tokens = False    # whether it takes steps with a DraftTree
 
     @abstractmethod
     def embed(self, step: StepTensors, table: torch.Tensor, residual: torch.Tensor) -> None:

@@ -82,6 +82,7 @@ class GqaAttention:
         self.norm_first = params.get("norm_first")
         self.q_temp = tuple(params["q_temp"]) if params.get("q_temp") else None
         self.taps = int(params.get("conv") or 0)
+        self.tree_safe = self.taps <= 1  # (a convolution's state moves on by every token of the step)
         self.gate_kind = params.get("gate")
         extras = extras or {}
         self.sink = extras.get("sink")

@@ -41,6 +41,11 @@ class PreNormBlock:
         """False when a part reads host-side batch data, which a captured step cannot replay."""
         return all(getattr(part, "graph_safe", True) for part in (self.mixer, self.feed_forward))
 
+    @property
+    def tree_safe(self) -> bool:
+        """Whether the mixer takes steps of drafted tokens (what else a block does, it does token by token)."""
+        return self.mixer is None or getattr(self.mixer, "tree_safe", False)
+
     @classmethod
     def tensor_specs(cls, layer: LayerSpec, hidden_size: int) -> list[TensorSpec]:
         return (
@@ -89,6 +94,11 @@ class ParallelBlock:
     @property
     def graph_safe(self) -> bool:
         return all(getattr(part, "graph_safe", True) for part in (self.mixer, self.feed_forward))
+
+    @property
+    def tree_safe(self) -> bool:
+        """Whether the mixer takes steps of drafted tokens (what else a block does, it does token by token)."""
+        return self.mixer is None or getattr(self.mixer, "tree_safe", False)
 
     @classmethod
     def tensor_specs(cls, layer: LayerSpec, hidden_size: int) -> list[TensorSpec]:
@@ -141,6 +151,11 @@ class SandwichBlock:
     @property
     def graph_safe(self) -> bool:
         return all(getattr(part, "graph_safe", True) for part in (self.mixer, self.feed_forward) if part is not None)
+
+    @property
+    def tree_safe(self) -> bool:
+        """Whether the mixer takes steps of drafted tokens (what else a block does, it does token by token)."""
+        return self.mixer is None or getattr(self.mixer, "tree_safe", False)
 
     @staticmethod
     def _has_ff(layer: LayerSpec) -> bool:

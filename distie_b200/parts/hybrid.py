@@ -41,6 +41,10 @@ class SideBySide:
     def graph_safe(self) -> bool:
         return all(getattr(part, "graph_safe", True) for part in (self.left, self.right))
 
+    @property
+    def tree_safe(self) -> bool:
+        return all(getattr(part, "tree_safe", False) for part in (self.left, self.right))
+
     @classmethod
     def tensor_specs(cls, spec: PartSpec, hidden_size: int) -> list[TensorSpec]:
         return [t for _, part in _sides(spec) for t in MIXERS.get(part.kind).tensor_specs(part, hidden_size)]
