@@ -169,6 +169,200 @@ rows_write_kernel(RowsInput in, RowsNorm norm, RowsTurn turn, RowsPlace place, T
   }
 }
 
+// The same for heads of 64 and 128 whose keys and values are of one size, turned whole (pairs half a head apart) or not at
+// all, from float32: D / 16 lanes a row, a lane 8 elements and the 8 that are turned with them.  A block takes as many tokens
+// as make one wave of blocks, up to 8, and walks their rows in one go, a lane's next row on its way: the tokens'
+// places, three loads that hang on one another, and their angles, one a thread, are then paid for once a block.  Where tokens
+// are few, a token's rows are spread over several blocks.  Behind the bytes (2,048 tokens of 40 and 8 heads of 128: 80 MB)
+// the instructions set the pace.
+constexpr int kFastThreads = 256, kFastTokens = 8, kFastBlocksPerSm = 3;
+
+template <typename T, int CACHE, int D>
+__global__ void __launch_bounds__(kFastThreads, kFastBlocksPerSm)
+rows_write_fast_kernel(RowsInput in, RowsNorm norm, RowsTurn turn, RowsPlace place, T* __restrict__ q_out, int q_out_stride,
+                       CachePages cache, void* k_out, void* v_out, float* __restrict__ k_scale, float* __restrict__ v_scale, int tokens,
+                       int per_block, int num_heads, int num_kv_heads, int write, int* __restrict__ error) {
+  constexpr int LANES = D / 16, HALF = D / 2, PART = D / 4, ROWS = kFastThreads / LANES;
+  constexpr unsigned ALL = 0xffffffffu;
+  __shared__ __align__(16) float cos_s[kFastTokens][HALF], sin_s[kFastTokens][HALF];
+  __shared__ long long place_s[kFastTokens];  // of kv head 0; -1: none
+  __shared__ float temperature_s[kFastTokens];
+  const int t0 = blockIdx.x * per_block, count = min(per_block, tokens - t0), e0 = (threadIdx.x % LANES) * 4;
+  const int k_row = num_heads, v_row = num_heads + num_kv_heads, rows_here = num_heads + (write ? 2 * num_kv_heads : 0);
+  const int step = gridDim.y * ROWS, total = count * rows_here;
+  const int passes = (total - (int)blockIdx.y * ROWS + step - 1) / step;  // the same for every thread of the block
+  grid_dependency_release();
+  // Elements e0 .. + 3 and PART + e0 .. + 3 of the row, then their partners HALF further on.
+  struct Row {
+    float4 x[4];
+    int token, row;  // of the block's tokens, of the token's rows
+  };
+  auto load = [&](Row& r) {  // a row as projected (behind the last one: a row of the last token, so that no load hangs on a branch)
+    const bool is_query = r.row < k_row, is_value = r.row >= v_row;
+    const bool own = is_value && in.v != nullptr;
+    const float* rows = reinterpret_cast<const float*>(is_query ? in.q : own ? in.v : in.k);
+    const int stride = is_query ? in.q_stride : own ? in.v_stride : in.k_stride;
+    const int head = r.row - (is_query ? 0 : is_value ? v_row : k_row);
+    const float* from = rows + (size_t)(t0 + min(r.token, count - 1)) * stride + head * D + e0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.x[i] = load4_cg(from + i * PART);
+    for (int s = 1; s < in.splits; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 more = load4_cg(from + s * in.split_stride + i * PART);
+        r.x[i].x += more.x; r.x[i].y += more.y; r.x[i].z += more.z; r.x[i].w += more.w;
+      }
+  };
+  auto advance = [&](Row& r, int by) {
+    r.row += by;
+    while (r.row >= rows_here) {
+      r.row -= rows_here;
+      ++r.token;
+    }
+  };
+  Row held[2];
+  grid_dependency_wait();  // the projection comes from the kernel before this one
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    held[u].token = 0;
+    held[u].row = blockIdx.y * ROWS + threadIdx.x / LANES;
+    advance(held[u], u * step);
+    load(held[u]);
+  }
+  // While they are on their way: the tokens' places and angles.
+  if (threadIdx.x / 32 < count && threadIdx.x % 32 == 0) {
+    const int mine = threadIdx.x / 32, t = t0 + mine, position = place.positions[t];
+    long long row = -1;
+    if (write) {
+      const int seat = place.seq_seat[place.token_seq[t]], slot = place.slots ? place.slots[t] : position;
+      row = slot < 0 ? -1 : cache.row_of(cache.block_table + (size_t)seat * cache.table_width, slot, 0);
+      if (row < 0 && blockIdx.y == 0 && error) atomicExch(error, 2);
+    }
+    place_s[mine] = row;
+    temperature_s[mine] =
+        turn.temp_every > 0.f ? 1.f + turn.temp_coef * logf(floorf((float)(position + 1) / turn.temp_every) + 1.f) : 1.f;
+  }
+  if (turn.inv_freq) {
+    for (int i = threadIdx.x; i < count * HALF; i += kFastThreads) {
+      float sn, cs;
+      exact_angle(place.positions[t0 + i / HALF], turn.inv_freq[i % HALF], sn, cs);
+      cos_s[i / HALF][i % HALF] = cs * turn.factor;
+      sin_s[i / HALF][i % HALF] = sn * turn.factor;
+    }
+  }
+  __syncthreads();
+  auto finish = [&](Row& r) {
+    const bool live = r.token < count, is_query = r.row < k_row, is_value = r.row >= v_row;
+    const int token = min(r.token, count - 1), head = r.row - (is_query ? 0 : is_value ? v_row : k_row);
+    const float* bias = is_query ? in.q_bias : is_value && in.v != nullptr ? in.v_bias : in.k_bias;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[4 * i] = r.x[i].x; v[4 * i + 1] = r.x[i].y; v[4 * i + 2] = r.x[i].z; v[4 * i + 3] = r.x[i].w;
+    }
+    if (bias) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>(bias + head * D + e0 + i * PART));
+        v[4 * i] += b.x; v[4 * i + 1] += b.y; v[4 * i + 2] += b.z; v[4 * i + 3] += b.w;
+      }
+    }
+    auto unit = [&]() {  // (all lanes: a warp's rows may be of several kinds)
+      float squares = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) squares += v[e] * v[e];
+#pragma unroll
+      for (int d = LANES / 2; d >= 1; d >>= 1) squares += __shfl_xor_sync(ALL, squares, d);
+      const float u = is_value ? 1.f : rsqrtf(squares / (float)D + norm.eps);
+      const float* weight = is_query ? norm.q_weight : norm.k_weight;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float4 w = make_float4(u, u, u, u);
+        if (weight && !is_value) {
+          const float4 given = __ldg(reinterpret_cast<const float4*>(weight + e0 + i * PART));
+          w = make_float4(u * given.x, u * given.y, u * given.z, u * given.w);
+        }
+        v[4 * i] *= w.x; v[4 * i + 1] *= w.y; v[4 * i + 2] *= w.z; v[4 * i + 3] *= w.w;
+      }
+    };
+    if (norm.mode == 1) unit();
+    if (turn.inv_freq && !is_value) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 cs = load4(&cos_s[token][e0 + i * PART]), sn = load4(&sin_s[token][e0 + i * PART]);
+        const float c[4] = {cs.x, cs.y, cs.z, cs.w}, s[4] = {sn.x, sn.y, sn.z, sn.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = v[4 * i + e], b = v[8 + 4 * i + e];
+          v[4 * i + e] = a * c[e] - b * s[e];
+          v[8 + 4 * i + e] = b * c[e] + a * s[e];
+        }
+      }
+    }
+    if (norm.mode == 2) unit();
+    if (__any_sync(ALL, !is_query)) {
+      const long long row = place_s[token] + (long long)head * cache.page_size;
+      const bool there = live && !is_query && place_s[token] >= 0;
+      void* out = is_value ? v_out : k_out;
+      if (CACHE == DISTIE_E4M3) {
+        float most = 0.f, nothing = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          most = fmaxf(most, fabsf(v[e]));
+          nothing += v[e] * 0.f;  // NaN where an element is not finite
+        }
+#pragma unroll
+        for (int d = LANES / 2; d >= 1; d >>= 1) {
+          most = fmaxf(most, __shfl_xor_sync(ALL, most, d));
+          nothing += __shfl_xor_sync(ALL, nothing, d);
+        }
+        if (there) {
+          const bool bad = nothing != nothing;
+          const float scale = row_scale(most, bad);
+          if (e0 == 0) (is_value ? v_scale : k_scale)[row] = scale;
+          if (scale >= 1e-37f) {  // (the reciprocal of a smaller one is not a number)
+            const float inv = 1.f / scale;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] *= inv;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = bad || scale == 0.f ? 0.f : v[e] / scale;
+          }
+          uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(out) + (size_t)row * D + e0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            to[i * PART / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
+                               (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
+        }
+      } else if (there) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 part = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          if (CACHE == DISTIE_BF16) store4(reinterpret_cast<__nv_bfloat16*>(out) + (size_t)row * D + e0 + i * PART, part);
+          else store4(reinterpret_cast<float*>(out) + (size_t)row * D + e0 + i * PART, part);
+        }
+      }
+    }
+    if (live && is_query) {
+      const float times = temperature_s[token];
+      T* to = q_out + (size_t)(t0 + token) * q_out_stride + head * D + e0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4(to + i * PART, make_float4(v[4 * i] * times, v[4 * i + 1] * times, v[4 * i + 2] * times, v[4 * i + 3] * times));
+    }
+  };
+  for (int pass = 0; pass < passes; pass += 2) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {  // (a row that moved from one place to the other would be waited for)
+      if (pass + u < passes) {
+        finish(held[u]);
+        advance(held[u], 2 * step);
+        load(held[u]);
+      }
+    }
+  }
+}
+
 // ---- read back ----------------------------------------------------------------------------------------------------
 // Pages of up to kReadRows requests, one page of the result per block: numbers times scales in the set's type, zeros behind
 // a request's last row.  A page of the cache is one run of memory over all kv heads, and so is a page of the result.
@@ -194,44 +388,18 @@ __device__ __forceinline__ void store_row16(T* to, const float (&v)[16]) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void read_rows(const uint8_t* __restrict__ numbers, const float* __restrict__ scales, T* __restrict__ to,
-                                          int rows, int dim, int page_size, int live) {
-  if ((dim & 15) == 0) {
-    const int pieces = rows * (dim / 16);
-    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
-      const int row = i / (dim / 16);
-      float v[16];
-      if (row % page_size < live) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(numbers + (size_t)i * 16);
-        const float s = scales[row];
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float f[4];
-          e4m3x4_to_float(w[j], f);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * j + e] = f[e] * s;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = 0.f;
-      }
-      store_row16(to + (size_t)i * 16, v);
-    }
-  } else {
-    for (int i = threadIdx.x; i < rows * dim; i += blockDim.x) {
-      const int row = i / dim;
-      to[i] = from_float<T>(row % page_size < live ? e4m3_to_float(numbers[i]) * scales[row] : 0.f);
-    }
-  }
-}
+constexpr int kReadThreads = 256;
+constexpr int kReadPieces = 4;  // 16 numbers each, per thread: all requested before the first is stored
 
+// A block takes kReadThreads * kReadPieces pieces of a page (blockIdx.y: which of them, K's first, then V's).
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kReadThreads)
 rows_read_kernel(const __grid_constant__ ReadPlan plan, CachePages cache, const int* __restrict__ seq_seat, T* __restrict__ k_out,
                  T* __restrict__ v_out, int* __restrict__ table_out, int page0, int pages, int* __restrict__ error) {
+  grid_dependency_release();
   if ((int)blockIdx.x >= pages) {  // blocks behind the pages: a row of the result's table each
+    if (blockIdx.y > 0) return;
+    grid_dependency_wait();
     const int i = blockIdx.x - pages;
     const int columns = (plan.length[i] + cache.page_size - 1) / cache.page_size;
     int* row = table_out + (size_t)seq_seat[plan.batch_row[i]] * cache.table_width;
@@ -248,17 +416,57 @@ rows_read_kernel(const __grid_constant__ ReadPlan plan, CachePages cache, const 
   if (column >= plan.hole[i] && column < plan.hole_end[i]) return;  // (no table entry names this page of the result)
   const int seat = seq_seat[plan.batch_row[i]];
   const int page = column < cache.table_width ? cache.block_table[(size_t)seat * cache.table_width + column] : -1;
-  int live = min(cache.page_size, plan.length[i] - column * cache.page_size);
-  if (page < 0 || page >= cache.num_pages) {
-    if (threadIdx.x == 0 && error) atomicExch(error, 5);
-    live = 0;
-  }
+  const bool held = page >= 0 && page < cache.num_pages;
+  const int live = held ? min(cache.page_size, plan.length[i] - column * cache.page_size) : 0;
   const int rows = cache.num_kv_heads * cache.page_size;
-  const size_t from = (size_t)max(page, 0) * rows, to = (size_t)page_out * rows;
-  read_rows(reinterpret_cast<const uint8_t*>(cache.k) + from * cache.key_dim, cache.k_scale + from, k_out + to * cache.key_dim, rows,
-            cache.key_dim, cache.page_size, live);
-  read_rows(reinterpret_cast<const uint8_t*>(cache.v) + from * cache.value_dim, cache.v_scale + from, v_out + to * cache.value_dim, rows,
-            cache.value_dim, cache.page_size, live);
+  const size_t from = (size_t)(held ? page : 0) * rows, to = (size_t)page_out * rows;
+  grid_dependency_wait();  // the newest rows come from the kernels before this one
+  if (!held && threadIdx.x == 0 && blockIdx.y == 0 && error) atomicExch(error, 5);
+  auto live_row = [&](int row) { return (cache.page_shift >= 0 ? row & (cache.page_size - 1) : row % cache.page_size) < live; };
+  if (((cache.key_dim | cache.value_dim) & 15) == 0) {
+    const int k_pieces = rows * (cache.key_dim / 16), all = k_pieces + rows * (cache.value_dim / 16);
+    const int first = blockIdx.y * kReadThreads * kReadPieces + threadIdx.x;
+    uint4 raw[kReadPieces];
+    float scale[kReadPieces];
+    int row[kReadPieces];
+#pragma unroll
+    for (int u = 0; u < kReadPieces; ++u) {  // (every piece is loaded, those behind the last one as copies of it)
+      const int p = min(first + u * kReadThreads, all - 1);
+      const bool is_v = p >= k_pieces;
+      const int piece = is_v ? p - k_pieces : p, dim = is_v ? cache.value_dim : cache.key_dim;
+      row[u] = piece / (dim / 16);
+      raw[u] = load16_cg(reinterpret_cast<const uint8_t*>(is_v ? cache.v : cache.k) + from * dim + (size_t)piece * 16);
+      scale[u] = __ldcg((is_v ? cache.v_scale : cache.k_scale) + from + row[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kReadPieces; ++u) {
+      const int p = first + u * kReadThreads;
+      if (p >= all) break;
+      const bool is_v = p >= k_pieces, there = live_row(row[u]);
+      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[4];
+        e4m3x4_to_float(w[j], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * j + e] = there ? f[e] * scale[u] : 0.f;
+      }
+      const int piece = is_v ? p - k_pieces : p;
+      store_row16((is_v ? v_out + to * cache.value_dim : k_out + to * cache.key_dim) + (size_t)piece * 16, v);
+    }
+  } else if (blockIdx.y == 0) {
+    for (int which = 0; which < 2; ++which) {
+      const int dim = which ? cache.value_dim : cache.key_dim;
+      const uint8_t* numbers = reinterpret_cast<const uint8_t*>(which ? cache.v : cache.k) + from * dim;
+      const float* scales = (which ? cache.v_scale : cache.k_scale) + from;
+      T* out = (which ? v_out : k_out) + to * dim;
+      for (int e = threadIdx.x; e < rows * dim; e += blockDim.x) {
+        const int row = e / dim;
+        out[e] = from_float<T>(live_row(row) ? e4m3_to_float(numbers[e]) * scales[row] : 0.f);
+      }
+    }
+  }
 }
 
 template <typename IN, typename T, int CACHE>
@@ -266,6 +474,29 @@ static int launch_write(const RowsInput& in, const RowsNorm& norm, const RowsTur
                         int q_out_stride, const CachePages& cache, void* k_out, void* v_out, float* k_scale, float* v_scale,
                         int tokens, int num_heads, int num_kv_heads, int write, int* error, cudaStream_t stream) {
   const int rows = num_heads + (write ? 2 * num_kv_heads : 0);
+  const int dim = cache.key_dim;
+  auto aligned = [](const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; };
+  if (sizeof(IN) == 4 && (dim == 64 || dim == 128) && cache.value_dim == dim &&
+      (turn.rotary_dim == 0 || (turn.rotary_dim == dim && !turn.interleaved)) && !((in.q_stride | in.k_stride | in.v_stride) & 3) &&
+      !(in.split_stride & 3) && !(q_out_stride & 3) && aligned(in.q, 16) && aligned(in.k, 16) && aligned(in.v, 16) && aligned(in.q_bias, 16) &&
+      aligned(in.k_bias, 16) && aligned(in.v_bias, 16) && aligned(norm.q_weight, 16) && aligned(norm.k_weight, 16) && aligned(q_out, 16) &&
+      aligned(k_out, 16) && aligned(v_out, 16)) {
+    static int sms = 0;
+    if (sms == 0) {
+      int device = 0;
+      if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 1)
+        sms = 148;
+    }
+    const int wave = sms * kFastBlocksPerSm, blocks_a_token = (rows * dim / 16 + kFastThreads - 1) / kFastThreads;
+    const int per_block = min(kFastTokens, (tokens + wave - 1) / wave);
+    const dim3 fast((tokens + per_block - 1) / per_block, max(1, min(blocks_a_token, wave / tokens)));
+#define DISTIE_ROWS_FAST(D)                                                                                                            \
+  return (int)launch_dependent(rows_write_fast_kernel<T, CACHE, D>, fast, dim3(kFastThreads), 0, stream, in, norm, turn, place, (T*)q_out, \
+                               q_out_stride, cache, k_out, v_out, k_scale, v_scale, tokens, per_block, num_heads, num_kv_heads, write, error)
+    if (dim == 64) DISTIE_ROWS_FAST(64);
+    DISTIE_ROWS_FAST(128);
+#undef DISTIE_ROWS_FAST
+  }
   const dim3 grid(tokens, tokens < 512 ? (rows + kWriteWarps - 1) / kWriteWarps : 1);
   const size_t shared = ((size_t)kWriteWarps * max(cache.key_dim, cache.value_dim) + turn.rotary_dim) * sizeof(float);
   rows_write_kernel<IN, T, CACHE><<<grid, kWriteWarps * 32, shared, stream>>>(in, norm, turn, place, (T*)q_out, q_out_stride, cache, k_out,
@@ -327,7 +558,8 @@ extern "C" int distie_rows_read(const int* plan, int count, const void* k_cache,
                                 int key_dim, int value_dim, int page_size, int num_pages, void* k_out, void* v_out, int* table_out,
                                 int page0, int pages, int out_type, int* error, cudaStream_t stream) {
   if (count <= 0 || pages <= 0) return 0;
-  if (count > kReadRows || num_kv_heads < 1 || key_dim < 1 || value_dim < 1 || page_size < 1 || table_width < 1 || k_scale == nullptr || v_scale == nullptr)
+  if (count > kReadRows || num_kv_heads < 1 || key_dim < 1 || value_dim < 1 || page_size < 1 || table_width < 1 || k_scale == nullptr || v_scale == nullptr ||
+      (long long)num_kv_heads * page_size * (key_dim + value_dim) > 1 << 30)
     return DISTIE_ERR_ARG;
   ReadPlan p;
   p.count = count;
@@ -341,14 +573,14 @@ extern "C" int distie_rows_read(const int* plan, int count, const void* k_cache,
   }
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, key_dim, value_dim,
                                       page_size, num_pages);
+  const long long pieces = (long long)num_kv_heads * page_size * (key_dim / 16 + value_dim / 16);
+  const int per_block = kReadThreads * kReadPieces;
+  const dim3 grid(pages + count, ((key_dim | value_dim) & 15) == 0 ? (unsigned)((pieces + per_block - 1) / per_block) : 1);
   if (out_type == DISTIE_BF16)
-    rows_read_kernel<<<pages + count, 256, 0, stream>>>(p, cache, seq_seat, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, table_out,
-                                                        page0, pages, error);
-  else if (out_type == DISTIE_F32)
-    rows_read_kernel<<<pages + count, 256, 0, stream>>>(p, cache, seq_seat, (float*)k_out, (float*)v_out, table_out, page0, pages,
-                                                        error);
-  else
-    return DISTIE_ERR_UNSUPPORTED;
-  DISTIE_LAUNCH_CHECK();
-  return 0;
+    return (int)launch_dependent(rows_read_kernel<__nv_bfloat16>, grid, dim3(kReadThreads), 0, stream, p, cache, seq_seat, (__nv_bfloat16*)k_out,
+                                 (__nv_bfloat16*)v_out, table_out, page0, pages, error);
+  if (out_type == DISTIE_F32)
+    return (int)launch_dependent(rows_read_kernel<float>, grid, dim3(kReadThreads), 0, stream, p, cache, seq_seat, (float*)k_out, (float*)v_out,
+                                 table_out, page0, pages, error);
+  return DISTIE_ERR_UNSUPPORTED;
 }
