@@ -24,6 +24,7 @@
 #include <cuda_fp16.h>
 
 #include "cached_rows.cuh"
+#include "packed.h"
 
 namespace distie {
 
@@ -518,3 +519,5 @@ extern "C" int distie_attention_decode_e4m3(const void* q, int q_stride, void* o
   if (splits > 1 && !cluster_merge) return rows_merge_bf16(parts, out, out_stride, tokens, num_heads, head_dim, sink, stream);
   return 0;
 }
+
+DISTIE_PACKED(distie_attention_decode_e4m3)

@@ -9,6 +9,7 @@
 #include <cuda_fp16.h>
 
 #include "cached_rows.cuh"
+#include "packed.h"
 
 namespace distie {
 
@@ -303,3 +304,5 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
 #undef DISTIE_ROWS
   return DISTIE_ERR_UNSUPPORTED;
 }
+
+DISTIE_PACKED(distie_attention_rows)

@@ -33,6 +33,7 @@
 #include <cuda_fp16.h>
 
 #include "cached_rows.cuh"
+#include "packed.h"
 #include "softmax_pairs.cuh"
 #include "tcgen05.cuh"
 
@@ -745,3 +746,5 @@ extern "C" int distie_attention_tree_tcgen05(const void* q, int q_stride, void* 
   if (status != 0 || splits == 1) return status;
   return rows_merge_bf16(parts, out, out_stride, tokens, num_heads, head_dim, sink, stream);
 }
+
+DISTIE_PACKED(distie_attention_tree_tcgen05)

@@ -3,6 +3,7 @@
 #include <cuda_fp16.h>
 
 #include "cached_rows.cuh"
+#include "packed.h"
 
 namespace distie {
 
@@ -584,3 +585,6 @@ extern "C" int distie_rows_read(const int* plan, int count, const void* k_cache,
                                  table_out, page0, pages, error);
   return DISTIE_ERR_UNSUPPORTED;
 }
+
+DISTIE_PACKED(distie_rows_write)
+DISTIE_PACKED(distie_rows_read)

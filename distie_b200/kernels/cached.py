@@ -14,14 +14,14 @@ import ctypes
 import torch
 
 from .interface import E4M3, MOST_DRAFTED, KvSlot, first_visible
-from .library import KernelError, check, function
+from .library import KernelError, check, function, packed
 
 _CACHE_CODE = {torch.float32: 0, torch.bfloat16: 1, E4M3: 2}
 _READ_ROWS = 256  # requests that one launch reads back
 
 
-def _ptr(x):
-    return x.data_ptr() if x is not None else None
+def _ptr(x) -> int:
+    return x.data_ptr() if x is not None else 0
 
 
 def tree_splits(tiles: int, blocks: int, sms: int) -> int:
@@ -46,7 +46,12 @@ class CachedRows:
         return kv is not None and (kv.k_scale is not None or step.slots is not None)
 
     def _check_slot(self, what: str, kv, num_kv_heads: int, key_dim: int, value_dim: int) -> int:
-        """The slot's element type code, after a look at what the kernels take for granted."""
+        """The slot's element type code, after a look at what the kernels take for granted.  A slot is handed to every step of a
+        request's life: the look is taken once for its tensors and sizes."""
+        seen = kv.__dict__.get("_seen")
+        if seen is not None and seen[0] is kv.k and seen[1] is kv.v and seen[2] is kv.block_table and seen[3] is kv.k_scale \
+                and seen[4] is kv.v_scale and seen[5] == (kv.num_pages, kv.page_size, num_kv_heads, key_dim, value_dim, self.dtype):
+            return seen[6]
         if kv.k.dtype != kv.v.dtype or (kv.k.dtype != self.dtype and kv.k.dtype != E4M3):
             raise KernelError(f"{what}: a cache of {self.dtype} or {E4M3} is expected, not of {kv.k.dtype}")
         rows = (kv.num_pages, num_kv_heads, kv.page_size)
@@ -61,41 +66,38 @@ class CachedRows:
         for scale in (kv.k_scale, kv.v_scale):
             if scale is not None and (scale.dtype != torch.float32 or tuple(scale.shape) != rows or not scale.is_contiguous()):
                 raise KernelError(f"{what}: contiguous float32 scales {rows} are expected")
-        return _CACHE_CODE[kv.k.dtype]
+        code = _CACHE_CODE[kv.k.dtype]
+        kv.__dict__["_seen"] = (kv.k, kv.v, kv.block_table, kv.k_scale, kv.v_scale,
+                                (kv.num_pages, kv.page_size, num_kv_heads, key_dim, value_dim, self.dtype), code)
+        return code
 
     # -- write ----------------------------------------------------------------------------------------------------
-    def _rows_write(self, what, q, k, v, bias, step, kv, rotary, num_heads, num_kv_heads, head_dim, value_dim, q_out,
-                    norm=(0, 0.0, None, None), q_temp=None) -> None:
-        """q, k, v: matrices ``[T, n]`` or slices ``[S, T, n]`` of one projection (q None: no queries; v None: the values are
-        the keys as projected); ``bias``: their three vectors."""
+    def _rows_write(self, what, rows, bias, step, kv, rotary, num_heads, num_kv_heads, head_dim, value_dim, q_out, norm=(0, 0.0, None, None),
+                    q_temp=None) -> None:
+        """``rows``: (element type code, slices, elements between slices, then pointer and row stride of q, of k and of v; a null q:
+        no queries, a null v: the values are the keys as projected); ``bias``: three pointers."""
         cache_code = self._check_slot(what, kv, num_kv_heads, head_dim, value_dim)
-        given = [x for x in (q, k, v) if x is not None]
-        if any(x.dtype != k.dtype or x.dim() != k.dim() or x.stride(-1) != 1 for x in given) or k.dtype not in (torch.float32, self.dtype):
-            raise KernelError(f"{what}: rows of float32 or {self.dtype} with unit column stride are expected")
-        if k.dim() == 3 and k.dtype != torch.float32:
-            raise KernelError(f"{what}: slices are float32")
         if rotary is not None and (rotary.rotary_dim > head_dim or rotary.rotary_dim % 2 or rotary.inv_freq.dtype != torch.float32
                                    or rotary.inv_freq.numel() * 2 < rotary.rotary_dim):
             raise KernelError(f"{what}: a rotary table of float32 frequencies for an even number of a head's elements is expected")
-        for vector in (*bias, norm[2], norm[3]):
-            if vector is not None and (vector.dtype != torch.float32 or vector.stride(-1) != 1):
-                raise KernelError(f"{what}: float32 vectors are expected")
+        for vector in norm[2:]:
+            if vector is not None and (vector.dtype != torch.float32 or vector.shape != (head_dim,) or vector.stride(0) != 1):
+                raise KernelError(f"{what}: float32 weights of {head_dim} elements are expected")
         if q_out is not None and (q_out.dtype != self.dtype or q_out.stride(-1) != 1):
             raise KernelError(f"{what}: q goes to rows of {self.dtype}")
-        stride = lambda x: x.stride(-2) if x is not None else 0  # noqa: E731
         coef, every = (float(q_temp[0]), float(q_temp[1])) if q_temp else (0.0, 0.0)
+        code, splits, split_stride, q, q_stride, k, k_stride, v, v_stride = rows
         with self._here():
             check(
-                function("distie_rows_write")(
-                    _ptr(q), stride(q), _ptr(k), stride(k), _ptr(v), stride(v), _CACHE_CODE[k.dtype], k.shape[0] if k.dim() == 3 else 1,
-                    k.stride(0) if k.dim() == 3 else 0, _ptr(bias[0]), _ptr(bias[1]), _ptr(bias[2]), int(norm[0]), float(norm[1]),
-                    _ptr(norm[2]), _ptr(norm[3]), _ptr(rotary.inv_freq) if rotary is not None else None,
-                    rotary.rotary_dim if rotary is not None else 0, int(rotary.interleaved) if rotary is not None else 0,
-                    float(rotary.factor) if rotary is not None else 1.0, coef, every, step.positions.data_ptr(), _ptr(step.slots),
-                    step.token_seq.data_ptr(), step.seq_seat.data_ptr(), kv.block_table.data_ptr(), kv.block_table.shape[-1],
-                    kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.k_scale), _ptr(kv.v_scale), step.num_tokens,
-                    num_heads if q is not None else 0, num_kv_heads, head_dim, value_dim, kv.page_size, kv.num_pages, 1, _ptr(q_out),
-                    stride(q_out), _CACHE_CODE[self.dtype], cache_code, self.error_flag.data_ptr(), self._stream(),
+                packed("distie_rows_write")(
+                    q, q_stride, k, k_stride, v, v_stride, code, splits, split_stride, *bias, norm[0], norm[1], _ptr(norm[2]), _ptr(norm[3]),
+                    rotary.inv_freq.data_ptr() if rotary is not None else 0, rotary.rotary_dim if rotary is not None else 0,
+                    int(rotary.interleaved) if rotary is not None else 0, rotary.factor if rotary is not None else 1.0, coef, every,
+                    step.positions.data_ptr(), _ptr(step.slots), step.token_seq.data_ptr(), step.seq_seat.data_ptr(),
+                    kv.block_table.data_ptr(), kv.block_table.shape[-1], kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.k_scale), _ptr(kv.v_scale),
+                    step.num_tokens, num_heads if q else 0, num_kv_heads, head_dim, value_dim, kv.page_size, kv.num_pages, 1,
+                    _ptr(q_out), q_out.stride(-2) if q_out is not None else 0, _CACHE_CODE[self.dtype], cache_code,
+                    self.error_flag.data_ptr(), self._stream(),
                 ),
                 "rows_write",
             )
@@ -103,14 +105,31 @@ class CachedRows:
 
     def _write_projection(self, what, qkv, bias, step, kv, rotary, num_heads, num_kv_heads, head_dim, value_dim, q_out, norm=(0, 0.0, None, None),
                           q_temp=None, values=True) -> None:
-        """The same from one projection ``[q | k | v]`` (``values`` False: ``[q | k]``, the values are the keys)."""
+        """From one projection ``[q | k | v]`` (``values`` False: ``[q | k]``, the values are the keys): a matrix ``[T, n]`` of
+        float32 or the set's dtype, or float32 slices ``[S, T, n]``."""
         k0, v0 = num_heads * head_dim, (num_heads + num_kv_heads) * head_dim
         end = v0 + num_kv_heads * value_dim if values else v0
-        if qkv.shape[-1] < end or (bias is not None and bias.shape[-1] < end):
-            raise KernelError(f"{what}: a projection of at least {end} columns is expected, not of {qkv.shape[-1]}")
-        cut = lambda x: (x[..., :k0], x[..., k0:v0], x[..., v0:end] if values else None)  # noqa: E731
-        self._rows_write(what, *cut(qkv), cut(bias) if bias is not None else (None, None, None), step, kv, rotary, num_heads, num_kv_heads,
+        sliced, dtype = qkv.dim() == 3, qkv.dtype
+        if qkv.shape[-1] < end or qkv.shape[-2] < step.num_tokens or qkv.stride(-1) != 1 or (dtype != torch.float32 and (sliced or dtype != self.dtype)):
+            raise KernelError(f"{what}: a projection [{step.num_tokens}, {end}] of {self.dtype} or float32, or float32 slices of one, with unit "
+                              f"column stride is expected, not {tuple(qkv.shape)} of {dtype}")
+        if bias is not None and (bias.dtype != torch.float32 or bias.shape[-1] < end or bias.stride(-1) != 1):
+            raise KernelError(f"{what}: a float32 bias of {end} elements is expected")
+        at, size, stride = qkv.data_ptr(), qkv.element_size(), qkv.stride(-2)
+        rows = (_CACHE_CODE[dtype], qkv.shape[0] if sliced else 1, qkv.stride(0) if sliced else 0, at, stride, at + k0 * size, stride,
+                at + v0 * size if values else 0, stride)
+        b = bias.data_ptr() if bias is not None else 0
+        self._rows_write(what, rows, (b, b + 4 * k0, b + 4 * v0) if b else (0, 0, 0), step, kv, rotary, num_heads, num_kv_heads,
                          head_dim, value_dim, q_out, norm, q_temp)
+
+    def _write_keys(self, what, k, v, step, kv) -> None:
+        """Finished keys and values ``[T, n]`` of one type, any row stride."""
+        num_kv_heads, key_dim, value_dim = kv.k.shape[1], kv.k.shape[-1], kv.v.shape[-1]
+        if k.dtype != v.dtype or k.dtype not in (torch.float32, self.dtype) or k.stride(-1) != 1 or v.stride(-1) != 1 \
+                or tuple(k.shape) != (step.num_tokens, num_kv_heads * key_dim) or tuple(v.shape) != (step.num_tokens, num_kv_heads * value_dim):
+            raise KernelError(f"{what}: keys and values of one float type, a row of every kv head's for each token, are expected")
+        rows = (_CACHE_CODE[k.dtype], 1, 0, 0, 0, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0))
+        self._rows_write(what, rows, (0, 0, 0), step, kv, None, 0, num_kv_heads, key_dim, value_dim, None)
 
     # -- read back ------------------------------------------------------------------------------------------------
     def kv_read(self, step, kv, window=None, chunk=None, keep_first=0) -> KvSlot:
@@ -118,35 +137,47 @@ class CachedRows:
         if kv.k_scale is None:
             raise KernelError("kv_read: the cache is in the engine's type already")
         self._check_slot("kv_read", kv, num_kv_heads, kv.k.shape[-1], kv.v.shape[-1])
-        portions = step.portions
-        if portions is None or len(portions) != step.num_seqs - step.num_decode_tokens:
-            raise KernelError("kv_read: the step's portions (cached and new tokens of every entry of several tokens) are expected")
-        keep_first = int(keep_first or 0) if window else 0
-        plan, total = [], 0
-        for row, (past, new) in enumerate(portions, start=step.num_decode_tokens):
-            columns, seen = -(-(past + new) // page), first_visible(past, window, chunk) // page
-            kept = min(seen, -(-keep_first // page))
-            first = 0 if kept else seen
-            plan.append((row, total, first, kept, seen if kept else kept, past + new))
-            total += columns - first
-        make = lambda like: torch.empty((total, num_kv_heads, page, like.shape[-1]), dtype=self.dtype, device=like.device)  # noqa: E731
-        out = KvSlot(make(kv.k), make(kv.v), torch.empty_like(kv.block_table), page, total)
-        for at in range(0, len(plan), _READ_ROWS):
-            part = plan[at : at + _READ_ROWS]
-            end = plan[at + _READ_ROWS][1] if at + _READ_ROWS < len(plan) else total
-            numbers = (ctypes.c_int * (6 * len(part)))(*[n for entry in part for n in entry])
-            with self._here():
+        plan, total = self._read_plan(step, page, int(window or 0), int(chunk or 0), int(keep_first or 0) if window else 0)
+        make = lambda dim: torch.empty((total, num_kv_heads, page, dim), dtype=self.dtype, device=kv.k.device)  # noqa: E731
+        out = KvSlot(make(kv.k.shape[-1]), make(kv.v.shape[-1]), torch.empty_like(kv.block_table), page, total)
+        with self._here():
+            for numbers, count, first, pages in plan:
                 check(
-                    function("distie_rows_read")(
-                        numbers, len(part), kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
+                    packed("distie_rows_read")(
+                        ctypes.addressof(numbers), count, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
                         kv.block_table.data_ptr(), kv.block_table.shape[-1], step.seq_seat.data_ptr(), num_kv_heads, kv.k.shape[-1],
-                        kv.v.shape[-1], page, kv.num_pages, out.k.data_ptr(), out.v.data_ptr(), out.block_table.data_ptr(), part[0][1],
-                        end - part[0][1], _CACHE_CODE[self.dtype], self.error_flag.data_ptr(), self._stream(),
+                        kv.v.shape[-1], page, kv.num_pages, out.k.data_ptr(), out.v.data_ptr(), out.block_table.data_ptr(), first, pages,
+                        _CACHE_CODE[self.dtype], self.error_flag.data_ptr(), self._stream(),
                     ),
                     "rows_read",
                 )
-            self._ran("rows_read")
+                self._ran("rows_read")
         return out
+
+    def _read_plan(self, step, page: int, window: int, chunk: int, keep_first: int):
+        """(launches, pages of the result): which pages of the step's portions are read and where they go, kept with the step for
+        all layers of a kind.  A launch: its rows of six numbers (see csrc/cached_rows.cu), their count, its first page, its pages."""
+        key = ("read_plan", page, window, chunk, keep_first)
+        made = step.derived.get(key)
+        if made is None:
+            portions = step.portions
+            if portions is None or len(portions) != step.num_seqs - step.num_decode_tokens:
+                raise KernelError("kv_read: the step's portions (cached and new tokens of every entry of several tokens) are expected")
+            rows, total = [], 0
+            for row, (past, new) in enumerate(portions, start=step.num_decode_tokens):
+                columns, seen = -(-(past + new) // page), first_visible(past, window, chunk) // page
+                kept = min(seen, -(-keep_first // page))
+                first = 0 if kept else seen
+                rows.append((row, total, first, kept, seen if kept else kept, past + new))
+                total += columns - first
+            plan = []
+            for at in range(0, len(rows), _READ_ROWS):
+                part = rows[at : at + _READ_ROWS]
+                end = rows[at + _READ_ROWS][1] if at + _READ_ROWS < len(rows) else total
+                numbers = (ctypes.c_int * (6 * len(part)))(*[n for entry in part for n in entry])
+                plan.append((numbers, len(part), part[0][1], end - part[0][1]))
+            made = step.derived[key] = (plan, total)
+        return made
 
     # -- attention ------------------------------------------------------------------------------------------------
     def _attention_rows(self, q, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first, softcap, sink,
@@ -179,10 +210,10 @@ class CachedRows:
             scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
         with self._here():
             check(
-                function("distie_attention_rows")(
+                packed("distie_attention_rows")(
                     q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
-                    step.token_seq.data_ptr(), step.seq_seat.data_ptr(), _ptr(tree.seqs) if tree is not None else None,
-                    _ptr(tree.bits) if tree is not None else None, tree.bits.shape[1] if tree is not None else 1, requests, tokens, most,
+                    step.token_seq.data_ptr(), step.seq_seat.data_ptr(), _ptr(tree.seqs) if tree is not None else 0,
+                    _ptr(tree.bits) if tree is not None else 0, tree.bits.shape[1] if tree is not None else 1, requests, tokens, most,
                     kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.k_scale), _ptr(kv.v_scale), kv.block_table.data_ptr(),
                     kv.block_table.shape[-1], num_heads, num_kv_heads, head_dim, value_dim, kv.page_size, kv.num_pages, window, chunk,
                     keep_first, float(scale), softcap, _ptr(sink), splits, _CACHE_CODE[self.dtype], cache_code,
@@ -207,7 +238,7 @@ class CachedRows:
             floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, head_dim, splits)
             scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
         with self._here():
-            code = function("distie_attention_decode_e4m3")(
+            code = packed("distie_attention_decode_e4m3")(
                 q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
                 step.token_seq.data_ptr(), step.seq_seat.data_ptr(), tokens, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(),
                 kv.v_scale.data_ptr(), kv.block_table.data_ptr(), kv.block_table.shape[-1], num_heads, num_kv_heads, head_dim,
@@ -233,7 +264,7 @@ class CachedRows:
             floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, head_dim, splits)
             scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
         with self._here():
-            code = function("distie_attention_tree_tcgen05")(
+            code = packed("distie_attention_tree_tcgen05")(
                 q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
                 step.seq_seat.data_ptr(), tree.seqs.data_ptr(), tree.bits.data_ptr(), tree.bits.shape[1], requests, tokens, most,
                 kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.k_scale), _ptr(kv.v_scale), kv.block_table.data_ptr(),

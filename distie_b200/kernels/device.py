@@ -809,7 +809,7 @@ class DeviceKernels(CachedRows, KernelSet):
 
     def kv_write(self, k, v, step, kv) -> None:
         if self._apart(step, kv):
-            self._rows_write("kv_write", None, k, v, (None, None, None), step, kv, None, 0, kv.k.shape[1], kv.k.shape[-1], kv.v.shape[-1], None)
+            self._write_keys("kv_write", k, v, step, kv)
             return
         if k.dtype != v.dtype or k.dtype not in _CODE or k.stride(1) != 1 or v.stride(1) != 1:
             raise KernelError("kv_write: keys and values of one float type with unit column stride are expected")

@@ -11,6 +11,7 @@ cannot be built or loaded the engine stops with the reason.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 P = c_void_p
@@ -196,6 +197,30 @@ def function(name: str):
         fn.restype = _RESULT.get(name, c_int)
         _functions[name] = fn
     return fn
+
+
+_CODES = {P: "P", I: "i", F: "f", L: "q"}
+_packed: dict[str, object] = {}
+
+
+def packed(name: str):
+    """The launcher called with one block of memory instead of its many arguments (csrc/packed.h): pointers are integers, 0 for none."""
+    call = _packed.get(name)
+    if call is None:
+        unit, argtypes = _SIGNATURES[name]
+        lib = load_unit(unit)
+        try:
+            fn = getattr(lib, name + "_packed")
+        except AttributeError as exc:
+            raise KernelError(f"kernel library of unit {unit!r} has no symbol {name}_packed") from exc
+        fn.argtypes, fn.restype = [ctypes.c_char_p], c_int
+        pack = struct.Struct("@" + "".join(_CODES[t] for t in argtypes)).pack
+
+        def call(*args):
+            return fn(pack(*args))
+
+        _packed[name] = call
+    return call
 
 
 _ARG_ERRORS = {-1: "invalid argument", -2: "size or dtype not supported by this kernel"}
