@@ -10,10 +10,12 @@
 //                    as 16-bit numbers, two keys to a column.  Warps whose rows are all empty take no part.
 //   O_g += P_g V_g   tcgen05.mma with P as the A operand straight from tensor memory
 //
-// Loaders (four warps, 32 keys each) copy K and V asynchronously, three tiles in flight, pages of any size: a lane looks up
-// the row of its key, and the warp takes the rows from its lanes, 16 bytes a lane and copy.  Rows of a 16-bit cache land
-// where the product reads them; those of an 8-bit one land packed where their warp's rows will be, are read into registers
-// and written back as float16, which holds every e4m3 number exactly, so that Q (times a power of two a row, float16), K, P and V are float16 there and bfloat16 here.  The
+// K and V: a warp each asks the copy engine for the rows of a block, page by page, as soon as a stage is free: of a 16-bit cache
+// with pages of 8, 16, ..., 128 rows they land swizzled, as the products read them; else they land packed (the rows of a page
+// and kv head are one run of memory), and four warps, 32 keys each, read them into registers and write them back
+// swizzled, of an 8-bit cache as float16, which holds every e4m3 number exactly.  (One set of warps for both took 6,600 cycles
+// a block, each step waiting for the one before.)  So Q (times a power of two a row, float16), K, P and V are float16 there
+// and bfloat16 of a 16-bit cache.  The
 // scales of the rows go beside the tiles: s^k multiplies the finished score; the weights of the second product are p s^v over
 // a running maximum m' of their own, p (s^v 2^(m - m')), so that float16 holds the largest of a row near 1 whatever
 // the scales.
@@ -26,7 +28,7 @@
 // Running maxima are raised only when exceeded by more than 8 (base 2), so O is read, scaled and written back rarely.
 // With several shares of the keys, the parts go to scratch in float32 and attention_rows.cu joins them.
 //
-//   warps 0..7    softmax, end        warp 8   tensor memory, MMA issue        warps 9..12   loaders
+//   warps 0..7    softmax, end        warp 8   tensor memory, MMA issue        warps 9, 10   copies        warps 11..14   unpacking
 //
 // Every wait on an mbarrier is bounded; when one runs out the CTA sets the error word to 6 and every role stops at its
 // next wait.
@@ -43,9 +45,10 @@ constexpr int kTreeRows = 128;
 constexpr int kTreeKeys = 128;
 constexpr int kTreeGroupKeys = 64;
 constexpr int kTreeMmaWarp = 8;
-constexpr int kTreeLoadWarp = 9;
-constexpr int kTreeLoaders = 4;    // warps
-constexpr int kTreeThreads = 32 * 13;
+constexpr int kTreeCopyWarp = 9;   // of K, and behind it of V
+constexpr int kTreeLoadWarp = 11;  // the first of those that unpack
+constexpr int kTreeLoaders = 4;
+constexpr int kTreeThreads = 32 * 15;
 constexpr int kTreeKStages = 2, kTreeVStages = 3, kTreeScaleSlots = 4;
 constexpr int kTreeHalf = kTreeRows * 128;  // bytes of one [128 rows x 64 elements] swizzled half tile
 constexpr int kTreeMostNodes = 256;
@@ -84,6 +87,7 @@ struct TreeShared {
   uint64_t q_full;
   uint64_t k_full[kTreeKStages], k_empty[kTreeKStages];
   uint64_t v_full[kTreeVStages], v_empty[kTreeVStages];
+  uint64_t k_landed[kTreeKStages], v_landed[kTreeVStages];  // the copies of a tile
   uint64_t scale_full[kTreeScaleSlots];
   uint64_t s_full[2];
   uint64_t p_full[2][2];  // [group][S buffer]
@@ -101,6 +105,15 @@ __device__ __forceinline__ uint32_t tree_offset(int row, int piece) {  // of 8 e
 __device__ __forceinline__ void store_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // whether that phase is over, without waiting
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ float tree_log2(float x) {
   float y;
   asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -115,8 +128,7 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t x, bool& bad) {
   return x & keep;
 }
 
-// Whether the row sees a key.  (Functions of their own, called where a block needs masks: what they look at takes no registers
-// elsewhere.)
+// Whether the row sees a key.
 template <int D>
 __device__ __forceinline__ bool tree_seen(const TreeShared<D>& sm, int r, int key, int key_end, const int* bits, int words, int keep_first) {
   const int token = sm.row_token[r];
@@ -131,14 +143,22 @@ __device__ __forceinline__ bool tree_seen(const TreeShared<D>& sm, int r, int ke
 }
 // The keys of [key0, key0 + 64) that the row sees, a bit each.
 template <int D>
-__device__ __noinline__ uint64_t tree_seen64(const TreeShared<D>& sm, int r, int key0, int key_end, const int* bits, int words, int keep_first) {
+__device__ __forceinline__ uint64_t tree_seen64(const TreeShared<D>& sm, int r, int key0, int key_end, const int* bits, int words, int keep_first) {
   uint64_t mask = 0;
   const int token = sm.row_token[r], past = sm.span.past;
   if (token < 0) return mask;
-  if (sm.row_first[r] == 0) {  // no window has moved: cached keys, then the row's mask
-    const int cached = min(max(past - key0, 0), 64);
-    if (cached > 0) mask = cached == 64 ? ~0ull : (1ull << cached) - 1;
-    const int there = min(64 - cached, key_end - max(key0, past));
+  const int first = sm.row_first[r];
+  if (first <= past) {  // the window holds all new tokens: two ranges of cached keys, then the row's mask
+    // Bits low .. high - 1 of the 64.
+    auto range = [](int low, int high) {
+      low = min(max(low, 0), 64);
+      high = min(max(high, 0), 64);
+      if (low >= high) return 0ull;
+      return (high == 64 ? ~0ull : (1ull << high) - 1) & ~((1ull << low) - 1);
+    };
+    const int end = min(past, key_end);
+    mask = range(first - key0, end - key0) | range(-key0, min(min(keep_first, first), end) - key0);
+    const int cached = min(max(past - key0, 0), 64), there = min(64 - cached, key_end - max(key0, past));
     if (there > 0) {
       const int skip = max(key0 - past, 0), word = skip >> 5, shift = skip & 31;  // new tokens before key0
       auto load = [&](int w) { return w < words ? (uint32_t)__ldg(bits + (size_t)token * words + w) : 0u; };
@@ -155,7 +175,7 @@ __device__ __noinline__ uint64_t tree_seen64(const TreeShared<D>& sm, int r, int
 }
 // What the values that are not finite, in blocks block0 .. block1 - 1 that need masks, add to element e of the row's sum.
 template <int D>
-__device__ __noinline__ float tree_not_finite(const TreeShared<D>& sm, int r, int e, int block0, int block1, const __nv_bfloat16* values,
+__device__ __forceinline__ float tree_not_finite(const TreeShared<D>& sm, int r, int e, int block0, int block1, const __nv_bfloat16* values,
                                               const CachePages& cache, const int* table, int kv_head, const int* bits, int words, int keep_first) {
   float sum = 0.f;
   for (int j = block0; j < block1; ++j) {
@@ -173,7 +193,8 @@ __device__ __noinline__ float tree_not_finite(const TreeShared<D>& sm, int r, in
 
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(kTreeThreads, 1)
-attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride, QueryRows rows,
+attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int direct,
+                              const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride, QueryRows rows,
                               CachePages cache, Partials parts, int* __restrict__ error) {
   extern __shared__ unsigned char raw_shared[];
   auto& sm = *reinterpret_cast<TreeShared<D>*>((reinterpret_cast<uintptr_t>(raw_shared) + 1023) & ~uintptr_t(1023));
@@ -182,7 +203,7 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
   volatile uint32_t* failed = &sm.failed;
 
   const int split = blockIdx.z;
-  const int kv_head = blockIdx.x % cache.num_kv_heads, tile = blockIdx.x / cache.num_kv_heads;
+  const int tiles = gridDim.x / cache.num_kv_heads, kv_head = blockIdx.x / tiles, tile = blockIdx.x % tiles;
   const Request request = request_of(rows, blockIdx.y);
   const int row0 = tile * kTreeRows, count = min(kTreeRows, request.nodes * rows.group - row0);
   if (count <= 0) return;
@@ -237,10 +258,12 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
     for (int s = 0; s < kTreeKStages; ++s) {
       mbar_init(&sm.k_full[s], kTreeLoaders);
       mbar_init(&sm.k_empty[s], 1);
+      mbar_init(&sm.k_landed[s], 1);
     }
     for (int s = 0; s < kTreeVStages; ++s) {
       mbar_init(&sm.v_full[s], kTreeLoaders);
       mbar_init(&sm.v_empty[s], 1);
+      mbar_init(&sm.v_landed[s], 1);
     }
     for (int s = 0; s < kTreeScaleSlots; ++s) mbar_init(&sm.scale_full[s], kTreeLoaders);
     for (int b = 0; b < 2; ++b) {
@@ -273,131 +296,179 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
   // The page ids of the share's keys from its window's first block on.
   const int column0 = cache.column_of(span.key0(max(block0, span.kept_blocks)));
   const int columns = block1 > span.kept_blocks ? min(kTreePages, cache.column_of(min(span.keys - 1, span.key0(block1 - 1) + kTreeKeys - 1)) - column0 + 1) : 0;
-  if (warp >= kTreeLoadWarp)  // (the loaders alone look at them)
-    for (int i = threadIdx.x - kTreeLoadWarp * 32; i < columns; i += kTreeLoaders * 32)
+  if (warp >= kTreeCopyWarp)  // (the warps below alone look at them)
+    for (int i = threadIdx.x - kTreeCopyWarp * 32; i < columns; i += (kTreeLoaders + 2) * 32)
       sm.pages[i] = column0 + i < cache.table_width ? table[column0 + i] : -1;
   const uint32_t tmem = sm.tmem_base;
   grid_dependency_wait();  // q and the newest rows come from the kernels before this one
 
-  if (warp >= kTreeLoadWarp) {
-    // ---- loaders: 16 bytes of a row per lane and copy ------------------------------------------------------------------
-    asm volatile("bar.sync 1, %0;" ::"n"(kTreeLoaders * 32) : "memory");  // the page ids are there
-    constexpr int PPR = E4M3 ? D / 16 : D / 8;  // 16-byte pieces of a row
-    constexpr int RPI = 32 / PPR;               // rows that one copy of the warp covers
-    constexpr int PIECES = 32 / RPI;            // copies of a tile, per lane
-    constexpr int LAG = 3;                      // tiles in flight
-    const int row0_mine = (warp - kTreeLoadWarp) * 32;  // the warp's keys of a block
-    const int sub_row = lane / PPR, piece = lane % PPR;
+  if (warp >= kTreeCopyWarp) {
+    constexpr int BYTES = E4M3 ? D : 2 * D;  // of a row in the cache
+    // Packed rows: those of 32 keys land in the first 32 lines of 128 bytes that these keys will take, rows of 256 bytes in two
+    // halves of 16 keys.
+    constexpr int FIT = BYTES > 128 ? 16 : 32;
+    asm volatile("bar.sync 1, %0;" ::"n"((kTreeLoaders + 2) * 32) : "memory");  // the page ids are there
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_unless(bar, parity, failed)) != 0; };
-    auto find = [&](int j) {  // the row of this lane's key of block j among the slot's rows, -1: none
-      const int key = span.key0(j) + row0_mine + lane;
-      int at = -1;
-      if (key < span.key_end(j) && (key >= span.oldest || key < span.kept)) {
-        const int column = cache.column_of(key), index = column - column0;
-        const int page = index >= 0 && index < columns ? sm.pages[index] : column < cache.table_width ? __ldg(table + column) : -1;
-        if (page >= 0 && page < cache.num_pages) at = (page * cache.num_kv_heads + kv_head) * cache.page_size + cache.within(key);
-        else if (error) atomicExch(error, 8);
-      }
-      __syncwarp();
-      return at;
+    auto page_at = [&](int column) {
+      const int index = column - column0;
+      return index >= 0 && index < columns ? sm.pages[index] : column < cache.table_width ? __ldg(table + column) : -1;
     };
-    auto copy = [&](unsigned char* stage, const void* rows_at, int at) {
-      const uint32_t base = smem_u32(stage) + (E4M3 ? row0_mine * 128 + lane * 16 : 0);
+    auto wanted = [&](int key, int key_end) { return key < key_end && (key >= span.oldest || key < span.kept); };
+    bool ok = true;
+    if (warp < kTreeLoadWarp) {
+      // ---- copies of K or V: a lane a page, in rounds of 32 pages -------------------------------------------------------------
+      const bool is_k = warp == kTreeCopyWarp;
+      const int stages = is_k ? kTreeKStages : kTreeVStages;
+      uint64_t* empty = is_k ? sm.k_empty : sm.v_empty;
+      uint64_t* landed = is_k ? sm.k_landed : sm.v_landed;
+      const CUtensorMap* map = is_k ? &map_k : &map_v;
+      const unsigned char* rows_at = reinterpret_cast<const unsigned char*>(is_k ? cache.k : cache.v);
+      int requested = 0;
+      for (; requested < blocks; ++requested) {
+        const int j = block0 + requested, stage = requested % stages;
+        const int key0 = span.key0(j), end = min(key0 + kTreeKeys, span.key_end(j));
+        const int first_column = cache.column_of(key0), last_column = end > key0 ? cache.column_of(end - 1) : first_column - 1;
+        unsigned char* tile_at = (is_k ? sm.k[0] : sm.v[0]) + (size_t)stage * kTreeKeys * D * 2;
+        bool waited = false;
+        for (int round = first_column; !waited || round <= last_column; round += 32) {
+          // The lane's run of a round: keys from .. to - 1 of its page, wanted ones and what lies between them.
+          const int column = round + lane;
+          int from = 0, to = 0, page = 0;
+          if (column <= last_column) {
+            const int page0 = column * cache.page_size;
+            from = max(key0, page0);
+            to = min(end, page0 + cache.page_size);
+            if (from < span.oldest && from >= span.kept) from = span.oldest;  // between the kept keys and the window
+            if (from < span.kept && to > span.kept && to <= span.oldest) to = span.kept;
+            to = max(to, from);
+            if (to > from) page = page_at(column);
+            if (page < 0 || page >= cache.num_pages) {
+              to = from;
+              if (error) atomicExch(error, 8);
+            }
+          }
+          const int bytes = __reduce_add_sync(0xffffffffu, direct ? (to > from ? cache.page_size : 0) : to - from) * BYTES;
+          if (!waited && !wait(&empty[stage], ((requested / stages) & 1) ^ 1)) { ok = false; break; }
+          waited = true;
+          if (lane == 0) {
+            if (round + 32 > last_column) mbar_expect_tx(&landed[stage], bytes);
+            else asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&landed[stage])), "r"(bytes) : "memory");
+          }
+          __syncwarp();
+          if (to > from) {
+            const long long row = ((long long)page * cache.num_kv_heads + kv_head) * cache.page_size;
+            if (!E4M3 && direct) {  // the whole page
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int row = i * RPI + sub_row, from_row = __shfl_sync(0xffffffffu, at, row);
-        const unsigned char* from = reinterpret_cast<const unsigned char*>(rows_at) + (size_t)max(from_row, 0) * (PPR * 16) + piece * 16;
-        const uint32_t to = E4M3 ? base + i * 512 : base + tree_offset(row0_mine + row, piece);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(from_row >= 0 ? 16 : 0) : "memory");
+              for (int h = 0; h < D / 64; ++h)
+                tma_load_2d(tile_at + h * kTreeHalf + (column * cache.page_size - key0) * 128, map, &landed[stage], h * 64, (int)row);
+            } else {
+              for (int at = from; at < to;) {
+                const int local = at - key0, stop = min(to, key0 + (local / FIT + 1) * FIT);
+                const unsigned char* source = rows_at + (size_t)(row + cache.within(at)) * BYTES;
+                const uint32_t target = smem_u32(tile_at) + (local % 32 / FIT) * kTreeHalf + local / 32 * 4096 + local % FIT * BYTES;
+                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(target), "l"(source),
+                             "r"((stop - at) * BYTES), "r"(smem_u32(&landed[stage])) : "memory");
+                at = stop;
+              }
+            }
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
       }
-    };
-    // A tile whose copies have landed (this warp's of them): made what the product reads.
-    auto finish = [&](unsigned char* stage, bool check) {
-      if (E4M3) {
+      // Copies still on their way must land before the CTA may leave.
+      for (int i = max(0, requested - stages); !ok && i < requested; ++i) mbar_wait(&landed[i % stages], (i / stages) & 1);
+    } else {
+      // ---- unpacking: 32 keys a warp --------------------------------------------------------------------------------------
+      constexpr int PPR = BYTES / 16;   // 16-byte pieces of a row
+      constexpr int RPI = 32 / PPR;     // rows that the warp reads at a time
+      constexpr int PIECES = 32 / RPI;  // of a tile, per lane
+      const int row0_mine = (warp - kTreeLoadWarp) * 32, sub_row = lane / PPR, piece = lane % PPR;
+      // A tile whose rows have landed (`there`: which of the warp's 32, a bit each): made what the product reads.  `check`: values
+      // that are not finite become zeros, and are remembered.
+      auto finish = [&](unsigned char* stage, uint32_t there, bool check) {
+        if (!E4M3 && direct && !check) return;
         uint4 raw[PIECES];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) raw[i] = *reinterpret_cast<const uint4*>(stage + row0_mine * 128 + i * 512 + lane * 16);
-        __syncwarp();
-        const uint32_t base = smem_u32(stage);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          const int row = row0_mine + i * RPI + sub_row;
-          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-          uint32_t h[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            h[2 * e] = e4m3x2_to_half2((uint16_t)(w[e] & 0xffffu));
-            h[2 * e + 1] = e4m3x2_to_half2((uint16_t)(w[e] >> 16));
-          }
-          store_shared16(base + tree_offset(row, 2 * piece), h[0], h[1], h[2], h[3]);
-          store_shared16(base + tree_offset(row, 2 * piece + 1), h[4], h[5], h[6], h[7]);
+          const int row = i * RPI + sub_row;
+          raw[i] = *reinterpret_cast<const uint4*>(stage + (!E4M3 && direct ? tree_offset(row0_mine + row, piece)
+                                                                           : row / FIT * kTreeHalf + row0_mine * 128 + row % FIT * BYTES + piece * 16));
         }
-      } else if (check) {
+        __syncwarp();
+        const uint32_t base = smem_u32(stage);
         bool bad = false;
-        for (int i = 0; i < PIECES; ++i) {  // (the lane's own copies)
-          uint4* at = reinterpret_cast<uint4*>(stage + tree_offset(row0_mine + i * RPI + sub_row, piece));
-          uint4 x = *at;
-          bool here = false;
-          x.x = finite_pair(x.x, here);
-          x.y = finite_pair(x.y, here);
-          x.z = finite_pair(x.z, here);
-          x.w = finite_pair(x.w, here);
-          if (here) *at = x;
-          bad |= here;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int row = i * RPI + sub_row;
+          uint4 x = (there >> row) & 1 ? raw[i] : make_uint4(0u, 0u, 0u, 0u);
+          if (E4M3) {
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t h[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              h[2 * e] = e4m3x2_to_half2((uint16_t)(w[e] & 0xffffu));
+              h[2 * e + 1] = e4m3x2_to_half2((uint16_t)(w[e] >> 16));
+            }
+            store_shared16(base + tree_offset(row0_mine + row, 2 * piece), h[0], h[1], h[2], h[3]);
+            store_shared16(base + tree_offset(row0_mine + row, 2 * piece + 1), h[4], h[5], h[6], h[7]);
+          } else {
+            if (check) {
+              x.x = finite_pair(x.x, bad);
+              x.y = finite_pair(x.y, bad);
+              x.z = finite_pair(x.z, bad);
+              x.w = finite_pair(x.w, bad);
+            }
+            store_shared16(base + tree_offset(row0_mine + row, piece), x.x, x.y, x.z, x.w);
+          }
         }
         if (bad) atomicExch(&sm.bad, 1u);
+      };
+      auto ready = [&](uint64_t* bar) {  // this warp's stores are in shared memory, for the tensor cores and for other warps
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+      };
+      // The row of this lane's key of block j among the slot's rows, -1: none.
+      auto find = [&](int j) -> long long {
+        if (j >= block1) return -1;
+        const int key = span.key0(j) + row0_mine + lane;
+        if (!wanted(key, span.key_end(j))) return -1;
+        const int page = page_at(cache.column_of(key));
+        if (page < 0 || page >= cache.num_pages) return -1;
+        return ((long long)page * cache.num_kv_heads + kv_head) * cache.page_size + cache.within(key);
+      };
+      // Scales, a lane per key, one block ahead in registers (of no key: the slot's first row's, never read behind the mask).
+      long long at = find(block0);
+      float ks = 0.f, vs = 0.f;
+      if (E4M3) {
+        ks = __ldcg(cache.k_scale + max(at, 0ll));
+        vs = __ldcg(cache.v_scale + max(at, 0ll));
       }
-    };
-    auto ready = [&](uint64_t* bar) {  // this warp's stores are in shared memory, for the tensor cores and for other warps
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-    };
-    // Tile 2 n is K of the share's block n, tile 2 n + 1 its V: requested when its stage is free, finished LAG tiles later.
-    bool ok = true;
-    float ks_ahead = 0.f, vs_ahead = 0.f;
-    int at = -1;
-    for (int i = 0; i < 2 * blocks + LAG && ok; ++i) {
-      const int n = i >> 1;
-      if (i < 2 * blocks) {
-        const bool is_k = !(i & 1);
-        if (is_k) at = find(block0 + n);
-        uint64_t* empty = is_k ? &sm.k_empty[n % kTreeKStages] : &sm.v_empty[n % kTreeVStages];
-        const int use = is_k ? n / kTreeKStages : n / kTreeVStages;
-        if (!wait(empty, (use & 1) ^ 1)) { ok = false; break; }
-        copy(is_k ? sm.k[n % kTreeKStages] : sm.v[n % kTreeVStages], is_k ? cache.k : cache.v, at);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (E4M3 && !(i & 1)) {
-        // Scales, a lane per key, one block ahead in registers.  The slot's last ones have been read: the S of two blocks
-        // ago, whose stage K has just taken, was issued behind the P before it.
-        if (n >= 1 && n <= blocks) {
-          const int slot = (n - 1) % kTreeScaleSlots;
-          sm.k_scale[slot][row0_mine + lane] = ks_ahead;
-          sm.v_scale[slot][row0_mine + lane] = vs_ahead;
-          sm.v_log[slot][row0_mine + lane] = tree_log2(vs_ahead);
+      for (int n = 0; n < blocks; ++n) {
+        const int k_stage = n % kTreeKStages, v_stage = n % kTreeVStages;
+        const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+        if (!wait(&sm.k_landed[k_stage], (n / kTreeKStages) & 1)) { ok = false; break; }
+        at = find(block0 + n + 1);
+        if (E4M3) {
+          // The slot's last scales have been read: the S of two blocks ago, whose stage K has taken, was issued behind the P of
+          // two blocks before that.
+          const int slot = n % kTreeScaleSlots, key = row0_mine + lane;
+          sm.k_scale[slot][key] = ks;
+          sm.v_scale[slot][key] = vs;
+          sm.v_log[slot][key] = tree_log2(vs);
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.scale_full[slot]);
+          ks = __ldcg(cache.k_scale + max(at, 0ll));
+          vs = __ldcg(cache.v_scale + max(at, 0ll));
         }
-        if (n < blocks) {
-          ks_ahead = __ldcg(cache.k_scale + max(at, 0));  // (of no key: never read behind the mask)
-          vs_ahead = __ldcg(cache.v_scale + max(at, 0));
-        }
-      }
-      if (i >= LAG) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
-        const int done = i - LAG, m = done >> 1;
-        if (!(done & 1)) {
-          finish(sm.k[m % kTreeKStages], false);
-          ready(&sm.k_full[m % kTreeKStages]);
-        } else {
-          finish(sm.v[m % kTreeVStages], !span.whole(block0 + m));
-          ready(&sm.v_full[m % kTreeVStages]);
-        }
+        finish(sm.k[k_stage], there, false);
+        ready(&sm.k_full[k_stage]);
+        if (!wait(&sm.v_landed[v_stage], (n / kTreeVStages) & 1)) { ok = false; break; }
+        finish(sm.v[v_stage], there, !span.whole(block0 + n));
+        ready(&sm.v_full[v_stage]);
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (!ok) atomicExch(&sm.failed, 1u);
   } else if (warp == kTreeMmaWarp) {
     // ---- MMA issuer ----------------------------------------------------------------------------------------------------
@@ -507,47 +578,53 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         if (E4M3 && !wait_all(&sm.scale_full[slot], (n / kTreeScaleSlots) & 1)) { ok = false; break; }
         if (!wait_all(&sm.s_full[s], (n >> 1) & 1)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint32_t sv[kTreeGroupKeys];
-        tmem_load_64(s_addr, sv);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         const float* k_scale = &sm.k_scale[slot][g * kTreeGroupKeys];
         const float* v_log = &sm.v_log[slot][g * kTreeGroupKeys];
         const float* v_scale = &sm.v_scale[slot][g * kTreeGroupKeys];
-        // Scores in base-2 units, on pairs of values.
         const uint64_t times2 = pair_of(times, times);
+        // Half of the group's scores in base-2 units.  They are fetched twice, for the maximum and for the weights: 64 at once do not
+        // fit a thread's registers beside the rest, and what spills goes to L2 (shared memory leaves L1 next to nothing).
+        auto scores = [&](int half, uint32_t (&sv)[32]) {
+          tmem_load_32(s_addr + half * 32, sv);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < kTreeGroupKeys; i += 2) {
-          uint64_t x = pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-          if (E4M3) x = mul_pairs(x, *reinterpret_cast<const uint64_t*>(k_scale + i));
-          x = mul_pairs(x, times2);
-          float x0, x1;
-          halves_of(x, x0, x1);
-          sv[i] = __float_as_uint(x0);
-          sv[i + 1] = __float_as_uint(x1);
-        }
-        if (rows.extras.cap > 0.f) {  // cap * tanh, by its exponential: off by 2^-22 of the cap
-#pragma unroll
-          for (int i = 0; i < kTreeGroupKeys; ++i)
-            sv[i] = __float_as_uint(cap * (1.f - __fdividef(2.f, exp2_approx(__uint_as_float(sv[i]) * 2.8853900817779268f) + 1.f)));
-        }
-        if (!whole) {
-          const uint32_t low = (uint32_t)mask, high = (uint32_t)(mask >> 32);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (!((low >> i) & 1)) sv[i] = 0xff800000u;  // -inf
-            if (!((high >> i) & 1)) sv[32 + i] = 0xff800000u;
+          for (int i = 0; i < 32; i += 2) {
+            uint64_t x = pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+            if (E4M3) x = mul_pairs(x, *reinterpret_cast<const uint64_t*>(k_scale + half * 32 + i));
+            x = mul_pairs(x, times2);
+            float x0, x1;
+            halves_of(x, x0, x1);
+            sv[i] = __float_as_uint(x0);
+            sv[i + 1] = __float_as_uint(x1);
           }
-        }
+          if (rows.extras.cap > 0.f) {  // cap * tanh, by its exponential: off by 2^-22 of the cap
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              sv[i] = __float_as_uint(cap * (1.f - __fdividef(2.f, exp2_approx(__uint_as_float(sv[i]) * 2.8853900817779268f) + 1.f)));
+          }
+          if (!whole) {
+            const uint32_t bits32 = half ? (uint32_t)(mask >> 32) : (uint32_t)mask;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((bits32 >> i) & 1)) sv[i] = 0xff800000u;  // -inf
+          }
+        };
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ox4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < kTreeGroupKeys; i += 2) {
-          float& m = mx4[(i >> 1) & 3];
-          m = max3(m, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-          if (E4M3) {
-            float z0, z1;
-            halves_of(add_pairs(pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), *reinterpret_cast<const uint64_t*>(v_log + i)), z0, z1);
-            float& o = ox4[(i >> 1) & 3];
-            o = max3(o, z0, z1);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t sv[32];
+          scores(half, sv);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float& m = mx4[(i >> 1) & 3];
+            m = max3(m, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+            if (E4M3) {
+              float z0, z1;
+              halves_of(add_pairs(pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), *reinterpret_cast<const uint64_t*>(v_log + half * 32 + i)),
+                        z0, z1);
+              float& o = ox4[(i >> 1) & 3];
+              o = max3(o, z0, z1);
+            }
           }
         }
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), ox = fmaxf(fmaxf(ox4[0], ox4[1]), fmaxf(ox4[2], ox4[3]));
@@ -591,21 +668,21 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
         uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          uint32_t packed[16];
+          uint32_t sv[32], packed[16];
+          scores(half, sv);
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const int at = half * 32 + i;
             float x0, x1;
-            halves_of(add_pairs(pair_of(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), shift2), x0, x1);
+            halves_of(add_pairs(pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), shift2), x0, x1);
             const uint64_t p = pair_of(exp2_approx(x0), exp2_approx(x1));
             uint64_t& sum = sum4[(i >> 1) & 3];
             float w0, w1;
             if (E4M3) {
               sum = add_pairs(sum, p);
-              halves_of(mul_pairs(p, mul_pairs(*reinterpret_cast<const uint64_t*>(v_scale + at), units2)), w0, w1);
+              halves_of(mul_pairs(p, mul_pairs(*reinterpret_cast<const uint64_t*>(v_scale + half * 32 + i), units2)), w0, w1);
               if (!whole) {  // (0 times the scale of a row that is not finite, or of nobody's, is not 0)
-                w0 = sv[at] == 0xff800000u ? 0.f : w0;
-                w1 = sv[at + 1] == 0xff800000u ? 0.f : w1;
+                w0 = sv[i] == 0xff800000u ? 0.f : w0;
+                w1 = sv[i + 1] == 0xff800000u ? 0.f : w1;
               }
               const __half2 pair = __floats2half2_rn(w0, w1);
               packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
@@ -663,12 +740,6 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
           float y[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) y[i] = __uint_as_float(a[i]) * f0 + __uint_as_float(b[i]) * f1;
-          if (!E4M3 && sm.bad && live) {  // values that are not finite, for the rows that see them
-            const __nv_bfloat16* values = reinterpret_cast<const __nv_bfloat16*>(cache.v);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              y[i] += tree_not_finite(sm, r, g * SIDE + c0 + i, block0, block1, values, cache, table, kv_head, rows.bits, rows.words, rows.keep_first);
-          }
           if (live && alone) {
             __nv_bfloat16* to = out + (size_t)token * out_stride + (size_t)head * D + g * SIDE + c0;
 #pragma unroll
@@ -680,6 +751,20 @@ attention_tree_tcgen05_kernel(const __nv_bfloat16* __restrict__ q, int q_stride,
             float* to = parts.o + part_row * D + g * SIDE + c0;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) store4(to + i, make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
+          }
+        }
+        if (!E4M3 && sm.bad && live) {  // values that are not finite join the sums of the rows that see them
+          const __nv_bfloat16* values = reinterpret_cast<const __nv_bfloat16*>(cache.v);
+#pragma unroll 1
+          for (int e = g * SIDE; e < (g + 1) * SIDE; ++e) {
+            const float more = tree_not_finite(sm, r, e, block0, block1, values, cache, table, kv_head, rows.bits, rows.words, rows.keep_first);
+            if (more == 0.f) continue;
+            if (alone) {
+              __nv_bfloat16* to = out + (size_t)token * out_stride + (size_t)head * D + e;
+              *to = __float2bfloat16_rn(__bfloat162float(*to) + more);
+            } else {
+              parts.o[part_row * D + e] += more;
+            }
           }
         }
         if (live && !alone && g == 0) {
@@ -702,10 +787,20 @@ template <int D, bool E4M3>
 static int launch_tree(const dim3& grid, const __nv_bfloat16* q, int q_stride, __nv_bfloat16* out, int out_stride, const QueryRows& rows,
                        const CachePages& cache, const Partials& parts, int* error, cudaStream_t stream) {
   const size_t shared = sizeof(TreeShared<D>) + 1024;
+  // Pages that the copy engine puts down swizzled: a box of [page_size x 64].
+  const int direct = !E4M3 && cache.page_size >= 8 && cache.page_size <= 128 && cache.page_shift >= 0;
+  CUtensorMap map_k = {}, map_v = {};
+  if (direct) {
+    const int all_rows = (int)((long long)cache.num_pages * cache.num_kv_heads * cache.page_size);
+    int status;
+    if ((status = make_map(&map_k, cache.k, all_rows, D, D, cache.page_size)) != 0) return status;
+    if ((status = make_map(&map_v, cache.v, all_rows, D, D, cache.page_size)) != 0) return status;
+  }
   auto kernel = attention_tree_tcgen05_kernel<D, E4M3>;
   cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
   if (err != cudaSuccess) return (int)err;
-  return (int)launch_dependent(kernel, grid, dim3(kTreeThreads), shared, stream, q, q_stride, out, out_stride, rows, cache, parts, error);
+  return (int)launch_dependent(kernel, grid, dim3(kTreeThreads), shared, stream, map_k, map_v, direct, q, q_stride, out, out_stride, rows, cache, parts,
+                               error);
 }
 
 }  // namespace distie
