@@ -25,7 +25,8 @@
 // finite are stored as zeros, and the rows that see them get them back at the end, element by element (8-bit rows carry
 // NaN in their scales, which masks reach).  Rows of keys that belong to nobody are zeros.
 //
-// Running maxima are raised only when exceeded by more than 8 (base 2), so O is read, scaled and written back rarely.
+// Running maxima are not searched for in every block, only in a row's first and where its weights outgrow the one in use;
+// then O is read, scaled and written back.
 // With several shares of the keys, the parts go to scratch in float32 and attention_rows.cu joins them.
 //
 //   warps 0..7    softmax, end        warp 8   tensor memory, MMA issue        warps 9, 10   copies        warps 11..14   unpacking
@@ -53,7 +54,7 @@ constexpr int kTreeKStages = 2, kTreeVStages = 3, kTreeScaleSlots = 4;
 constexpr int kTreeHalf = kTreeRows * 128;  // bytes of one [128 rows x 64 elements] swizzled half tile
 constexpr int kTreeMostNodes = 256;
 constexpr int kTreePages = 2048;   // page ids of a CTA's share that are kept in shared memory
-constexpr float kTreeRaise = 8.f;
+constexpr float kTreeMostSum = 1073741824.f, kTreeMostWeight = 16384.f;  // of a row's weights of 64 keys
 
 // The blocks of 128 keys that a tile of rows walks: those of the kept first keys, then those from the window's start on.
 struct TreeSpan {
@@ -174,9 +175,9 @@ __device__ __forceinline__ uint64_t tree_seen64(const TreeShared<D>& sm, int r, 
   return mask;
 }
 // What the values that are not finite, in blocks block0 .. block1 - 1 that need masks, add to element e of the row's sum.
-template <int D>
-__device__ __forceinline__ float tree_not_finite(const TreeShared<D>& sm, int r, int e, int block0, int block1, const __nv_bfloat16* values,
-                                              const CachePages& cache, const int* table, int kv_head, const int* bits, int words, int keep_first) {
+template <int D, bool E4M3>
+__device__ __forceinline__ float tree_not_finite(const TreeShared<D>& sm, int r, int e, int block0, int block1, const CachePages& cache,
+                                                 const int* table, int kv_head, const int* bits, int words, int keep_first) {
   float sum = 0.f;
   for (int j = block0; j < block1; ++j) {
     if (sm.span.whole(j)) continue;
@@ -184,11 +185,20 @@ __device__ __forceinline__ float tree_not_finite(const TreeShared<D>& sm, int r,
       if (!tree_seen(sm, r, key, sm.span.key_end(j), bits, words, keep_first)) continue;
       const long long at = cache.row_of(table, key, kv_head);
       if (at < 0) continue;
-      const float v = __bfloat162float(values[(size_t)at * D + e]);
+      float v;
+      if (E4M3) v = e4m3_to_float(reinterpret_cast<const uint8_t*>(cache.v)[(size_t)at * D + e]) * cache.v_scale[at];
+      else v = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(cache.v)[(size_t)at * D + e]);
       if (!(fabsf(v) <= 3.402823466e38f)) sum += v;
     }
   }
   return sum;
+}
+
+// Four floats of shared memory.  (Volatile: the compiler otherwise keeps a block's scales in registers from one look to the next.)
+__device__ __forceinline__ float4 tree_shared4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
 }
 
 template <int D, bool E4M3>
@@ -454,6 +464,11 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
           // The slot's last scales have been read: the S of two blocks ago, whose stage K has taken, was issued behind the P of
           // two blocks before that.
           const int slot = n % kTreeScaleSlots, key = row0_mine + lane;
+          if (!((there >> lane) & 1)) ks = vs = 0.f;
+          if (!span.whole(block0 + n) && !(fabsf(vs) <= 3.402823466e38f)) {  // (the weight of who does not see it would not be 0)
+            vs = 0.f;
+            atomicExch(&sm.bad, 1u);
+          }
           sm.k_scale[slot][key] = ks;
           sm.v_scale[slot][key] = vs;
           sm.v_log[slot][key] = tree_log2(vs);
@@ -578,129 +593,147 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
         if (E4M3 && !wait_all(&sm.scale_full[slot], (n / kTreeScaleSlots) & 1)) { ok = false; break; }
         if (!wait_all(&sm.s_full[s], (n >> 1) & 1)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const float* k_scale = &sm.k_scale[slot][g * kTreeGroupKeys];
-        const float* v_log = &sm.v_log[slot][g * kTreeGroupKeys];
-        const float* v_scale = &sm.v_scale[slot][g * kTreeGroupKeys];
+        const uint32_t k_scale = smem_u32(&sm.k_scale[slot][g * kTreeGroupKeys]), v_log = smem_u32(&sm.v_log[slot][g * kTreeGroupKeys]);
+        const uint32_t v_scale = smem_u32(&sm.v_scale[slot][g * kTreeGroupKeys]);
         const uint64_t times2 = pair_of(times, times);
-        // Half of the group's scores in base-2 units.  They are fetched twice, for the maximum and for the weights: 64 at once do not
-        // fit a thread's registers beside the rest, and what spills goes to L2 (shared memory leaves L1 next to nothing).
-        auto scores = [&](int half, uint32_t (&sv)[32]) {
-          tmem_load_32(s_addr + half * 32, sv);
+        constexpr int PIECE = E4M3 ? 16 : 32;
+        // A piece of the group's scores in base-2 units, minus `shift`.  (64 at once do not fit a thread's registers beside the rest,
+        // and what spills goes to L2: shared memory leaves L1 next to nothing.)
+        auto scores = [&](int piece, float shift, uint32_t (&sv)[PIECE]) {
+          if constexpr (PIECE == 32) tmem_load_32(s_addr + piece * PIECE, sv);
+          else tmem_load_16(s_addr + piece * PIECE, sv);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          const bool capped = rows.extras.cap > 0.f;
+          const uint64_t less2 = capped ? pair_of(0.f, 0.f) : pair_of(-shift, -shift);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            uint64_t x = pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-            if (E4M3) x = mul_pairs(x, *reinterpret_cast<const uint64_t*>(k_scale + half * 32 + i));
-            x = mul_pairs(x, times2);
-            float x0, x1;
-            halves_of(x, x0, x1);
-            sv[i] = __float_as_uint(x0);
-            sv[i + 1] = __float_as_uint(x1);
+          for (int i = 0; i < PIECE; i += 4) {
+            float4 ks = make_float4(1.f, 1.f, 1.f, 1.f);
+            if (E4M3) ks = tree_shared4(k_scale + (piece * PIECE + i) * 4);
+            uint64_t x = pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), y = pair_of(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
+            if (E4M3) {
+              x = mul_pairs(x, pair_of(ks.x, ks.y));
+              y = mul_pairs(y, pair_of(ks.z, ks.w));
+            }
+            float v[4];
+            halves_of(fma_pairs(x, times2, less2), v[0], v[1]);
+            halves_of(fma_pairs(y, times2, less2), v[2], v[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sv[i + e] = __float_as_uint(v[e]);
           }
-          if (rows.extras.cap > 0.f) {  // cap * tanh, by its exponential: off by 2^-22 of the cap
+          if (capped) {  // cap * tanh, by its exponential: off by 2^-22 of the cap
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              sv[i] = __float_as_uint(cap * (1.f - __fdividef(2.f, exp2_approx(__uint_as_float(sv[i]) * 2.8853900817779268f) + 1.f)));
+            for (int i = 0; i < PIECE; ++i)
+              sv[i] = __float_as_uint(cap * (1.f - __fdividef(2.f, exp2_approx(__uint_as_float(sv[i]) * 2.8853900817779268f) + 1.f)) - shift);
           }
           if (!whole) {
-            const uint32_t bits32 = half ? (uint32_t)(mask >> 32) : (uint32_t)mask;
+            const uint32_t bits = (uint32_t)(mask >> (piece * PIECE));
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((bits32 >> i) & 1)) sv[i] = 0xff800000u;  // -inf
+            for (int i = 0; i < PIECE; ++i)
+              if (!((bits >> i) & 1)) sv[i] = 0xff800000u;  // -inf
           }
         };
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, ox4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // The maxima in use are searched for where a row has none yet, and again where its weights outgrow them: of bfloat16
+        // weights the sum may reach 2^30, of float16 ones 2^14 (numbers keep their precision up to there, and far beyond).
+        bool search = __any_sync(0xffffffffu, (m_used == -INFINITY || (E4M3 && o_used == -INFINITY)) && mask != 0);
+        uint32_t packed[32];
+        float sum = 0.f;
+        for (int attempt = 0;; ++attempt) {
+          if (search) {
+            float mx = -INFINITY, ox = -INFINITY;
+#pragma unroll 1
+            for (int piece = 0; piece < kTreeGroupKeys / PIECE; ++piece) {
+              uint32_t sv[PIECE];
+              scores(piece, 0.f, sv);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t sv[32];
-          scores(half, sv);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float& m = mx4[(i >> 1) & 3];
-            m = max3(m, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-            if (E4M3) {
-              float z0, z1;
-              halves_of(add_pairs(pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), *reinterpret_cast<const uint64_t*>(v_log + half * 32 + i)),
-                        z0, z1);
-              float& o = ox4[(i >> 1) & 3];
-              o = max3(o, z0, z1);
-            }
-          }
-        }
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), ox = fmaxf(fmaxf(ox4[0], ox4[1]), fmaxf(ox4[2], ox4[3]));
-        // The maximum in use for the sum, and the one for O (of a 16-bit cache they are one).
-        const float m_new = fmaxf(m_used, mx);
-        const bool raise_sum = m_new > m_used + kTreeRaise || (m_used == -INFINITY && m_new > -INFINITY);
-        float corr = 1.f;
-        if (raise_sum) {
-          corr = exp2_approx(m_used - m_new);
-          l *= corr;
-          m_used = m_new;
-        }
-        bool raise = raise_sum;
-        if (E4M3) {
-          const float o_new = fmaxf(o_used, ox);
-          raise = o_new > o_used + kTreeRaise || (o_used == -INFINITY && o_new > -INFINITY);
-          corr = 1.f;
-          if (raise) {
-            corr = exp2_approx(o_used - o_new);
-            o_used = o_new;
-          }
-        }
-        // The group's O is in use by its product of the block before this one until that has completed.
-        if (n > 0 && __any_sync(0xffffffffu, raise)) {
-          if (!wait_all(&sm.pv_done[g], (n - 1) & 1)) { ok = false; break; }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t v[32];
-            tmem_load_32(o_addr + c0, v);
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
-            tmem_store_32(o_addr + c0, v);
-          }
-        }
-        const float shift = m_used == -INFINITY ? 0.f : m_used;
-        // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0)
-        const float units = E4M3 && o_used != -INFINITY ? exp2_approx(fminf(shift - o_used, 126.f)) : 0.f;
-        const uint64_t shift2 = pair_of(-shift, -shift), units2 = pair_of(units, units);
-        uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t sv[32], packed[16];
-          scores(half, sv);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float x0, x1;
-            halves_of(add_pairs(pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), shift2), x0, x1);
-            const uint64_t p = pair_of(exp2_approx(x0), exp2_approx(x1));
-            uint64_t& sum = sum4[(i >> 1) & 3];
-            float w0, w1;
-            if (E4M3) {
-              sum = add_pairs(sum, p);
-              halves_of(mul_pairs(p, mul_pairs(*reinterpret_cast<const uint64_t*>(v_scale + half * 32 + i), units2)), w0, w1);
-              if (!whole) {  // (0 times the scale of a row that is not finite, or of nobody's, is not 0)
-                w0 = sv[i] == 0xff800000u ? 0.f : w0;
-                w1 = sv[i + 1] == 0xff800000u ? 0.f : w1;
+              for (int i = 0; i < PIECE; i += 4) {
+                mx = fmaxf(max3(mx, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), fmaxf(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])));
+                if (E4M3) {
+                  const float4 vl = tree_shared4(v_log + (piece * PIECE + i) * 4);
+                  ox = fmaxf(max3(ox, __uint_as_float(sv[i]) + vl.x, __uint_as_float(sv[i + 1]) + vl.y),
+                             fmaxf(__uint_as_float(sv[i + 2]) + vl.z, __uint_as_float(sv[i + 3]) + vl.w));
+                }
               }
-              const __half2 pair = __floats2half2_rn(w0, w1);
-              packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
-            } else {  // the sum is that of the weights as the product takes them
-              halves_of(p, w0, w1);
-              const __nv_bfloat162 pair = __floats2bfloat162_rn(w0, w1);
-              const uint32_t both = *reinterpret_cast<const uint32_t*>(&pair);
-              packed[i >> 1] = both;
-              sum = add_pairs(sum, pair_of(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)));
+            }
+            // The maximum for the sum, and the one for O (of a 16-bit cache they are one).
+            const float m_new = fmaxf(m_used, mx);
+            float corr = 1.f;
+            if (m_new > m_used) {
+              corr = exp2_approx(m_used - m_new);
+              l *= corr;
+              m_used = m_new;
+            }
+            if (E4M3) {
+              const float o_new = fmaxf(o_used, ox);
+              corr = 1.f;
+              if (o_new > o_used) {
+                corr = exp2_approx(o_used - o_new);
+                o_used = o_new;
+              }
+            }
+            // The group's O is in use by its product of the block before this one until that has completed.
+            if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+              if (!wait_all(&sm.pv_done[g], (n - 1) & 1)) { ok = false; break; }
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+              for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t v[32];
+                tmem_load_32(o_addr + c0, v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+                tmem_store_32(o_addr + c0, v);
+              }
             }
           }
-          tmem_store_16(s_addr + half * 16, packed);
-        }
-        {
+          const float shift = m_used == -INFINITY ? 0.f : m_used;
+          // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0)
+          const float units = E4M3 && o_used != -INFINITY ? exp2_approx(fminf(shift - o_used, 126.f)) : 0.f;
+          const uint64_t units2 = pair_of(units, units);
+          uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull}, weight4[2] = {0ull, 0ull};
+#pragma unroll
+          for (int piece = 0; piece < kTreeGroupKeys / PIECE; ++piece) {
+            uint32_t sv[PIECE];
+            scores(piece, shift, sv);
+#pragma unroll
+            for (int i = 0; i < PIECE; i += 4) {
+              float4 vs = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (E4M3) vs = tree_shared4(v_scale + (piece * PIECE + i) * 4);
+              const uint64_t scale2[2] = {pair_of(vs.x, vs.y), pair_of(vs.z, vs.w)};
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                const uint64_t p = pair_of(exp2_approx(__uint_as_float(sv[i + e])), exp2_approx(__uint_as_float(sv[i + e + 1])));
+                uint64_t& total = sum4[((i + e) >> 1) & 3];
+                float w0, w1;
+                if (E4M3) {
+                  total = add_pairs(total, p);
+                  halves_of(mul_pairs(p, mul_pairs(scale2[e >> 1], units2)), w0, w1);
+                  weight4[e >> 1] = add_pairs(weight4[e >> 1], pair_of(w0, w1));
+                  const __half2 pair = __floats2half2_rn(w0, w1);
+                  packed[piece * (PIECE / 2) + ((i + e) >> 1)] = *reinterpret_cast<const uint32_t*>(&pair);
+                } else {  // the sum is that of the weights as the product takes them
+                  halves_of(p, w0, w1);
+                  const __nv_bfloat162 pair = __floats2bfloat162_rn(w0, w1);
+                  const uint32_t both = *reinterpret_cast<const uint32_t*>(&pair);
+                  packed[piece * (PIECE / 2) + ((i + e) >> 1)] = both;
+                  total = add_pairs(total, pair_of(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)));
+                }
+              }
+            }
+          }
           float even, odd;
           halves_of(add_pairs(add_pairs(sum4[0], sum4[1]), add_pairs(sum4[2], sum4[3])), even, odd);
-          l += even + odd;
+          sum = even + odd;
+          bool outgrown = sum > kTreeMostSum;
+          if (E4M3) {
+            halves_of(add_pairs(weight4[0], weight4[1]), even, odd);
+            outgrown = outgrown || even + odd > kTreeMostWeight;
+          }
+          if (search || !__any_sync(0xffffffffu, outgrown)) break;
+          search = true;
         }
+        if (!ok) break;
+        tmem_store_32(s_addr, packed);
+        l += sum;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -753,11 +786,10 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
             for (int i = 0; i < 16; i += 4) store4(to + i, make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
           }
         }
-        if (!E4M3 && sm.bad && live) {  // values that are not finite join the sums of the rows that see them
-          const __nv_bfloat16* values = reinterpret_cast<const __nv_bfloat16*>(cache.v);
+        if (sm.bad && live) {  // values that are not finite join the sums of the rows that see them
 #pragma unroll 1
           for (int e = g * SIDE; e < (g + 1) * SIDE; ++e) {
-            const float more = tree_not_finite(sm, r, e, block0, block1, values, cache, table, kv_head, rows.bits, rows.words, rows.keep_first);
+            const float more = tree_not_finite<D, E4M3>(sm, r, e, block0, block1, cache, table, kv_head, rows.bits, rows.words, rows.keep_first);
             if (more == 0.f) continue;
             if (alone) {
               __nv_bfloat16* to = out + (size_t)token * out_stride + (size_t)head * D + e;
