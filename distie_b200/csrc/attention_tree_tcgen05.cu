@@ -54,7 +54,7 @@ constexpr int kTreeKStages = 2, kTreeVStages = 3, kTreeScaleSlots = 4;
 constexpr int kTreeHalf = kTreeRows * 128;  // bytes of one [128 rows x 64 elements] swizzled half tile
 constexpr int kTreeMostNodes = 256;
 constexpr int kTreePages = 2048;   // page ids of a CTA's share that are kept in shared memory
-constexpr float kTreeMostSum = 1073741824.f, kTreeMostWeight = 16384.f;  // of a row's weights of 64 keys
+constexpr float kTreeMostSum = 1073741824.f, kTreeMostWeight = 16384.f;  // of a row's weights of 32 keys
 
 // The blocks of 128 keys that a tile of rows walks: those of the kept first keys, then those from the window's start on.
 struct TreeSpan {
@@ -582,6 +582,8 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
       };
       ok = wait_all(&sm.q_full, 0);
       const float times = E4M3 ? sm.q_times[r] : (rows.extras.cap > 0.f ? rows.extras.cap_pre : rows.scale_log2);
+      const uint64_t times2 = pair_of(times, times);
+      const bool capped = rows.extras.cap > 0.f;
       const float cap = rows.extras.cap * 1.4426950408889634f;
       float m_used = -INFINITY, o_used = -INFINITY, l = 0.f;  // o_used: the maximum that P is taken with, of scores with the values' scales
       for (int n = 0; n < blocks && ok; ++n) {
@@ -593,24 +595,23 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
         if (E4M3 && !wait_all(&sm.scale_full[slot], (n / kTreeScaleSlots) & 1)) { ok = false; break; }
         if (!wait_all(&sm.s_full[s], (n >> 1) & 1)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t k_scale = smem_u32(&sm.k_scale[slot][g * kTreeGroupKeys]), v_log = smem_u32(&sm.v_log[slot][g * kTreeGroupKeys]);
-        const uint32_t v_scale = smem_u32(&sm.v_scale[slot][g * kTreeGroupKeys]);
-        const uint64_t times2 = pair_of(times, times);
-        constexpr int PIECE = E4M3 ? 16 : 32;
-        // A piece of the group's scores in base-2 units, minus `shift`.  (64 at once do not fit a thread's registers beside the rest,
-        // and what spills goes to L2: shared memory leaves L1 next to nothing.)
-        auto scores = [&](int piece, float shift, uint32_t (&sv)[PIECE]) {
-          if constexpr (PIECE == 32) tmem_load_32(s_addr + piece * PIECE, sv);
-          else tmem_load_16(s_addr + piece * PIECE, sv);
+        const uint32_t scales = smem_u32(&sm.k_scale[slot][g * kTreeGroupKeys]);
+        // 32 keys at a time: 64 scores do not fit a thread's registers beside the rest, and what spills goes to L2 (shared memory
+        // leaves L1 next to nothing).  P, two keys a column, takes the columns of scores that have been read.
+#pragma unroll 1
+        for (int piece = 0; piece < 2; ++piece) {
+          uint32_t sv[32];  // scores in base-2 units, less the maximum in use
+          tmem_load_32(s_addr + piece * 32, sv);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          const bool capped = rows.extras.cap > 0.f;
+          const uint32_t bits = (uint32_t)(mask >> (piece * 32));
+          const uint32_t k_scale = scales + piece * 128, v_scale = k_scale + (uint32_t)sizeof(sm.k_scale), v_log = v_scale + (uint32_t)sizeof(sm.v_scale);
+          float shift = m_used == -INFINITY ? 0.f : m_used;
           const uint64_t less2 = capped ? pair_of(0.f, 0.f) : pair_of(-shift, -shift);
 #pragma unroll
-          for (int i = 0; i < PIECE; i += 4) {
-            float4 ks = make_float4(1.f, 1.f, 1.f, 1.f);
-            if (E4M3) ks = tree_shared4(k_scale + (piece * PIECE + i) * 4);
+          for (int i = 0; i < 32; i += 4) {
             uint64_t x = pair_of(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), y = pair_of(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
             if (E4M3) {
+              const float4 ks = tree_shared4(k_scale + i * 4);
               x = mul_pairs(x, pair_of(ks.x, ks.y));
               y = mul_pairs(y, pair_of(ks.z, ks.w));
             }
@@ -622,82 +623,90 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
           }
           if (capped) {  // cap * tanh, by its exponential: off by 2^-22 of the cap
 #pragma unroll
-            for (int i = 0; i < PIECE; ++i)
+            for (int i = 0; i < 32; ++i)
               sv[i] = __float_as_uint(cap * (1.f - __fdividef(2.f, exp2_approx(__uint_as_float(sv[i]) * 2.8853900817779268f) + 1.f)) - shift);
           }
           if (!whole) {
-            const uint32_t bits = (uint32_t)(mask >> (piece * PIECE));
 #pragma unroll
-            for (int i = 0; i < PIECE; ++i)
+            for (int i = 0; i < 32; ++i)
               if (!((bits >> i) & 1)) sv[i] = 0xff800000u;  // -inf
           }
-        };
-        // The maxima in use are searched for where a row has none yet, and again where its weights outgrow them: of bfloat16
-        // weights the sum may reach 2^30, of float16 ones 2^14 (numbers keep their precision up to there, and far beyond).
-        bool search = __any_sync(0xffffffffu, (m_used == -INFINITY || (E4M3 && o_used == -INFINITY)) && mask != 0);
-        uint32_t packed[32];
-        float sum = 0.f;
-        for (int attempt = 0;; ++attempt) {
-          if (search) {
-            float mx = -INFINITY, ox = -INFINITY;
+          // The maxima in use (whole numbers: what they scale, they scale exactly) are raised where a row has none yet, and where
+          // its weights outgrow them: the sum of 32 bfloat16 weights may reach 2^30, of float16 ones 2^14.
+          bool search = __any_sync(0xffffffffu, (m_used == -INFINITY || (E4M3 && o_used == -INFINITY)) && bits != 0);
+          uint32_t packed[16];
+          float sum;
 #pragma unroll 1
-            for (int piece = 0; piece < kTreeGroupKeys / PIECE; ++piece) {
-              uint32_t sv[PIECE];
-              scores(piece, 0.f, sv);
+          while (true) {
+            if (search) {
+              float mx = -INFINITY, ox = -INFINITY;
 #pragma unroll
-              for (int i = 0; i < PIECE; i += 4) {
+              for (int i = 0; i < 32; i += 4) {
                 mx = fmaxf(max3(mx, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), fmaxf(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])));
                 if (E4M3) {
-                  const float4 vl = tree_shared4(v_log + (piece * PIECE + i) * 4);
+                  const float4 vl = tree_shared4(v_log + i * 4);
                   ox = fmaxf(max3(ox, __uint_as_float(sv[i]) + vl.x, __uint_as_float(sv[i + 1]) + vl.y),
                              fmaxf(__uint_as_float(sv[i + 2]) + vl.z, __uint_as_float(sv[i + 3]) + vl.w));
                 }
               }
-            }
-            // The maximum for the sum, and the one for O (of a 16-bit cache they are one).
-            const float m_new = fmaxf(m_used, mx);
-            float corr = 1.f;
-            if (m_new > m_used) {
-              corr = exp2_approx(m_used - m_new);
-              l *= corr;
-              m_used = m_new;
-            }
-            if (E4M3) {
-              const float o_new = fmaxf(o_used, ox);
-              corr = 1.f;
-              if (o_new > o_used) {
-                corr = exp2_approx(o_used - o_new);
-                o_used = o_new;
+              // The maximum for the sum, and the one for O (of a 16-bit cache they are one).
+              const float m_new = fmaxf(m_used, shift + ceilf(mx));
+              float corr = 1.f;
+              if (E4M3) {
+                const float o_new = fmaxf(o_used, shift + ceilf(ox));
+                if (o_new > o_used) {
+                  corr = exp2_approx(o_used - o_new);
+                  o_used = o_new;
+                }
               }
-            }
-            // The group's O is in use by its product of the block before this one until that has completed.
-            if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-              if (!wait_all(&sm.pv_done[g], (n - 1) & 1)) { ok = false; break; }
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              if (m_new > m_used) {
+                const float down = exp2_approx(m_used - m_new), less = m_new - shift;
+                if (!E4M3) corr = down;
+                l *= down;
+                m_used = shift = m_new;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) - less);
+              }
+              if ((n > 0 || piece > 0) && __any_sync(0xffffffffu, corr != 1.f)) {
+                if (n > 0) {  // the group's O is in use by its product of the block before this one until that has completed
+                  if (!wait_all(&sm.pv_done[g], (n - 1) & 1)) { ok = false; break; }
+                  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-              for (int c0 = 0; c0 < D; c0 += 32) {
-                uint32_t v[32];
-                tmem_load_32(o_addr + c0, v);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                  for (int c0 = 0; c0 < D; c0 += 16) {
+                    tmem_load_16(o_addr + c0, packed);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
-                tmem_store_32(o_addr + c0, v);
+                    for (int i = 0; i < 16; ++i) packed[i] = __float_as_uint(__uint_as_float(packed[i]) * corr);
+                    tmem_store_16(o_addr + c0, packed);
+                  }
+                }
+                if (piece > 0) {  // and the weights of the block's first 32 keys
+                  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                  tmem_load_16(s_addr, packed);
+                  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    if (E4M3) {
+                      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&packed[i]));
+                      const __half2 pair = __floats2half2_rn(f.x * corr, f.y * corr);
+                      packed[i] = *reinterpret_cast<const uint32_t*>(&pair);
+                    } else {
+                      const __nv_bfloat162 pair = __floats2bfloat162_rn(__uint_as_float(packed[i] << 16) * corr, __uint_as_float(packed[i] & 0xffff0000u) * corr);
+                      packed[i] = *reinterpret_cast<const uint32_t*>(&pair);
+                    }
+                  }
+                  tmem_store_16(s_addr, packed);
+                }
               }
             }
-          }
-          const float shift = m_used == -INFINITY ? 0.f : m_used;
-          // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0)
-          const float units = E4M3 && o_used != -INFINITY ? exp2_approx(fminf(shift - o_used, 126.f)) : 0.f;
-          const uint64_t units2 = pair_of(units, units);
-          uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull}, weight4[2] = {0ull, 0ull};
+            // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0)
+            const float units = E4M3 && o_used != -INFINITY ? exp2_approx(fminf(shift - o_used, 126.f)) : 0.f;
+            const uint64_t units2 = pair_of(units, units);
+            uint64_t sum4[4] = {0ull, 0ull, 0ull, 0ull}, weight4[2] = {0ull, 0ull};
 #pragma unroll
-          for (int piece = 0; piece < kTreeGroupKeys / PIECE; ++piece) {
-            uint32_t sv[PIECE];
-            scores(piece, shift, sv);
-#pragma unroll
-            for (int i = 0; i < PIECE; i += 4) {
+            for (int i = 0; i < 32; i += 4) {
               float4 vs = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (E4M3) vs = tree_shared4(v_scale + (piece * PIECE + i) * 4);
+              if (E4M3) vs = tree_shared4(v_scale + i * 4);
               const uint64_t scale2[2] = {pair_of(vs.x, vs.y), pair_of(vs.z, vs.w)};
 #pragma unroll
               for (int e = 0; e < 4; e += 2) {
@@ -706,34 +715,36 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                 float w0, w1;
                 if (E4M3) {
                   total = add_pairs(total, p);
-                  halves_of(mul_pairs(p, mul_pairs(scale2[e >> 1], units2)), w0, w1);
-                  weight4[e >> 1] = add_pairs(weight4[e >> 1], pair_of(w0, w1));
+                  const uint64_t w = mul_pairs(p, mul_pairs(scale2[e >> 1], units2));
+                  weight4[e >> 1] = add_pairs(weight4[e >> 1], w);
+                  halves_of(w, w0, w1);
                   const __half2 pair = __floats2half2_rn(w0, w1);
-                  packed[piece * (PIECE / 2) + ((i + e) >> 1)] = *reinterpret_cast<const uint32_t*>(&pair);
+                  packed[(i + e) >> 1] = *reinterpret_cast<const uint32_t*>(&pair);
                 } else {  // the sum is that of the weights as the product takes them
                   halves_of(p, w0, w1);
                   const __nv_bfloat162 pair = __floats2bfloat162_rn(w0, w1);
                   const uint32_t both = *reinterpret_cast<const uint32_t*>(&pair);
-                  packed[piece * (PIECE / 2) + ((i + e) >> 1)] = both;
+                  packed[(i + e) >> 1] = both;
                   total = add_pairs(total, pair_of(__uint_as_float(both << 16), __uint_as_float(both & 0xffff0000u)));
                 }
               }
             }
+            float even, odd;
+            halves_of(add_pairs(add_pairs(sum4[0], sum4[1]), add_pairs(sum4[2], sum4[3])), even, odd);
+            sum = even + odd;
+            bool outgrown = sum > kTreeMostSum;
+            if (E4M3) {
+              halves_of(add_pairs(weight4[0], weight4[1]), even, odd);
+              outgrown = outgrown || even + odd > kTreeMostWeight;
+            }
+            if (search || !__any_sync(0xffffffffu, outgrown)) break;
+            search = true;
           }
-          float even, odd;
-          halves_of(add_pairs(add_pairs(sum4[0], sum4[1]), add_pairs(sum4[2], sum4[3])), even, odd);
-          sum = even + odd;
-          bool outgrown = sum > kTreeMostSum;
-          if (E4M3) {
-            halves_of(add_pairs(weight4[0], weight4[1]), even, odd);
-            outgrown = outgrown || even + odd > kTreeMostWeight;
-          }
-          if (search || !__any_sync(0xffffffffu, outgrown)) break;
-          search = true;
+          if (!ok) break;
+          tmem_store_16(s_addr + piece * 16, packed);
+          l += sum;
         }
         if (!ok) break;
-        tmem_store_32(s_addr, packed);
-        l += sum;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
