@@ -66,9 +66,9 @@ struct TreeSpan {
   __device__ __forceinline__ int key0(int j) const { return j < kept_blocks ? j * kTreeKeys : start + (j - kept_blocks) * kTreeKeys; }
   __device__ __forceinline__ int key_end(int j) const { return j < kept_blocks ? min(kept, start) : keys; }
   // Whether every row of the tile sees every key of the block.
-  __device__ __forceinline__ bool whole(int j) const {
-    return j >= kept_blocks && key0(j) >= newest && key0(j) + kTreeKeys <= past;
-  }
+  __device__ __forceinline__ bool whole(int j) const { return j >= whole_from() && j < whole_to(); }
+  __device__ __forceinline__ int whole_from() const { return kept_blocks + (max(newest - start, 0) + kTreeKeys - 1) / kTreeKeys; }
+  __device__ __forceinline__ int whole_to() const { return kept_blocks + max(past - start, 0) / kTreeKeys; }
 };
 
 template <int D>
@@ -573,25 +573,19 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
       const uint32_t lane_base = tmem + ((uint32_t)(quadrant * 32) << 16);
       const uint32_t o_addr = lane_base + O_COL + g * D;
       bool ok = true;
-      auto wait_all = [&](uint64_t* bar, uint32_t parity) {  // one lane polls
-        int done = 1;
-        if (lane == 0) done = mbar_wait_unless(bar, parity, failed) ? 1 : 0;
-        done = __shfl_sync(0xffffffffu, done, 0);
-        __syncwarp();
-        return done != 0;
-      };
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_unless(bar, parity, failed)) != 0; };
       ok = wait_all(&sm.q_full, 0);
       const float times = E4M3 ? sm.q_times[r] : (rows.extras.cap > 0.f ? rows.extras.cap_pre : rows.scale_log2);
       const uint64_t times2 = pair_of(times, times);
       const bool capped = rows.extras.cap > 0.f;
       const float cap = rows.extras.cap * 1.4426950408889634f;
+      const int whole0 = span.whole_from(), whole1 = span.whole_to();
       float m_used = -INFINITY, o_used = -INFINITY, l = 0.f;  // o_used: the maximum that P is taken with, of scores with the values' scales
       for (int n = 0; n < blocks && ok; ++n) {
         const int j = block0 + n, s = n & 1, slot = n % kTreeScaleSlots;
-        const int key0 = span.key0(j) + g * kTreeGroupKeys;
         const uint32_t s_addr = lane_base + s * kTreeKeys + g * kTreeGroupKeys;
-        const bool whole = span.whole(j);
-        const uint64_t mask = whole ? ~0ull : tree_seen64(sm, r, key0, span.key_end(j), rows.bits, rows.words, rows.keep_first);
+        const bool whole = j >= whole0 && j < whole1;
+        const uint64_t mask = whole ? ~0ull : tree_seen64(sm, r, span.key0(j) + g * kTreeGroupKeys, span.key_end(j), rows.bits, rows.words, rows.keep_first);
         if (E4M3 && !wait_all(&sm.scale_full[slot], (n / kTreeScaleSlots) & 1)) { ok = false; break; }
         if (!wait_all(&sm.s_full[s], (n >> 1) & 1)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
