@@ -201,6 +201,11 @@ __device__ __forceinline__ float4 tree_shared4(uint32_t at) {
   return v;
 }
 
+__device__ __forceinline__ void tree_loaded(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
 template <int D, bool E4M3>
 __global__ void __launch_bounds__(kTreeThreads, 1)
 attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int direct,
@@ -592,11 +597,15 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
         const uint32_t scales = smem_u32(&sm.k_scale[slot][g * kTreeGroupKeys]);
         // 32 keys at a time: 64 scores do not fit a thread's registers beside the rest, and what spills goes to L2 (shared memory
         // leaves L1 next to nothing).  P, two keys a column, takes the columns of scores that have been read.
-#pragma unroll 1
+        uint32_t next[32];
+#pragma unroll (E4M3 ? 1 : 2)
         for (int piece = 0; piece < 2; ++piece) {
           uint32_t sv[32];  // scores in base-2 units, less the maximum in use
-          tmem_load_32(s_addr + piece * 32, sv);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (E4M3 || piece == 0) tmem_load_32(s_addr + piece * 32, next);
+          tree_loaded(next);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sv[i] = next[i];
+          if (!E4M3 && piece == 0) tmem_load_32(s_addr + 32, next);
           const uint32_t bits = (uint32_t)(mask >> (piece * 32));
           const uint32_t k_scale = scales + piece * 128, v_scale = k_scale + (uint32_t)sizeof(sm.k_scale), v_log = v_scale + (uint32_t)sizeof(sm.v_scale);
           float shift = m_used == -INFINITY ? 0.f : m_used;
