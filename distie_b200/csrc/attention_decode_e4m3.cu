@@ -16,10 +16,11 @@
 // and one byte permutation makes them two pairs of keys.  q is multiplied by a power of two per head that brings its largest
 // element to [1, 2), so that float16 holds it exactly down to 2^-24 of that.
 //
-// Scales: s^k multiplies the finished score.  s^v cannot ride on V without rounding it; p_j s^v_j is taken as one exponential,
-// exp2(score_j + log2 s^v_j - m'), with a running maximum m' of its own beside the softmax's, so the weights that the second
-// product gets in float16 have a largest element of 1 however the scales differ, and are off by at most 2^-11 of
-// themselves (or of 2^-14).  Sums and maxima are float32.  The warps, and with several splits the CTAs, are merged in the
+// Scales: s^k multiplies the finished score.  s^v cannot ride on V without rounding it; p_j s^v_j goes into the second product
+// in float16, in units of a running maximum m' of its own beside the softmax's m: p_j (s^v_j 2^(m - m')), however the scales
+// differ at most a few, and off by at most 2^-11 of itself (or of 2^-14).  Both maxima are whole numbers (what they scale,
+// they scale exactly) and are not searched for in every group, only in a head's first and where weights outgrow the ones in
+// use: no shuffles and no correction of O in most groups.  Sums and maxima are float32.  The warps, and with several splits the CTAs, are merged in the
 // softmax's units: inside the cluster up to 8 splits, by a second kernel beyond.
 #include <cuda_fp16.h>
 
@@ -30,8 +31,9 @@ namespace distie {
 
 constexpr int kDecWarps = 4;
 constexpr int kDecKeys = 32;      // keys of a group
-constexpr int kDecPages = 1024;   // page ids of a split that are kept in shared memory
+constexpr int kDecPages = 992;    // page ids of a split that are kept in shared memory (so many, that three CTAs fit an SM)
 constexpr int kDecClusterSplits = 8;
+constexpr float kDecMostSum = 1073741824.f, kDecMostWeight = 16384.f;  // of a lane's four weights of a head
 
 __device__ __forceinline__ void dec_copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -75,6 +77,22 @@ __device__ __forceinline__ float dec_log2(float x) {  // of a positive number or
   return y;
 }
 
+// Into the shared memory of CTA `rank` of the cluster, where `local` lies in this one's.
+__device__ __forceinline__ void cluster_store(float* local, uint32_t rank, float v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_store(float* local, uint32_t rank, const float4& v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void store_row4(__nv_bfloat16* to, const float4& v) {  // (rows of the output may lie at any stride)
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+  to[0] = lo.x; to[1] = lo.y; to[2] = hi.x; to[3] = hi.y;
+}
+
 template <int D>
 __device__ __forceinline__ uint32_t dec_offset(int row, int piece) {  // of a 16-byte piece of a row: free of bank conflicts by 8 rows
   return (uint32_t)(row * D + ((D == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3)) << 4));
@@ -90,14 +108,17 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
   constexpr int STAGE = 2 * TILE + 2 * kDecKeys * 4;
   constexpr int RPI = 32 / MT;                // rows that one copy instruction of the warp covers
   extern __shared__ __align__(128) unsigned char dyn[];
-  // The ring [warp][stage][K | V | scales of K | of V]; behind the main loop the merge areas.
-  float(*sh_o)[NH * 8][D + 1] = reinterpret_cast<float(*)[NH * 8][D + 1]>(dyn);
-  float(*cl_o)[D] = reinterpret_cast<float(*)[D]>(dyn + kDecWarps * NH * 8 * (D + 1) * sizeof(float));
+  // The ring [warp][stage][K | V | scales of K | of V]; behind the main loop the warps' sums.
+  constexpr int ROW = D + 8;  // (free of bank conflicts where the warps put theirs down)
+  float(*sh_o)[NH * 8][ROW] = reinterpret_cast<float(*)[NH * 8][ROW]>(dyn);
   __shared__ float sh_m[kDecWarps][NH * 8], sh_l[kDecWarps][NH * 8], sh_f[kDecWarps][NH * 8];
-  __shared__ float cl_m[NH * 8], cl_l[NH * 8];
+  // What the CTAs of the cluster send here: their sums of this CTA's share of the output, their maxima and sums of weights.
+  __shared__ alignas(16) float from_o[NH * 8 * D + kDecClusterSplits * 4];  // (the last share may be shorter than the others)
+  __shared__ float from_m[kDecClusterSplits][NH * 8], from_l[kDecClusterSplits][NH * 8];
   __shared__ int sh_pages[kDecPages];
 
   grid_dependency_release();
+  if (cluster_merge) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (waited for before anything is sent)
   const int t = blockIdx.x, split = blockIdx.z, num_splits = gridDim.z;
   const int kv_head = blockIdx.y / head_chunks, chunk = blockIdx.y % head_chunks;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
@@ -185,6 +206,14 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // (q is asked for first: behind the copies its loads would queue, and nothing begins without it.  Columns behind the last
+  // head are nobody's: copies of it, so that no load hangs on a branch.)
+  uint2 q_raw[NH][MT];
+#pragma unroll
+  for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+    for (int ks = 0; ks < MT; ++ks)
+      q_raw[nh][ks] = __ldcg(reinterpret_cast<const uint2*>(q + (size_t)t * q_stride + (size_t)(head0 + min(nh * 8 + g, heads_here - 1)) * D + 16 * ks + 4 * c));
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) issue(warp + s * kDecWarps, s);
 
@@ -193,13 +222,12 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
   float times[NH][2];  // what turns the raw products of columns 2 c and 2 c + 1 into scores, before the keys' scales
 #pragma unroll
   for (int nh = 0; nh < NH; ++nh) {
-    const int hd = nh * 8 + g;
     float x[MT][4], most = 0.f;
 #pragma unroll
     for (int ks = 0; ks < MT; ++ks) {
-      // (columns behind the last head are nobody's: copies of it, so that no load hangs on a branch)
-      const float4 v = load4_cg(q + (size_t)t * q_stride + (size_t)(head0 + min(hd, heads_here - 1)) * D + 16 * ks + 4 * c);
-      x[ks][0] = v.x; x[ks][1] = v.y; x[ks][2] = v.z; x[ks][3] = v.w;
+      const uint2 raw = q_raw[nh][ks];
+      x[ks][0] = __uint_as_float(raw.x << 16); x[ks][1] = __uint_as_float(raw.x & 0xffff0000u);
+      x[ks][2] = __uint_as_float(raw.y << 16); x[ks][3] = __uint_as_float(raw.y & 0xffff0000u);
 #pragma unroll
       for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[ks][e]));
     }
@@ -218,7 +246,7 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
   }
 
   float o[NH][MT][4];  // O^T: dims 16 mt + 2 g (+ 1), heads 2 c (+ 1): [dim 2g: head, head + 1 | dim 2g + 1: head, head + 1]
-  float col_max[NH][2], col_sum[NH][2], out_max[NH][2];
+  float col_max[NH][2], col_sum[NH][2], out_max[NH][2], units[NH][2];  // units: 2^(col_max - out_max)
 #pragma unroll
   for (int nh = 0; nh < NH; ++nh) {
 #pragma unroll
@@ -228,9 +256,10 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       col_max[nh][e] = out_max[nh][e] = -INFINITY;
-      col_sum[nh][e] = 0.f;
+      col_sum[nh][e] = units[nh][e] = 0.f;
     }
   }
+  const float cap = rows.extras.cap * 1.4426950408889634f;
   const int lm_mat = lane >> 3, lm_row = lane & 7;
   int stage = 0;
   for (int grp = warp; grp < groups; grp += kDecWarps) {
@@ -273,70 +302,97 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
     }
     // ---- scales, mask, maxima, exponentials ------------------------------------------------------------------------
     constexpr int RK = kDecKeys / 8;  // keys of a lane: g, g + 8, ...
-    float ks_s[RK], vs_log[RK];
+    float ks_s[RK], vs_s[RK];
     bool keep[RK];
     const bool edge = base < lo_key || base + kDecKeys - 1 > hi_key;
 #pragma unroll
     for (int i = 0; i < RK; ++i) {
       ks_s[i] = scales[8 * i + g];
-      vs_log[i] = dec_log2(scales[kDecKeys + 8 * i + g]);
+      vs_s[i] = scales[kDecKeys + 8 * i + g];
       keep[i] = !edge || (base + 8 * i + g >= lo_key && base + 8 * i + g <= hi_key);
     }
     uint32_t pb[kDecKeys / 16][NH][2];
-    float corr[NH][2];
 #pragma unroll
     for (int nh = 0; nh < NH; ++nh) {
-      float w[RK][2];
+      float x[RK][2], w[RK][2], sum[2];  // scores less the maximum in use
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float x[RK], m = -INFINITY, mo = -INFINITY;
+        const float shift = col_max[nh][e] == -INFINITY ? 0.f : col_max[nh][e];
 #pragma unroll
         for (int i = 0; i < RK; ++i) {
-          float s = st[i >> 1][nh][(i & 1) * 2 + e] * (ks_s[i] * times[nh][e]);
-          if (rows.extras.cap > 0.f)  // cap * tanh, by its exponential: off by 2^-22 of the cap
-            s = rows.extras.cap * 1.4426950408889634f * (1.f - __fdividef(2.f, dec_exp2(s * 2.8853900817779268f) + 1.f));
-          x[i] = keep[i] ? s : -INFINITY;
-          w[i][e] = keep[i] ? s + vs_log[i] : -INFINITY;
-          m = fmaxf(m, x[i]);
-          mo = fmaxf(mo, w[i][e]);
+          const float raw = st[i >> 1][nh][(i & 1) * 2 + e], each = ks_s[i] * times[nh][e];
+          // (cap * tanh, by its exponential: off by 2^-22 of the cap)
+          const float s = rows.extras.cap > 0.f ? cap * (1.f - __fdividef(2.f, dec_exp2(raw * each * 2.8853900817779268f) + 1.f)) - shift
+                                                : fmaf(raw, each, -shift);
+          x[i][e] = keep[i] ? s : -INFINITY;
         }
-#pragma unroll
-        for (int d = 4; d <= 16; d <<= 1) {
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-          mo = fmaxf(mo, __shfl_xor_sync(0xffffffffu, mo, d));
-        }
-        m = fmaxf(col_max[nh][e], m);
-        mo = fmaxf(out_max[nh][e], mo);
-        const float shift = m == -INFINITY ? 0.f : m, out_shift = mo == -INFINITY ? 0.f : mo;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < RK; ++i) {
-          sum += dec_exp2(x[i] - shift);
-          w[i][e] = dec_exp2(w[i][e] - out_shift);
-        }
-        col_sum[nh][e] = col_sum[nh][e] * dec_exp2(col_max[nh][e] - shift) + sum;  // (exp2(-inf) is 0)
-        corr[nh][e] = dec_exp2(out_max[nh][e] - out_shift);
-        col_max[nh][e] = m;
-        out_max[nh][e] = mo;
       }
+      bool search = false;
+#pragma unroll 1
+      while (true) {
+        if (search) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float m = -INFINITY, mo = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < RK; ++i) {
+              m = fmaxf(m, x[i][e]);
+              mo = fmaxf(mo, keep[i] ? x[i][e] + dec_log2(vs_s[i]) : -INFINITY);
+            }
+#pragma unroll
+            for (int d = 4; d <= 16; d <<= 1) {
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+              mo = fmaxf(mo, __shfl_xor_sync(0xffffffffu, mo, d));
+            }
+            const float shift = col_max[nh][e] == -INFINITY ? 0.f : col_max[nh][e];
+            const float o_new = fmaxf(out_max[nh][e], shift + ceilf(mo)), m_new = fmaxf(col_max[nh][e], shift + ceilf(m));
+            const float corr = o_new > out_max[nh][e] ? dec_exp2(out_max[nh][e] - o_new) : 1.f;  // (exp2(-inf) is 0)
+            if (m_new > col_max[nh][e]) {
+              col_sum[nh][e] *= dec_exp2(col_max[nh][e] - m_new);
+#pragma unroll
+              for (int i = 0; i < RK; ++i) x[i][e] -= m_new - shift;
+            }
+            col_max[nh][e] = m_new;
+            out_max[nh][e] = o_new;
+            // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0)
+            units[nh][e] = o_new == -INFINITY ? 0.f : dec_exp2(fminf((m_new == -INFINITY ? 0.f : m_new) - o_new, 126.f));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              o[nh][mt][e] *= corr;
+              o[nh][mt][e + 2] *= corr;
+            }
+          }
+        }
+        bool outgrown = false;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float weights = 0.f;
+          sum[e] = 0.f;
+#pragma unroll
+          for (int i = 0; i < RK; ++i) {
+            const float p = dec_exp2(x[i][e]);
+            sum[e] += p;
+            w[i][e] = keep[i] ? p * (vs_s[i] * units[nh][e]) : 0.f;
+            weights += w[i][e];
+          }
+          outgrown = outgrown || sum[e] > kDecMostSum || weights > kDecMostWeight || col_max[nh][e] == -INFINITY || out_max[nh][e] == -INFINITY;
+        }
+        if (search || !__any_sync(0xffffffffu, outgrown)) break;
+        search = true;
+      }
+      col_sum[nh][0] += sum[0];
+      col_sum[nh][1] += sum[1];
 #pragma unroll
       for (int sub = 0; sub < kDecKeys / 16; ++sub) {
         pb[sub][nh][0] = dec_movmatrix(pack_half(w[2 * sub][0], w[2 * sub][1]));
         pb[sub][nh][1] = dec_movmatrix(pack_half(w[2 * sub + 1][0], w[2 * sub + 1][1]));
       }
     }
-    // ---- O^T = O^T * corr + V^T P^T --------------------------------------------------------------------------------
+    // ---- O^T += V^T P^T --------------------------------------------------------------------------------
     {
       const int key = lm_row + 8 * (lm_mat & 1);
 #pragma unroll
       for (int mt = 0; mt < MT; mt += 2) {
-#pragma unroll
-        for (int nh = 0; nh < NH; ++nh)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            o[nh][mt + u][0] *= corr[nh][0]; o[nh][mt + u][1] *= corr[nh][1];
-            o[nh][mt + u][2] *= corr[nh][0]; o[nh][mt + u][3] *= corr[nh][1];
-          }
 #pragma unroll
         for (int sub = 0; sub < kDecKeys / 16; ++sub) {
           uint32_t a[4];
@@ -371,73 +427,80 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
         sh_f[warp][hd] = out_max[nh][e];
       }
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        sh_o[warp][hd][16 * mt + 2 * g] = o[nh][mt][e];
-        sh_o[warp][hd][16 * mt + 2 * g + 1] = o[nh][mt][e + 2];
-      }
+      for (int mt = 0; mt < MT; ++mt) *reinterpret_cast<float2*>(&sh_o[warp][hd][16 * mt + 2 * g]) = make_float2(o[nh][mt][e], o[nh][mt][e + 2]);
     }
   __syncthreads();
-  for (int idx = threadIdx.x; idx < heads_here * D; idx += kDecWarps * 32) {
-    const int hd = idx / D, e = idx % D;
-    float m_all = -INFINITY;
+  if (threadIdx.x < heads_here) {  // a head's maximum and sum, and what a warp's sum of values counts
+    const int hd = threadIdx.x;
+    float m_all = -INFINITY, l_all = 0.f, factor[kDecWarps];
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) m_all = fmaxf(m_all, sh_m[w][hd]);
     const float shift = m_all == -INFINITY ? 0.f : m_all;
-    float l_all = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
       // (a warp without a key has a sum of 0; one whose scores are all NaN a sum of NaN, and both have no maximum)
-      const float l = sh_l[w][hd], weight = sh_m[w][hd] == -INFINITY ? l : exp2f(sh_m[w][hd] - shift);
-      l_all += l * weight;
-      acc += sh_o[w][hd][e] * (sh_f[w][hd] == -INFINITY ? l - l : exp2f(sh_f[w][hd] - shift));
+      const float l = sh_l[w][hd];
+      l_all += l * (sh_m[w][hd] == -INFINITY ? l : dec_exp2(sh_m[w][hd] - shift));
+      factor[w] = sh_f[w][hd] == -INFINITY ? l - l : dec_exp2(sh_f[w][hd] - shift);
     }
     const int head = head0 + hd;
-    if (num_splits == 1) {
-      const float inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
-      out[(size_t)t * out_stride + (size_t)head * D + e] = __float2bfloat16_rn(acc * inv);
-    } else if (cluster_merge) {
-      cl_o[hd][e] = acc;
-      if (e == 0) { cl_m[hd] = m_all; cl_l[hd] = l_all; }
-    } else {
+    float inv = 1.f;
+    if (num_splits == 1) inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) sh_f[w][hd] = factor[w] * inv;
+    if (cluster_merge) {
+      sh_m[0][hd] = m_all;
+      sh_l[0][hd] = l_all;
+    } else if (num_splits > 1) {
       const size_t row = ((size_t)t * rows.num_heads + head) * num_splits + split;
-      parts.o[row * D + e] = acc;
-      if (e == 0) {
-        parts.ml[row * 2] = m_all;
-        parts.ml[row * 2 + 1] = l_all;
-      }
+      parts.ml[row * 2] = m_all;
+      parts.ml[row * 2 + 1] = l_all;
     }
   }
-  if (num_splits > 1 && cluster_merge) {
-    // The splits of a (token, head chunk) are the CTAs of one cluster: each combines its share of the output elements from
-    // every CTA's shared memory, splits in order.
-    cluster_barrier();
-    const int total = heads_here * D, part = (total + num_splits - 1) / num_splits;
-    const int end = min(total, (split + 1) * part);
-    for (int idx = split * part + threadIdx.x; idx < end; idx += kDecWarps * 32) {
-      const int hd = idx / D, e = idx % D;
-      float ms[kDecClusterSplits], ls[kDecClusterSplits], os[kDecClusterSplits];
-#pragma unroll
-      for (int s = 0; s < kDecClusterSplits; ++s) {  // all loads from the other CTAs together
-        const bool there = s < num_splits;
-        ms[s] = there ? cluster_load(&cl_m[hd], s) : -INFINITY;
-        ls[s] = there ? cluster_load(&cl_l[hd], s) : 0.f;
-        os[s] = there ? cluster_load(&cl_o[hd][e], s) : 0.f;
-      }
-      float m_all = -INFINITY;
-#pragma unroll
-      for (int s = 0; s < kDecClusterSplits; ++s) m_all = fmaxf(m_all, ms[s]);
-      float l_all = 0.f, acc = 0.f;
-#pragma unroll
-      for (int s = 0; s < kDecClusterSplits; ++s) {
-        const float weight = ms[s] == -INFINITY ? ls[s] : exp2f(ms[s] - m_all);
-        l_all += ls[s] * weight;
-        acc += os[s] * weight;
-      }
-      const int head = head0 + hd;
-      const float inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
-      out[(size_t)t * out_stride + (size_t)head * D + e] = __float2bfloat16_rn(acc * inv);
+  if (cluster_merge) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all CTAs of the cluster have begun
+  __syncthreads();
+  // Of the cluster, CTA s puts together the part4 pieces of 4 elements from s * part4 on.
+  const int total4 = heads_here * (D / 4), part4 = (total4 + num_splits - 1) / num_splits;
+  if (cluster_merge)
+    for (int i = threadIdx.x; i < num_splits * heads_here; i += kDecWarps * 32) {
+      const int hd = i % heads_here, to = i / heads_here;
+      cluster_store(&from_m[split][hd], to, sh_m[0][hd]);
+      cluster_store(&from_l[split][hd], to, sh_l[0][hd]);
     }
-    cluster_barrier_exit();  // no CTA leaves while another may still read its shared memory
+  for (int i = threadIdx.x; i < total4; i += kDecWarps * 32) {
+    const int hd = i / (D / 4), e = i % (D / 4) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(&sh_o[w][hd][e]);
+      const float f = sh_f[w][hd];
+      acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+    }
+    if (num_splits == 1) {
+      store_row4(out + (size_t)t * out_stride + (size_t)(head0 + hd) * D + e, acc);
+    } else if (cluster_merge) {
+      const int to = i / part4;
+      cluster_store(&from_o[(split * part4 + i - to * part4) * 4], to, acc);
+    } else {
+      store4(parts.o + (((size_t)t * rows.num_heads + head0 + hd) * num_splits + split) * D + e, acc);
+    }
+  }
+  if (cluster_merge) {
+    cluster_barrier();  // everything has arrived
+    for (int i = threadIdx.x; i < min(part4, total4 - split * part4); i += kDecWarps * 32) {
+      const int hd = (split * part4 + i) / (D / 4), e = (split * part4 + i) % (D / 4) * 4, head = head0 + hd;
+      float m_all = -INFINITY, l_all = 0.f;
+      for (int s = 0; s < num_splits; ++s) m_all = fmaxf(m_all, from_m[s][hd]);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s = 0; s < num_splits; ++s) {  // splits in order
+        const float l = from_l[s][hd], weight = from_m[s][hd] == -INFINITY ? l : dec_exp2(from_m[s][hd] - m_all);
+        const float4 v = *reinterpret_cast<const float4*>(&from_o[(s * part4 + i) * 4]);
+        l_all += l * weight;
+        acc.x += v.x * weight; acc.y += v.y * weight; acc.z += v.z * weight; acc.w += v.w * weight;
+      }
+      const float inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
+      store_row4(out + (size_t)t * out_stride + (size_t)head * D + e, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    }
   }
 }
 
@@ -445,7 +508,7 @@ template <int D, int STAGES, int NH, bool PAGE16>
 static cudaError_t launch_decode(const dim3& grid, const __nv_bfloat16* q, int q_stride, __nv_bfloat16* out, int out_stride, const QueryRows& rows,
                                  const CachePages& cache, const Partials& parts, int head_chunks, int cluster_merge, int* error, cudaStream_t stream) {
   constexpr size_t ring = (size_t)kDecWarps * STAGES * (2 * kDecKeys * D + 2 * kDecKeys * 4);
-  constexpr size_t merge = (size_t)kDecWarps * NH * 8 * (D + 1) * sizeof(float) + (size_t)NH * 8 * D * sizeof(float);
+  constexpr size_t merge = (size_t)kDecWarps * NH * 8 * (D + 8) * sizeof(float);
   constexpr size_t shared = ring > merge ? ring : merge;
   auto kernel = attention_decode_e4m3_kernel<D, STAGES, NH, PAGE16>;
   if (shared > 48 * 1024) {

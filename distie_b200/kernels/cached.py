@@ -36,6 +36,21 @@ def tree_splits(tiles: int, blocks: int, sms: int) -> int:
     return best
 
 
+def decode_splits(blocks: int, keys: int, sms: int) -> int:
+    """Shares that the keys of ``blocks`` (token, group of heads) pairs are cut into (attention_decode_e4m3.cu): the number for
+    which the fullest SM takes the least time, three CTAs or fewer that of three (a CTA alone does not keep an SM busy), and a
+    CTA that of its keys and of 192 more for its start and end.  Up to 8 shares are joined inside the kernel, by a cluster of
+    CTAs; up to 12 are not worth a second kernel."""
+    best, least = 1, None
+    for splits in range(1, max(1, min(keys // 256, 64)) + 1):
+        if 8 < splits <= 12:
+            continue
+        cost = max(3, -(-blocks * splits // sms)) * (-(-keys // splits) + 192)
+        if least is None or cost < least:
+            best, least = splits, cost
+    return best
+
+
 class CachedRows:
     caches_in_8_bits = True
     drafted_tokens = True
@@ -230,9 +245,7 @@ class CachedRows:
             return False
         blocks = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 16)
         seen = min(step.max_kv_len, window or chunk or step.max_kv_len)
-        splits = max(1, min(3 * self.sm_count // blocks, seen // 256, 64))
-        if splits <= 12:
-            splits = min(splits, 8)  # joined inside the kernel, by a cluster of CTAs
+        splits = decode_splits(blocks, seen, self.sm_count)
         scratch = None
         if splits > 8:
             floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, head_dim, splits)
