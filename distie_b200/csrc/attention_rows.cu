@@ -187,66 +187,117 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   }
 }
 
-// Joins the parts of a (token, head): a block each.  A row of parts takes a group of threads, four columns a thread, and
-// the groups share out the splits, so that the loads of many of them are in flight together; the order of the additions
-// follows from the number of splits alone.
-constexpr int kMergeThreads = 256;
+// Joins the parts of (token, head) rows, SHARE warps a row.  Lane s looks at part s (and s + 32, ...): its maximum, its sum, and
+// with the row's maximum what it counts, so that the loads of the parts wait for nothing but their addresses; a lane owns four
+// columns (and, of more than 128, four more), and parts of up to 64 columns go to the halves (quarters, ...) of the warp in
+// turn.  The order of the additions follows from the numbers of splits and rows alone.  SHARE 4 where a row has more than 16
+// parts, or more than 4 and the rows are few: one warp would ask for them in several turns.  (A block of 256 threads a row took 20 us for 1,344 rows of 3 parts, 4 of it
+// necessary: bound by the blocks' starts and barriers.)
+constexpr int kMergeThreads = 128;
 
-template <typename T>
+template <typename T, int SHARE>
 __global__ void __launch_bounds__(kMergeThreads)
-attention_rows_merge_kernel(Partials parts, T* __restrict__ out, int out_stride, int value_dim, const float* __restrict__ sink) {
-  __shared__ float sh_acc[kMergeThreads][4];
-  __shared__ float sh_l[kMergeThreads];
-  __shared__ float sh_max[kMergeThreads / 32];
+attention_rows_merge_kernel(Partials parts, T* __restrict__ out, int out_stride, int num_rows, int num_heads, int value_dim, const float* __restrict__ sink) {
+  constexpr int ROWS = kMergeThreads / 32 / SHARE, PASSES = kRowsMostDim / 128;
+  __shared__ float sh_acc[SHARE][PASSES * 128 + 4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % SHARE;
+  const int row = blockIdx.x * ROWS + warp / SHARE;
   grid_dependency_release();
+  if (SHARE == 1 && row >= num_rows) return;
+  int across = 1;  // lanes that a part's row takes
+  while (across < 32 && across * 4 < value_dim) across *= 2;
+  const int groups = 32 / across, mine = lane / across, column = lane % across * 4;
+  const bool whole = value_dim % 4 == 0;
+  const size_t part0 = (size_t)row * parts.splits;
   grid_dependency_wait();
-  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const size_t row0 = ((size_t)token * gridDim.y + head) * parts.splits;
-  const int per_row = (value_dim + 3) / 4, groups = kMergeThreads / per_row;  // up to 64 threads, at least 4 groups
-  const int mine = threadIdx.x / per_row, column = threadIdx.x % per_row * 4;
-  float m_all = -INFINITY;
-  for (int s = threadIdx.x; s < parts.splits; s += kMergeThreads) m_all = fmaxf(m_all, __ldcg(parts.ml + (row0 + s) * 2));
+  // A part without a key has a sum of 0, one whose scores are all NaN a sum of NaN; both have no maximum.
+  float m_mine = lane < parts.splits ? __ldcg(parts.ml + (part0 + lane) * 2) : -INFINITY, l_mine = lane < parts.splits ? __ldcg(parts.ml + (part0 + lane) * 2 + 1) : 0.f;
+  float m_all = m_mine;
+  for (int s = lane + 32; s < parts.splits; s += 32) m_all = fmaxf(m_all, __ldcg(parts.ml + (part0 + s) * 2));
   m_all = warp_max(m_all);
-  if (lane == 0) sh_max[warp] = m_all;
-  __syncthreads();
+  float l_all = 0.f, acc[PASSES][4] = {};
+  for (int base = 0; base < parts.splits; base += 32) {
+    if (base > 0) {
+      m_mine = lane < parts.splits - base ? __ldcg(parts.ml + (part0 + base + lane) * 2) : -INFINITY;
+      l_mine = lane < parts.splits - base ? __ldcg(parts.ml + (part0 + base + lane) * 2 + 1) : 0.f;
+    }
+    const float weight = m_mine == -INFINITY ? l_mine : exp2f(m_mine - m_all);
+    l_all += l_mine * weight;
+    const int n = min(32, parts.splits - base);
+    for (int first = share * groups; first < n; first += groups * SHARE * 4) {  // four turns' loads together
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 32; ++w) m_all = fmaxf(m_all, sh_max[w]);
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, l_mine = 0.f;
-  if (mine < groups) {
-#pragma unroll 4
-    for (int s = mine; s < parts.splits; s += groups) {
-      const float m = __ldcg(parts.ml + (row0 + s) * 2), l = __ldcg(parts.ml + (row0 + s) * 2 + 1);
-      // (a part without a key has a sum of 0, one whose scores are all NaN a sum of NaN; both have no maximum)
-      const float weight = m == -INFINITY ? l : exp2f(m - m_all);
-      l_mine += l * weight;
+      for (int pass = 0; pass < PASSES; ++pass) {
+        const int e = column + pass * 128;
+        if (pass > 0 && pass * 128 >= value_dim) continue;
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = min(first + u * groups * SHARE + mine, n - 1);
+          const float* from = parts.o + (part0 + base + i) * value_dim;
+          if (whole) {
+            v[u] = __ldcg(reinterpret_cast<const float4*>(from + min(e, value_dim - 4)));
+          } else {
+            v[u].x = __ldcg(from + min(e, value_dim - 1));
+            v[u].y = __ldcg(from + min(e + 1, value_dim - 1));
+            v[u].z = __ldcg(from + min(e + 2, value_dim - 1));
+            v[u].w = __ldcg(from + min(e + 3, value_dim - 1));
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = first + u * groups * SHARE + mine;
+          const float w = __shfl_sync(0xffffffffu, weight, min(i, 31));
+          if (i < n) {
+            acc[pass][0] += v[u].x * w; acc[pass][1] += v[u].y * w; acc[pass][2] += v[u].z * w; acc[pass][3] += v[u].w * w;
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) {
+    l_all += __shfl_xor_sync(0xffffffffu, l_all, d);
+    if (d >= across)
+#pragma unroll
+      for (int pass = 0; pass < PASSES; ++pass)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[pass][e] += __shfl_xor_sync(0xffffffffu, acc[pass][e], d);
+  }
+  if (SHARE > 1) {
+    if (mine == 0)
+#pragma unroll
+      for (int pass = 0; pass < PASSES; ++pass)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sh_acc[share][pass * 128 + column + e] = acc[pass][e];
+    __syncthreads();
+    if (share != 0) return;
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (column + e < value_dim) acc[e] += __ldcg(parts.o + (row0 + s) * value_dim + column + e) * weight;
-    }
+        for (int w = 1; w < SHARE; ++w) acc[pass][e] += sh_acc[w][pass * 128 + column + e];
   }
+  if (mine != 0) return;
+  const int token = row / num_heads, head = row % num_heads;
+  const float inv = sink ? sink_inverse_log2(m_all, l_all, sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) sh_acc[threadIdx.x][e] = acc[e];
-  if (column == 0) sh_l[mine] = l_mine;
-  __syncthreads();
-  if (threadIdx.x < per_row) {
-    float l_all = 0.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int r = 0; r < groups; ++r) {
-      l_all += sh_l[r];
+  for (int pass = 0; pass < PASSES; ++pass)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += sh_acc[r * per_row + threadIdx.x][e];
+    for (int e = 0; e < 4; ++e) {
+      const int at = pass * 128 + column + e;
+      if (at < value_dim) out[(size_t)token * out_stride + (size_t)head * value_dim + at] = from_float<T>(acc[pass][e] * inv);
     }
-    const float inv = sink ? sink_inverse_log2(m_all, l_all, sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (column + e < value_dim) out[(size_t)token * out_stride + (size_t)head * value_dim + column + e] = from_float<T>(sum[e] * inv);
-  }
 }
 
 template <typename T>
 static int rows_merge(const Partials& parts, void* out, int out_stride, int tokens, int num_heads, int value_dim, const float* sink,
                       cudaStream_t stream) {
-  return (int)launch_dependent(attention_rows_merge_kernel<T>, dim3(tokens, num_heads), dim3(kMergeThreads), 0, stream, parts, (T*)out, out_stride,
-                               value_dim, sink);
+  const int rows = tokens * num_heads;
+  if (parts.splits > 16 || (parts.splits > 4 && rows <= 512))
+    return (int)launch_dependent(attention_rows_merge_kernel<T, 4>, dim3(rows), dim3(kMergeThreads), 0, stream, parts, (T*)out, out_stride, rows,
+                                 num_heads, value_dim, sink);
+  return (int)launch_dependent(attention_rows_merge_kernel<T, 1>, dim3((rows + 3) / 4), dim3(kMergeThreads), 0, stream, parts, (T*)out, out_stride, rows,
+                               num_heads, value_dim, sink);
 }
 
 int rows_merge_bf16(const Partials& parts, void* out, int out_stride, int tokens, int num_heads, int value_dim, const float* sink,

@@ -7,7 +7,8 @@ the cache as it is (csrc/attention_rows.cu).  :class:`~distie_b200.kernels.devic
 here when the slot is in eight bits or the step's places are not its positions.
 """
 
-from __future__ import annotations
+from __future__ import functools
+import annotations
 
 import ctypes
 
@@ -24,6 +25,7 @@ def _ptr(x) -> int:
     return x.data_ptr() if x is not None else 0
 
 
+@functools.lru_cache(maxsize=256)
 def tree_splits(tiles: int, blocks: int, sms: int) -> int:
     """Shares that the keys of ``tiles`` tiles of rows, ``blocks`` blocks of 128 keys each, are cut into
     (attention_tree_tcgen05.cu): the number for which whole waves of CTAs take the least time, a CTA the time of its blocks
@@ -36,16 +38,22 @@ def tree_splits(tiles: int, blocks: int, sms: int) -> int:
     return best
 
 
-def decode_splits(blocks: int, keys: int, sms: int) -> int:
-    """Shares that the keys of ``blocks`` (token, group of heads) pairs are cut into (attention_decode_e4m3.cu): the number for
-    which the fullest SM takes the least time, three CTAs or fewer that of three (a CTA alone does not keep an SM busy), and a
-    CTA that of its keys and of 192 more for its start and end.  Up to 8 shares are joined inside the kernel, by a cluster of
-    CTAs; up to 12 are not worth a second kernel."""
+@functools.lru_cache(maxsize=256)
+def decode_splits(blocks: int, keys: int, sms: int, wide: bool, many: bool) -> int:
+    """Shares that the keys of ``blocks`` (token, group of heads) pairs are cut into (attention_decode_e4m3.cu): the number that
+    takes the least time, counted in keys of a CTA that has an SM to itself.  An SM holds four CTAs of heads of 64 and three of
+    128 (``wide``), one fewer with more than 8 heads each (``many``).  Two take 1.07 times as long as one, three 1.5 times (narrow
+    heads 1.07), four 1.45; a CTA's start and end are 700 keys, joining up to 8 shares by a cluster of CTAs another 240, more
+    than 8 by a second kernel 800.  (28 heads of 128 over 4,099 keys of 48 requests, 4 key heads: 57, 48, 56 and 52 us with 1 to 4
+    shares; 1,024 keys of 64 requests: 23, 31, 30, 33.)"""
+    slots = (3 if wide else 4) - many
+    slower = (0.0, 1.0, 1.07, 1.5 if wide else 1.07, 1.45)
     best, least = 1, None
     for splits in range(1, max(1, min(keys // 256, 64)) + 1):
-        if 8 < splits <= 12:
-            continue
-        cost = max(3, -(-blocks * splits // sms)) * (-(-keys // splits) + 192)
+        waves, rest = divmod(blocks * splits, slots * sms)
+        each = -(-keys // splits)
+        cost = waves * (each * slower[slots] + 700) + (each * slower[-(-rest // sms)] + 700 if rest else 0)
+        cost += 0 if splits == 1 else 240 if splits <= 8 else 800
         if least is None or cost < least:
             best, least = splits, cost
     return best
@@ -245,7 +253,7 @@ class CachedRows:
             return False
         blocks = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 16)
         seen = min(step.max_kv_len, window or chunk or step.max_kv_len)
-        splits = decode_splits(blocks, seen, self.sm_count)
+        splits = decode_splits(blocks, seen, self.sm_count, head_dim == 128, num_heads // num_kv_heads > 8)
         scratch = None
         if splits > 8:
             floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, head_dim, splits)
