@@ -7,10 +7,10 @@ the cache as it is (csrc/attention_rows.cu).  :class:`~distie_b200.kernels.devic
 here when the slot is in eight bits or the step's places are not its positions.
 """
 
-from __future__ import functools
-import annotations
+from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
