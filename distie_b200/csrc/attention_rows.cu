@@ -30,6 +30,7 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   __shared__ float p_s[kRowsKeys][kRowsTile + 4];   // weights, a key's rows side by side
   __shared__ float corr_s[kRowsTile], m_s[kRowsTile], l_s[kRowsTile];
   __shared__ int bad_s;                             // a value of this tile is not finite
+  __shared__ int first_s[kRowsTile];                // a row's oldest visible key
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.y, split = blockIdx.z;
   const Request request = request_of(rows, b);
@@ -51,12 +52,14 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   if (threadIdx.x < kRowsTile) {
     m_s[threadIdx.x] = -INFINITY;
     l_s[threadIdx.x] = 0.f;
+    const int token = request.first + (row0 + min((int)threadIdx.x, count - 1)) / rows.group;
+    first_s[threadIdx.x] = first_visible_key(rows.positions[token], rows.window, rows.chunk);
   }
+  __syncthreads();
   // The oldest cached key that any row of the tile sees inside its window (all new tokens' keys are walked); the keys
   // before it are walked up to keep_first only.
   int oldest = request.past;
-  for (int r = 0; r < count; ++r)
-    oldest = min(oldest, first_visible_key(rows.positions[request.first + (row0 + r) / rows.group], rows.window, rows.chunk));
+  for (int r = 0; r < count; ++r) oldest = min(oldest, first_s[r]);
   const int keys = request.past + request.nodes;
   const int kept = min(rows.keep_first, oldest);
   // Tiles of keys: those of the kept first keys, then those from the oldest one on; the splits share them out.
@@ -77,26 +80,54 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
     __syncthreads();  // the tile before this one is done with
     if (threadIdx.x == 0) bad_s = 0;
     __syncthreads();
-    for (int r = warp; r < kRowsKeys; r += kRowsThreads / 32) {
-      const int key = key0 + r;
-      long long at = -1;
-      if (key < key_end && (key >= oldest || key < kept)) {
-        at = cache.row_of(table, key, kv_head);
-        if (at < 0 && lane == 0 && error) atomicExch(error, rows.seqs ? 8 : 4);
-      }
-      const float ks = CACHE == DISTIE_E4M3 && at >= 0 ? cache.k_scale[at] : 1.f, vs = CACHE == DISTIE_E4M3 && at >= 0 ? cache.v_scale[at] : 1.f;
-      for (int e = lane; e < dim; e += 32) k_s[r * (dim + 1) + e] = at >= 0 ? cached_value<CACHE>(cache.k, (size_t)at * dim + e) * ks : 0.f;
-      bool bad = false;
-      for (int e = lane; e < vdim; e += 32) {
-        const float x = at >= 0 ? cached_value<CACHE>(cache.v, (size_t)at * vdim + e) * vs : 0.f;
-        bad |= !(fabsf(x) <= 3.402823466e38f);
-        v_s[r * vdim + e] = x;
-      }
-      if (bad) bad_s = 1;
+    // Lane r of every warp finds key r's row; a warp then takes 8 rows, all their loads together (of no row: the cache's first,
+    // not used).
+    const int key = key0 + lane;
+    long long at = -1;
+    if (key < key_end && (key >= oldest || key < kept)) {
+      at = cache.row_of(table, key, kv_head);
+      if (at < 0 && warp == 0 && error) atomicExch(error, rows.seqs ? 8 : 4);
     }
+    int key_position = key;
+    if (rows.seqs && key >= request.past && key < keys) key_position = rows.positions[request.first + key - request.past];
+    float k_scale = 1.f, v_scale = 1.f;
+    if (CACHE == DISTIE_E4M3) {
+      k_scale = cache.k_scale[max(at, 0ll)];
+      v_scale = cache.v_scale[max(at, 0ll)];
+    }
+    constexpr int MINE = kRowsKeys / (kRowsThreads / 32);
+    const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+    long long from[MINE];
+    float ks[MINE], vs[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      from[i] = max(__shfl_sync(0xffffffffu, at, warp * MINE + i), 0ll);
+      ks[i] = __shfl_sync(0xffffffffu, k_scale, warp * MINE + i);
+      vs[i] = __shfl_sync(0xffffffffu, v_scale, warp * MINE + i);
+    }
+    bool bad = false;
+    for (int e = lane; e < max(dim, vdim); e += 32) {
+      float kx[MINE], vx[MINE];
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        kx[i] = cached_value<CACHE>(cache.k, (size_t)from[i] * dim + min(e, dim - 1));
+        vx[i] = cached_value<CACHE>(cache.v, (size_t)from[i] * vdim + min(e, vdim - 1));
+      }
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int r = warp * MINE + i;
+        const bool live = (there >> r) & 1;
+        if (e < dim) k_s[r * (dim + 1) + e] = live ? kx[i] * ks[i] : 0.f;
+        if (e < vdim) {
+          const float x = live ? vx[i] * vs[i] : 0.f;
+          bad |= !(fabsf(x) <= 3.402823466e38f);
+          v_s[r * vdim + e] = x;
+        }
+      }
+    }
+    if (bad) bad_s = 1;
     __syncthreads();
     {  // scores: key `lane`, rows 4 warp .. 4 warp + 3; then their softmax statistics over the warp
-      const int key = key0 + lane;
       float dot[4] = {0.f, 0.f, 0.f, 0.f};
       const float* k_row = k_s + lane * (dim + 1);
       const float* q_row = q_s + warp * 4 * dim;
@@ -108,17 +139,8 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int r = warp * 4 + u;
-        bool seen = r < count && key < key_end;
-        if (seen) {
-          const int token = request.first + (row0 + r) / rows.group;
-          const int first = first_visible_key(rows.positions[token], rows.window, rows.chunk);
-          int key_position = key;
-          if (key >= request.past) {
-            seen = mask_bit(rows, token, key - request.past);
-            key_position = rows.positions[request.first + key - request.past];
-          }
-          seen = seen && (key_position >= first || key_position < rows.keep_first) && cache.row_of(table, key, kv_head) >= 0;
-        }
+        bool seen = r < count && at >= 0 && (key_position >= first_s[r] || key_position < rows.keep_first);
+        if (seen && key >= request.past) seen = mask_bit(rows, request.first + (row0 + r) / rows.group, key - request.past);
         const float x = seen ? score_log2(dot[u], rows) : -INFINITY;
         const float m_old = m_s[r];
         const float m_new = fmaxf(m_old, warp_max(x));
