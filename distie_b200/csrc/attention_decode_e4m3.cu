@@ -5,7 +5,7 @@
 // with n the e4m3 numbers of a row and s its scale.  Decoding reads every cached row once, here half the bytes of a 16-bit
 // cache, so the instructions between the bytes and the products are what there is to save:
 //
-//   grid   (token, kv head * chunks of up to 16 query heads, split)
+//   grid   (token, kv head * chunks of up to 16 query heads, split); how many splits: decode_splits in kernels/cached.py
 //   block  4 warps; a warp takes groups of 32 keys of the split in turn, through a ring of its own in shared memory (cp.async)
 //   S^T    16 keys are the rows of mma.m16n8k16, up to 8 (or 2 x 8) heads the columns, head_dim the reduction
 //   O^T    16 dims are the rows, the heads the columns, 16 keys the reduction
@@ -20,8 +20,15 @@
 // in float16, in units of a running maximum m' of its own beside the softmax's m: p_j (s^v_j 2^(m - m')), however the scales
 // differ at most a few, and off by at most 2^-11 of itself (or of 2^-14).  Both maxima are whole numbers (what they scale,
 // they scale exactly) and are not searched for in every group, only in a head's first and where weights outgrow the ones in
-// use: no shuffles and no correction of O in most groups.  Sums and maxima are float32.  The warps, and with several splits the CTAs, are merged in the
-// softmax's units: inside the cluster up to 8 splits, by a second kernel beyond.
+// use: no shuffles and no correction of O in most groups.  Sums and maxima are float32.  The warps, and with several splits the
+// CTAs, are merged in the softmax's units: inside the cluster up to 8 splits, where every CTA sends its sums to the one that puts
+// them together (no CTA reads another's memory, none waits to leave), by a second kernel beyond.
+//
+// What bounds it: with many keys the bytes (13 requests of 30,011 keys, 8 key heads of 128: 824 MB in 130 us, 6.3 TB/s; 48 of
+// 4,099, 8 key heads of 64: 214 MB in 45 us inside the kernel, where a CTA's rounds of four groups take 1,600 cycles however
+// many of them an SM holds up to two).  With few keys a CTA's start (positions, seat, page ids, then q and the first rows: 5,000
+// cycles) and end (merge 1,200, cluster 3,500).  What was tried and took as long or longer: rings of 3, 4 and 6 groups and
+// CTAs of 8 warps (fewer CTAs fit an SM), boxes of 16 rows by the copy engine in place of cp.async.
 #include <cuda_fp16.h>
 
 #include "cached_rows.cuh"
@@ -31,6 +38,7 @@ namespace distie {
 
 constexpr int kDecWarps = 4;
 constexpr int kDecKeys = 32;      // keys of a group
+constexpr int kDecStages = 2;     // groups of a warp's ring
 constexpr int kDecPages = 992;    // page ids of a split that are kept in shared memory (so many, that three CTAs fit an SM)
 constexpr int kDecClusterSplits = 8;
 constexpr float kDecMostSum = 1073741824.f, kDecMostWeight = 16384.f;  // of a lane's four weights of a head
@@ -99,7 +107,7 @@ __device__ __forceinline__ uint32_t dec_offset(int row, int piece) {  // of a 16
 }
 
 // PAGE16: the page size is a power of two from 16 on, so 16 keys from a multiple of 16 on lie in one page.
-template <int D, int STAGES, int NH, bool PAGE16>
+template <int D, int NH, bool PAGE16>
 __global__ void __launch_bounds__(kDecWarps * 32, NH == 1 ? 3 : 2)
 attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, __nv_bfloat16* __restrict__ out, int out_stride, QueryRows rows,
                              CachePages cache, Partials parts, int head_chunks, int cluster_merge, int* __restrict__ error) {
@@ -145,7 +153,7 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
     if (i >= 0 && i < min(share, kDecPages)) return sh_pages[i];
     return column < cache.table_width ? table[column] : -1;
   };
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(dyn) + (uint32_t)warp * STAGES * STAGE;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(dyn) + (uint32_t)warp * kDecStages * STAGE;
   const int row0 = lane / MT, piece = lane % MT;
   const uint8_t* k_numbers = reinterpret_cast<const uint8_t*>(cache.k);
   const uint8_t* v_numbers = reinterpret_cast<const uint8_t*>(cache.v);
@@ -215,7 +223,7 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
     for (int ks = 0; ks < MT; ++ks)
       q_raw[nh][ks] = __ldcg(reinterpret_cast<const uint2*>(q + (size_t)t * q_stride + (size_t)(head0 + min(nh * 8 + g, heads_here - 1)) * D + 16 * ks + 4 * c));
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) issue(warp + s * kDecWarps, s);
+  for (int s = 0; s < kDecStages - 1; ++s) issue(warp + s * kDecWarps, s);
 
   // B fragments of S^T: head g of a column tile, dims 16 ks + 4 c .. + 3, times the head's power of two.
   uint32_t qb[NH][MT][2];
@@ -266,12 +274,12 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
     const bool in_window = grp < window_groups;
     const int base = in_window ? lo16 + grp * kDecKeys : (grp - window_groups) * kDecKeys;
     const int lo_key = in_window ? lo : 0, hi_key = in_window ? hi : kept - 1;
-    issue(grp + (STAGES - 1) * kDecWarps, (stage + STAGES - 1) % STAGES);  // an empty group past the end
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    issue(grp + (kDecStages - 1) * kDecWarps, (stage + kDecStages - 1) % kDecStages);  // an empty group past the end
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDecStages - 1) : "memory");
     __syncwarp();
     const uint32_t k_tile = ring + (uint32_t)stage * STAGE, v_tile = k_tile + TILE;
-    const float* scales = reinterpret_cast<const float*>(dyn + (size_t)warp * STAGES * STAGE + (size_t)stage * STAGE + 2 * TILE);
-    stage = (stage + 1) % STAGES;
+    const float* scales = reinterpret_cast<const float*>(dyn + (size_t)warp * kDecStages * STAGE + (size_t)stage * STAGE + 2 * TILE);
+    stage = (stage + 1) % kDecStages;
 
     // ---- S^T: rows = keys 16 sub + g (+ 8), columns = heads 2 c, 2 c + 1 -------------------------------------------
     float st[kDecKeys / 16][NH][4];
@@ -362,6 +370,7 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
               o[nh][mt][e + 2] *= corr;
             }
           }
+          __syncwarp();
         }
         bool outgrown = false;
 #pragma unroll
@@ -504,13 +513,13 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
   }
 }
 
-template <int D, int STAGES, int NH, bool PAGE16>
+template <int D, int NH, bool PAGE16>
 static cudaError_t launch_decode(const dim3& grid, const __nv_bfloat16* q, int q_stride, __nv_bfloat16* out, int out_stride, const QueryRows& rows,
                                  const CachePages& cache, const Partials& parts, int head_chunks, int cluster_merge, int* error, cudaStream_t stream) {
-  constexpr size_t ring = (size_t)kDecWarps * STAGES * (2 * kDecKeys * D + 2 * kDecKeys * 4);
+  constexpr size_t ring = (size_t)kDecWarps * kDecStages * (2 * kDecKeys * D + 2 * kDecKeys * 4);
   constexpr size_t merge = (size_t)kDecWarps * NH * 8 * (D + 8) * sizeof(float);
   constexpr size_t shared = ring > merge ? ring : merge;
-  auto kernel = attention_decode_e4m3_kernel<D, STAGES, NH, PAGE16>;
+  auto kernel = attention_decode_e4m3_kernel<D, NH, PAGE16>;
   if (shared > 48 * 1024) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
     if (err != cudaSuccess) return err;
@@ -568,9 +577,9 @@ extern "C" int distie_attention_decode_e4m3(const void* q, int q_stride, void* o
   const bool page16 = cache.page_shift >= 4;
   cudaError_t err;
 #define DISTIE_DECODE_E4M3(D, NH)                                                                                                       \
-  err = page16 ? launch_decode<D, 2, NH, true>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts,   \
+  err = page16 ? launch_decode<D, NH, true>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts,   \
                                                chunks, cluster_merge, error, stream)                                                     \
-               : launch_decode<D, 2, NH, false>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts,  \
+               : launch_decode<D, NH, false>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts,  \
                                                 chunks, cluster_merge, error, stream)
   if (head_dim == 64) {
     if (group <= 8) DISTIE_DECODE_E4M3(64, 1); else DISTIE_DECODE_E4M3(64, 2);

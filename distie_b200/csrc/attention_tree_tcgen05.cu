@@ -22,11 +22,17 @@
 //
 // Masks: a block that lies before every row's new tokens and inside every row's window needs none; the others get 64 bits a
 // row and group.  A masked weight is 0, and 0 * (what is not finite) is not 0: in blocks that need masks, values that are not
-// finite are stored as zeros, and the rows that see them get them back at the end, element by element (8-bit rows carry
-// NaN in their scales, which masks reach).  Rows of keys that belong to nobody are zeros.
+// finite (of an 8-bit cache: scales) are stored as zeros, and the rows that see them get them back at the end, element by
+// element.  Rows of keys that belong to nobody are zeros.
 //
 // Running maxima are not searched for in every block, only in a row's first and where its weights outgrow the one in use;
-// then O is read, scaled and written back.
+// then O, and what P of the block is there already, are read, scaled and written back.  The maxima are whole numbers, so that
+// scaling is exact.
+//
+// What bounds it: the softmax warps.  Two trees of 64 new tokens over 16,001 keys (40 heads of 128, 8 key heads, bfloat16): 72 us
+// with the joining kernel, 144 CTAs of 44 blocks at 2,400 cycles a block, of which the products take 1,050 and each
+// scheduler's 128 exponentials 1,024; over an 8-bit cache 103 us, 3,500 cycles a block (scales read and multiplied, weights summed
+// once more for their limit).  Registers decide: 15 warps have 128 each, and a version that keeps 64 scores a thread spills.
 // With several shares of the keys, the parts go to scratch in float32 and attention_rows.cu joins them.
 //
 //   warps 0..7    softmax, end        warp 8   tensor memory, MMA issue        warps 9, 10   copies        warps 11..14   unpacking
@@ -213,7 +219,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                               CachePages cache, Partials parts, int* __restrict__ error) {
   extern __shared__ unsigned char raw_shared[];
   auto& sm = *reinterpret_cast<TreeShared<D>*>((reinterpret_cast<uintptr_t>(raw_shared) + 1023) & ~uintptr_t(1023));
-  constexpr uint32_t TMEM_COLS = D == 128 ? 512 : 512, O_COL = 256;  // S0 | S1 | O of group 0 | O of group 1
+  constexpr uint32_t TMEM_COLS = 512, O_COL = 256;  // S0 | S1 | O of group 0 | O of group 1
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile uint32_t* failed = &sm.failed;
 
@@ -701,6 +707,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                   tmem_store_16(s_addr, packed);
                 }
               }
+              __syncwarp();
             }
             // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0)
             const float units = E4M3 && o_used != -INFINITY ? exp2_approx(fminf(shift - o_used, 126.f)) : 0.f;

@@ -69,30 +69,30 @@ class CachedRows:
         return kv is not None and (kv.k_scale is not None or step.slots is not None)
 
     def _check_slot(self, what: str, kv, num_kv_heads: int, key_dim: int, value_dim: int) -> int:
-        """The slot's element type code, after a look at what the kernels take for granted.  A slot is handed to every step of a
-        request's life: the look is taken once for its tensors and sizes."""
-        seen = kv.__dict__.get("_seen")
-        if seen is not None and seen[0] is kv.k and seen[1] is kv.v and seen[2] is kv.block_table and seen[3] is kv.k_scale \
-                and seen[4] is kv.v_scale and seen[5] == (kv.num_pages, kv.page_size, num_kv_heads, key_dim, value_dim, self.dtype):
-            return seen[6]
-        if kv.k.dtype != kv.v.dtype or (kv.k.dtype != self.dtype and kv.k.dtype != E4M3):
-            raise KernelError(f"{what}: a cache of {self.dtype} or {E4M3} is expected, not of {kv.k.dtype}")
+        """The slot's element type code, after a look at what the kernels take for granted."""
+        k, v, table, scales, device = kv.k, kv.v, kv.block_table, (kv.k_scale, kv.v_scale), self.error_flag.device
+        if k.dtype != v.dtype or (k.dtype != self.dtype and k.dtype != E4M3):
+            raise KernelError(f"{what}: a cache of {self.dtype} or {E4M3} is expected, not of {k.dtype}")
         rows = (kv.num_pages, num_kv_heads, kv.page_size)
-        if tuple(kv.k.shape) != (*rows, key_dim) or tuple(kv.v.shape) != (*rows, value_dim):
+        if k.shape != (*rows, key_dim) or v.shape != (*rows, value_dim):
             raise KernelError(f"{what}: keys {(*rows, key_dim)} and values {(*rows, value_dim)} are expected, not "
-                              f"{tuple(kv.k.shape)} and {tuple(kv.v.shape)}")
-        if not kv.k.is_contiguous() or not kv.v.is_contiguous() or kv.block_table.dtype != torch.int32 or kv.block_table.stride(-1) != 1 \
-                or kv.block_table.stride(0) != kv.block_table.shape[-1]:
+                              f"{tuple(k.shape)} and {tuple(v.shape)}")
+        if not (k.is_contiguous() and v.is_contiguous() and table.is_contiguous()) or table.dtype != torch.int32 or table.dim() != 2:
             raise KernelError(f"{what}: contiguous pages and a contiguous int32 block table are expected")
-        if (kv.k.dtype == E4M3) != (kv.k_scale is not None) or (kv.k_scale is None) != (kv.v_scale is None):
+        if (k.dtype == E4M3) != (scales[0] is not None) or (scales[0] is None) != (scales[1] is None):
             raise KernelError(f"{what}: a cache in eight bits comes with the scales of its rows, and only such a cache")
-        for scale in (kv.k_scale, kv.v_scale):
-            if scale is not None and (scale.dtype != torch.float32 or tuple(scale.shape) != rows or not scale.is_contiguous()):
-                raise KernelError(f"{what}: contiguous float32 scales {rows} are expected")
-        code = _CACHE_CODE[kv.k.dtype]
-        kv.__dict__["_seen"] = (kv.k, kv.v, kv.block_table, kv.k_scale, kv.v_scale,
-                                (kv.num_pages, kv.page_size, num_kv_heads, key_dim, value_dim, self.dtype), code)
-        return code
+        if k.device != device or v.device != device or table.device != device:
+            raise KernelError(f"{what}: a cache on {device} is expected")
+        for scale in scales:
+            if scale is not None and (scale.dtype != torch.float32 or scale.shape != rows or not scale.is_contiguous() or scale.device != device):
+                raise KernelError(f"{what}: contiguous float32 scales {rows} on {device} are expected")
+        return _CACHE_CODE[k.dtype]
+
+    def _check_slots(self, what: str, step) -> None:
+        slots = step.slots
+        if slots is not None and (slots.dtype != torch.int32 or slots.numel() < step.num_tokens or not slots.is_contiguous()
+                                  or slots.device != self.error_flag.device):
+            raise KernelError(f"{what}: an int32 place in the cache for each of {step.num_tokens} tokens is expected")
 
     # -- write ----------------------------------------------------------------------------------------------------
     def _rows_write(self, what, rows, bias, step, kv, rotary, num_heads, num_kv_heads, head_dim, value_dim, q_out, norm=(0, 0.0, None, None),
@@ -100,14 +100,16 @@ class CachedRows:
         """``rows``: (element type code, slices, elements between slices, then pointer and row stride of q, of k and of v; a null q:
         no queries, a null v: the values are the keys as projected); ``bias``: three pointers."""
         cache_code = self._check_slot(what, kv, num_kv_heads, head_dim, value_dim)
+        self._check_slots(what, step)
         if rotary is not None and (rotary.rotary_dim > head_dim or rotary.rotary_dim % 2 or rotary.inv_freq.dtype != torch.float32
                                    or rotary.inv_freq.numel() * 2 < rotary.rotary_dim):
             raise KernelError(f"{what}: a rotary table of float32 frequencies for an even number of a head's elements is expected")
         for vector in norm[2:]:
             if vector is not None and (vector.dtype != torch.float32 or vector.shape != (head_dim,) or vector.stride(0) != 1):
                 raise KernelError(f"{what}: float32 weights of {head_dim} elements are expected")
-        if q_out is not None and (q_out.dtype != self.dtype or q_out.stride(-1) != 1):
-            raise KernelError(f"{what}: q goes to rows of {self.dtype}")
+        if q_out is not None and (q_out.dtype != self.dtype or q_out.stride(-1) != 1 or q_out.shape[-1] < num_heads * head_dim
+                                  or q_out.shape[-2] < step.num_tokens):
+            raise KernelError(f"{what}: q goes to {step.num_tokens} rows of {num_heads * head_dim} elements of {self.dtype}")
         coef, every = (float(q_temp[0]), float(q_temp[1])) if q_temp else (0.0, 0.0)
         code, splits, split_stride, q, q_stride, k, k_stride, v, v_stride = rows
         with self._here():
@@ -209,13 +211,18 @@ class CachedRows:
         tree = step.tree
         cache_code = self._check_slot("attention", kv, num_kv_heads, head_dim, kv.v.shape[-1])
         value_dim, most = kv.v.shape[-1], 1
-        if q.dtype != self.dtype or out.dtype != self.dtype or q.stride(-1) != 1 or out.stride(-1) != 1:
-            raise KernelError(f"attention: queries and output of {self.dtype} with unit column stride are expected")
+        if q.dtype != self.dtype or out.dtype != self.dtype or q.stride(-1) != 1 or out.stride(-1) != 1 \
+                or q.shape[0] < tokens or q.shape[-1] < num_heads * head_dim or out.shape[0] < tokens or out.shape[-1] < num_heads * value_dim:
+            raise KernelError(f"attention: queries and output of {self.dtype} with unit column stride, {num_heads} heads for each of "
+                              f"{tokens} tokens, are expected")
+        if tokens == 0:
+            return
         if tree is not None:
             most = int(tree.most_nodes)
             if not 1 <= most <= MOST_DRAFTED or tree.bits.dtype != torch.int32 or tree.seqs.dtype != torch.int32 \
                     or tree.bits.shape[0] < tokens or not most <= 32 * tree.bits.shape[1] <= MOST_DRAFTED or not tree.bits.is_contiguous() \
-                    or tuple(tree.seqs.shape) != (requests, 3) or not tree.seqs.is_contiguous():
+                    or tuple(tree.seqs.shape) != (requests, 3) or not tree.seqs.is_contiguous() \
+                    or tree.bits.device != self.error_flag.device or tree.seqs.device != self.error_flag.device:
                 raise KernelError(f"attention: a tree of 1 to {MOST_DRAFTED} new tokens a request with int32 masks [tokens, words] and "
                                   f"rows [{requests}, 3] is expected")
         group = num_heads // num_kv_heads
