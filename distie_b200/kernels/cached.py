@@ -70,23 +70,24 @@ class CachedRows:
 
     def _check_slot(self, what: str, kv, num_kv_heads: int, key_dim: int, value_dim: int) -> int:
         """The slot's element type code, after a look at what the kernels take for granted."""
-        k, v, table, scales, device = kv.k, kv.v, kv.block_table, (kv.k_scale, kv.v_scale), self.error_flag.device
-        if k.dtype != v.dtype or (k.dtype != self.dtype and k.dtype != E4M3):
-            raise KernelError(f"{what}: a cache of {self.dtype} or {E4M3} is expected, not of {k.dtype}")
-        rows = (kv.num_pages, num_kv_heads, kv.page_size)
+        k, v, table, k_scale, v_scale, device = kv.k, kv.v, kv.block_table, kv.k_scale, kv.v_scale, self.error_flag.device
+        dtype, rows = k.dtype, (kv.num_pages, num_kv_heads, kv.page_size)
+        if dtype != v.dtype or (dtype != self.dtype and dtype != E4M3):
+            raise KernelError(f"{what}: a cache of {self.dtype} or {E4M3} is expected, not of {dtype}")
         if k.shape != (*rows, key_dim) or v.shape != (*rows, value_dim):
             raise KernelError(f"{what}: keys {(*rows, key_dim)} and values {(*rows, value_dim)} are expected, not "
                               f"{tuple(k.shape)} and {tuple(v.shape)}")
         if not (k.is_contiguous() and v.is_contiguous() and table.is_contiguous()) or table.dtype != torch.int32 or table.dim() != 2:
             raise KernelError(f"{what}: contiguous pages and a contiguous int32 block table are expected")
-        if (k.dtype == E4M3) != (scales[0] is not None) or (scales[0] is None) != (scales[1] is None):
+        if (dtype == E4M3) != (k_scale is not None) or (k_scale is None) != (v_scale is None):
             raise KernelError(f"{what}: a cache in eight bits comes with the scales of its rows, and only such a cache")
         if k.device != device or v.device != device or table.device != device:
             raise KernelError(f"{what}: a cache on {device} is expected")
-        for scale in scales:
-            if scale is not None and (scale.dtype != torch.float32 or scale.shape != rows or not scale.is_contiguous() or scale.device != device):
-                raise KernelError(f"{what}: contiguous float32 scales {rows} on {device} are expected")
-        return _CACHE_CODE[k.dtype]
+        if k_scale is not None and not (
+                k_scale.dtype == v_scale.dtype == torch.float32 and k_scale.shape == rows and v_scale.shape == rows
+                and k_scale.is_contiguous() and v_scale.is_contiguous() and k_scale.device == device and v_scale.device == device):
+            raise KernelError(f"{what}: contiguous float32 scales {rows} on {device} are expected")
+        return _CACHE_CODE[dtype]
 
     def _check_slots(self, what: str, step) -> None:
         slots = step.slots
@@ -100,28 +101,37 @@ class CachedRows:
         """``rows``: (element type code, slices, elements between slices, then pointer and row stride of q, of k and of v; a null q:
         no queries, a null v: the values are the keys as projected); ``bias``: three pointers."""
         cache_code = self._check_slot(what, kv, num_kv_heads, head_dim, value_dim)
-        self._check_slots(what, step)
-        if rotary is not None and (rotary.rotary_dim > head_dim or rotary.rotary_dim % 2 or rotary.inv_freq.dtype != torch.float32
-                                   or rotary.inv_freq.numel() * 2 < rotary.rotary_dim):
-            raise KernelError(f"{what}: a rotary table of float32 frequencies for an even number of a head's elements is expected")
-        for vector in norm[2:]:
-            if vector is not None and (vector.dtype != torch.float32 or vector.shape != (head_dim,) or vector.stride(0) != 1):
+        slots, norm_kind, norm_eps, q_weight, k_weight = step.slots, *norm
+        if slots is not None:
+            self._check_slots(what, step)
+        frequencies, rotary_dim, interleaved, factor = 0, 0, 0, 1.0
+        if rotary is not None:
+            rotary_dim, inv_freq = rotary.rotary_dim, rotary.inv_freq
+            if rotary_dim > head_dim or rotary_dim % 2 or inv_freq.dtype != torch.float32 or inv_freq.numel() * 2 < rotary_dim:
+                raise KernelError(f"{what}: a rotary table of float32 frequencies for an even number of a head's elements is expected")
+            frequencies, interleaved, factor = inv_freq.data_ptr(), int(rotary.interleaved), rotary.factor
+        for vector in (q_weight, k_weight):
+            if vector is not None and (vector.dtype != torch.float32 or vector.numel() != head_dim or not vector.is_contiguous()):
                 raise KernelError(f"{what}: float32 weights of {head_dim} elements are expected")
-        if q_out is not None and (q_out.dtype != self.dtype or q_out.stride(-1) != 1 or q_out.shape[-1] < num_heads * head_dim
-                                  or q_out.shape[-2] < step.num_tokens):
-            raise KernelError(f"{what}: q goes to {step.num_tokens} rows of {num_heads * head_dim} elements of {self.dtype}")
+        q_to = q_to_stride = 0
+        if q_out is not None:
+            shape, strides = q_out.shape, q_out.stride()
+            if q_out.dtype != self.dtype or strides[-1] != 1 or shape[-1] < num_heads * head_dim or shape[-2] < step.num_tokens:
+                raise KernelError(f"{what}: q goes to {step.num_tokens} rows of {num_heads * head_dim} elements of {self.dtype}")
+            q_to, q_to_stride = q_out.data_ptr(), strides[-2]
         coef, every = (float(q_temp[0]), float(q_temp[1])) if q_temp else (0.0, 0.0)
         code, splits, split_stride, q, q_stride, k, k_stride, v, v_stride = rows
+        table, k_scale, v_scale = kv.block_table, kv.k_scale, kv.v_scale
         with self._here():
             check(
                 packed("distie_rows_write")(
-                    q, q_stride, k, k_stride, v, v_stride, code, splits, split_stride, *bias, norm[0], norm[1], _ptr(norm[2]), _ptr(norm[3]),
-                    rotary.inv_freq.data_ptr() if rotary is not None else 0, rotary.rotary_dim if rotary is not None else 0,
-                    int(rotary.interleaved) if rotary is not None else 0, rotary.factor if rotary is not None else 1.0, coef, every,
-                    step.positions.data_ptr(), _ptr(step.slots), step.token_seq.data_ptr(), step.seq_seat.data_ptr(),
-                    kv.block_table.data_ptr(), kv.block_table.shape[-1], kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.k_scale), _ptr(kv.v_scale),
-                    step.num_tokens, num_heads if q else 0, num_kv_heads, head_dim, value_dim, kv.page_size, kv.num_pages, 1,
-                    _ptr(q_out), q_out.stride(-2) if q_out is not None else 0, _CACHE_CODE[self.dtype], cache_code,
+                    q, q_stride, k, k_stride, v, v_stride, code, splits, split_stride, *bias, norm_kind, norm_eps,
+                    0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+                    frequencies, rotary_dim, interleaved, factor, coef, every, step.positions.data_ptr(),
+                    0 if slots is None else slots.data_ptr(), step.token_seq.data_ptr(), step.seq_seat.data_ptr(),
+                    table.data_ptr(), table.shape[1], kv.k.data_ptr(), kv.v.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
+                    0 if v_scale is None else v_scale.data_ptr(), step.num_tokens, num_heads if q else 0, num_kv_heads, head_dim, value_dim,
+                    kv.page_size, kv.num_pages, 1, q_to, q_to_stride, _CACHE_CODE[self.dtype], cache_code,
                     self.error_flag.data_ptr(), self._stream(),
                 ),
                 "rows_write",
@@ -134,14 +144,15 @@ class CachedRows:
         float32 or the set's dtype, or float32 slices ``[S, T, n]``."""
         k0, v0 = num_heads * head_dim, (num_heads + num_kv_heads) * head_dim
         end = v0 + num_kv_heads * value_dim if values else v0
-        sliced, dtype = qkv.dim() == 3, qkv.dtype
-        if qkv.shape[-1] < end or qkv.shape[-2] < step.num_tokens or qkv.stride(-1) != 1 or (dtype != torch.float32 and (sliced or dtype != self.dtype)):
+        dtype, shape, strides = qkv.dtype, qkv.shape, qkv.stride()
+        sliced = len(shape) == 3
+        if shape[-1] < end or shape[-2] < step.num_tokens or strides[-1] != 1 or (dtype != torch.float32 and (sliced or dtype != self.dtype)):
             raise KernelError(f"{what}: a projection [{step.num_tokens}, {end}] of {self.dtype} or float32, or float32 slices of one, with unit "
-                              f"column stride is expected, not {tuple(qkv.shape)} of {dtype}")
-        if bias is not None and (bias.dtype != torch.float32 or bias.shape[-1] < end or bias.stride(-1) != 1):
+                              f"column stride is expected, not {tuple(shape)} of {dtype}")
+        if bias is not None and (bias.dtype != torch.float32 or bias.numel() < end or not bias.is_contiguous()):
             raise KernelError(f"{what}: a float32 bias of {end} elements is expected")
-        at, size, stride = qkv.data_ptr(), qkv.element_size(), qkv.stride(-2)
-        rows = (_CACHE_CODE[dtype], qkv.shape[0] if sliced else 1, qkv.stride(0) if sliced else 0, at, stride, at + k0 * size, stride,
+        at, size, stride = qkv.data_ptr(), 4 if dtype == torch.float32 else 2, strides[-2]
+        rows = (_CACHE_CODE[dtype], shape[0] if sliced else 1, strides[0] if sliced else 0, at, stride, at + k0 * size, stride,
                 at + v0 * size if values else 0, stride)
         b = bias.data_ptr() if bias is not None else 0
         self._rows_write(what, rows, (b, b + 4 * k0, b + 4 * v0) if b else (0, 0, 0), step, kv, rotary, num_heads, num_kv_heads,
@@ -158,25 +169,30 @@ class CachedRows:
 
     # -- read back ------------------------------------------------------------------------------------------------
     def kv_read(self, step, kv, window=None, chunk=None, keep_first=0) -> KvSlot:
-        num_kv_heads, page = kv.k.shape[1], kv.page_size
+        k, v, table, page, pages = kv.k, kv.v, kv.block_table, kv.page_size, kv.num_pages
         if kv.k_scale is None:
             raise KernelError("kv_read: the cache is in the engine's type already")
-        self._check_slot("kv_read", kv, num_kv_heads, kv.k.shape[-1], kv.v.shape[-1])
+        num_kv_heads, key_dim, value_dim = k.shape[1], k.shape[-1], v.shape[-1]
+        self._check_slot("kv_read", kv, num_kv_heads, key_dim, value_dim)
         plan, total = self._read_plan(step, page, int(window or 0), int(chunk or 0), int(keep_first or 0) if window else 0)
-        make = lambda dim: torch.empty((total, num_kv_heads, page, dim), dtype=self.dtype, device=kv.k.device)  # noqa: E731
-        out = KvSlot(make(kv.k.shape[-1]), make(kv.v.shape[-1]), torch.empty_like(kv.block_table), page, total)
-        with self._here():
-            for numbers, count, first, pages in plan:
+        if key_dim == value_dim and key_dim % 8 == 0:  # (one piece of memory; the values then begin at a multiple of 16 bytes)
+            k_out, v_out = torch.empty((2, total, num_kv_heads, page, key_dim), dtype=self.dtype, device=k.device).unbind()
+        else:
+            k_out = torch.empty((total, num_kv_heads, page, key_dim), dtype=self.dtype, device=k.device)
+            v_out = torch.empty((total, num_kv_heads, page, value_dim), dtype=self.dtype, device=k.device)
+        out = KvSlot(k_out, v_out, torch.empty_like(table), page, total)
+        for numbers, count, first, size in plan:
+            with self._here():
                 check(
                     packed("distie_rows_read")(
-                        ctypes.addressof(numbers), count, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
-                        kv.block_table.data_ptr(), kv.block_table.shape[-1], step.seq_seat.data_ptr(), num_kv_heads, kv.k.shape[-1],
-                        kv.v.shape[-1], page, kv.num_pages, out.k.data_ptr(), out.v.data_ptr(), out.block_table.data_ptr(), first, pages,
+                        ctypes.addressof(numbers), count, k.data_ptr(), v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
+                        table.data_ptr(), table.shape[1], step.seq_seat.data_ptr(), num_kv_heads, key_dim, value_dim, page, pages,
+                        k_out.data_ptr(), v_out.data_ptr(), out.block_table.data_ptr(), first, size,
                         _CACHE_CODE[self.dtype], self.error_flag.data_ptr(), self._stream(),
                     ),
                     "rows_read",
                 )
-                self._ran("rows_read")
+            self._ran("rows_read")
         return out
 
     def _read_plan(self, step, page: int, window: int, chunk: int, keep_first: int):
