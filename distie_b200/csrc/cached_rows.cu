@@ -367,15 +367,16 @@ rows_write_fast_kernel(RowsInput in, RowsNorm norm, RowsTurn turn, RowsPlace pla
 // ---- read back ----------------------------------------------------------------------------------------------------
 // Pages of up to kReadRows requests, one page of the result per block: numbers times scales in the set's type, zeros behind
 // a request's last row.  A page of the cache is one run of memory over all kv heads, and so is a page of the result.
-constexpr int kReadRows = 256;
+constexpr int kReadRows = 256, kReadFewRows = 8;  // (a launch copies the whole plan: 6 KB or 200 bytes)
+template <int ROWS>
 struct ReadPlan {
   int count;
-  int batch_row[kReadRows];    // of the step: its seat is read, and that seat's row of the result's table filled
-  int first_page[kReadRows];   // pages of the result before this request's
-  int first_column[kReadRows]; // its first logical page that is read
-  int hole[kReadRows];         // logical pages hole .. hole_end - 1 are not read: a window has passed them
-  int hole_end[kReadRows];
-  int length[kReadRows];       // its keys
+  int batch_row[ROWS];    // of the step: its seat is read, and that seat's row of the result's table filled
+  int first_page[ROWS];   // pages of the result before this request's
+  int first_column[ROWS]; // its first logical page that is read
+  int hole[ROWS];         // logical pages hole .. hole_end - 1 are not read: a window has passed them
+  int hole_end[ROWS];
+  int length[ROWS];       // its keys
 };
 
 template <typename T>
@@ -393,9 +394,9 @@ constexpr int kReadThreads = 256;
 constexpr int kReadPieces = 4;  // 16 numbers each, per thread: all requested before the first is stored
 
 // A block takes kReadThreads * kReadPieces pieces of a page (blockIdx.y: which of them, K's first, then V's).
-template <typename T>
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(kReadThreads)
-rows_read_kernel(const __grid_constant__ ReadPlan plan, CachePages cache, const int* __restrict__ seq_seat, T* __restrict__ k_out,
+rows_read_kernel(const __grid_constant__ ReadPlan<ROWS> plan, CachePages cache, const int* __restrict__ seq_seat, T* __restrict__ k_out,
                  T* __restrict__ v_out, int* __restrict__ table_out, int page0, int pages, int* __restrict__ error) {
   grid_dependency_release();
   if ((int)blockIdx.x >= pages) {  // blocks behind the pages: a row of the result's table each
@@ -411,7 +412,7 @@ rows_read_kernel(const __grid_constant__ ReadPlan plan, CachePages cache, const 
   }
   const int page_out = page0 + blockIdx.x;
   int i = 0;
-  for (int step = kReadRows / 2; step > 0; step >>= 1)
+  for (int step = ROWS / 2; step > 0; step >>= 1)
     if (i + step < plan.count && plan.first_page[i + step] <= page_out) i += step;
   const int column = plan.first_column[i] + page_out - plan.first_page[i];
   if (column >= plan.hole[i] && column < plan.hole_end[i]) return;  // (no table entry names this page of the result)
@@ -552,6 +553,23 @@ extern "C" int distie_rows_write(const void* q, int q_stride, const void* k, int
   return DISTIE_ERR_UNSUPPORTED;
 }
 
+template <typename T, int ROWS>
+static int launch_read(const int* plan, int count, const dim3& grid, const CachePages& cache, const int* seq_seat, void* k_out, void* v_out,
+                       int* table_out, int page0, int pages, int* error, cudaStream_t stream) {
+  ReadPlan<ROWS> p;
+  p.count = count;
+  for (int i = 0; i < count; ++i) {
+    p.batch_row[i] = plan[6 * i];
+    p.first_page[i] = plan[6 * i + 1];
+    p.first_column[i] = plan[6 * i + 2];
+    p.hole[i] = plan[6 * i + 3];
+    p.hole_end[i] = plan[6 * i + 4];
+    p.length[i] = plan[6 * i + 5];
+  }
+  return (int)launch_dependent(rows_read_kernel<T, ROWS>, grid, dim3(kReadThreads), 0, stream, p, cache, seq_seat, (T*)k_out, (T*)v_out, table_out,
+                               page0, pages, error);
+}
+
 // plan: `count` rows (batch row, first page of the result, first logical page, hole, end of the hole, keys) on the host; their
 // pages of the result are page0 .. page0 + pages - 1.  table_out: of the shape of block_table.
 extern "C" int distie_rows_read(const int* plan, int count, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -562,27 +580,17 @@ extern "C" int distie_rows_read(const int* plan, int count, const void* k_cache,
   if (count > kReadRows || num_kv_heads < 1 || key_dim < 1 || value_dim < 1 || page_size < 1 || table_width < 1 || k_scale == nullptr || v_scale == nullptr ||
       (long long)num_kv_heads * page_size * (key_dim + value_dim) > 1 << 30)
     return DISTIE_ERR_ARG;
-  ReadPlan p;
-  p.count = count;
-  for (int i = 0; i < count; ++i) {
-    p.batch_row[i] = plan[6 * i];
-    p.first_page[i] = plan[6 * i + 1];
-    p.first_column[i] = plan[6 * i + 2];
-    p.hole[i] = plan[6 * i + 3];
-    p.hole_end[i] = plan[6 * i + 4];
-    p.length[i] = plan[6 * i + 5];
-  }
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, key_dim, value_dim,
                                       page_size, num_pages);
   const long long pieces = (long long)num_kv_heads * page_size * (key_dim / 16 + value_dim / 16);
   const int per_block = kReadThreads * kReadPieces;
   const dim3 grid(pages + count, ((key_dim | value_dim) & 15) == 0 ? (unsigned)((pieces + per_block - 1) / per_block) : 1);
   if (out_type == DISTIE_BF16)
-    return (int)launch_dependent(rows_read_kernel<__nv_bfloat16>, grid, dim3(kReadThreads), 0, stream, p, cache, seq_seat, (__nv_bfloat16*)k_out,
-                                 (__nv_bfloat16*)v_out, table_out, page0, pages, error);
+    return count <= kReadFewRows ? launch_read<__nv_bfloat16, kReadFewRows>(plan, count, grid, cache, seq_seat, k_out, v_out, table_out, page0, pages, error, stream)
+                                 : launch_read<__nv_bfloat16, kReadRows>(plan, count, grid, cache, seq_seat, k_out, v_out, table_out, page0, pages, error, stream);
   if (out_type == DISTIE_F32)
-    return (int)launch_dependent(rows_read_kernel<float>, grid, dim3(kReadThreads), 0, stream, p, cache, seq_seat, (float*)k_out, (float*)v_out,
-                                 table_out, page0, pages, error);
+    return count <= kReadFewRows ? launch_read<float, kReadFewRows>(plan, count, grid, cache, seq_seat, k_out, v_out, table_out, page0, pages, error, stream)
+                                 : launch_read<float, kReadRows>(plan, count, grid, cache, seq_seat, k_out, v_out, table_out, page0, pages, error, stream);
   return DISTIE_ERR_UNSUPPORTED;
 }
 
