@@ -235,15 +235,16 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
   int block0, blocks;
   {
     TreeSpan span;
-    int low = 0x7fffffff, high = 0;
+    const bool everything = rows.window == 0 && rows.chunk == 0;  // (no need to look at positions)
+    int low = everything ? 0 : 0x7fffffff, high = 0;
     const int node0 = row0 / rows.group, node1 = (row0 + count - 1) / rows.group;
-    for (int n = node0 + lane; n <= node1; n += 32) {
+    for (int n = node0 + lane; n <= node1 && !everything; n += 32) {
       const int first = first_visible_key(rows.positions[request.first + n], rows.window, rows.chunk);
       low = min(low, first);
       high = max(high, first);
     }
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) {
+    for (int d = 16; d >= 1 && !everything; d >>= 1) {
       low = min(low, __shfl_xor_sync(0xffffffffu, low, d));
       high = max(high, __shfl_xor_sync(0xffffffffu, high, d));
     }
@@ -470,7 +471,6 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
         const int k_stage = n % kTreeKStages, v_stage = n % kTreeVStages;
         const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
         if (!wait(&sm.k_landed[k_stage], (n / kTreeKStages) & 1)) { ok = false; break; }
-        at = find(block0 + n + 1);
         if (E4M3) {
           // The slot's last scales have been read: the S of two blocks ago, whose stage K has taken, was issued behind the P of
           // two blocks before that.
@@ -485,11 +485,14 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
           sm.v_log[slot][key] = tree_log2(vs);
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.scale_full[slot]);
-          ks = __ldcg(cache.k_scale + max(at, 0ll));
-          vs = __ldcg(cache.v_scale + max(at, 0ll));
         }
         finish(sm.k[k_stage], there, false);
         ready(&sm.k_full[k_stage]);
+        at = find(block0 + n + 1);
+        if (E4M3) {
+          ks = __ldcg(cache.k_scale + max(at, 0ll));
+          vs = __ldcg(cache.v_scale + max(at, 0ll));
+        }
         if (!wait(&sm.v_landed[v_stage], (n / kTreeVStages) & 1)) { ok = false; break; }
         finish(sm.v[v_stage], there, !span.whole(block0 + n));
         ready(&sm.v_full[v_stage]);
@@ -551,7 +554,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = min(warp * 16 + i, count - 1);  // (rows behind the last one are nobody's: copies of it)
-        const int token = request.first + (row0 + r) / rows.group, head = kv_head * rows.group + (row0 + r) % rows.group;
+        const int token = sm.row_token[r], head = kv_head * rows.group + row0 + r - (token - request.first) * rows.group;
         const __nv_bfloat16* from = q + (size_t)token * q_stride + (size_t)head * D + lane * PER_LANE;
         if (PER_LANE == 4) x[i] = __ldcg(reinterpret_cast<const uint2*>(from));
         else x[i] = make_uint2(__ldcg(reinterpret_cast<const unsigned int*>(from)), 0u);
@@ -785,6 +788,10 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
         const float f0 = f[0] * inv, f1 = f[1] * inv;
         constexpr int SIDE = D / 2;  // group g writes columns g * D / 2 ... of the row, from both accumulators
         const size_t part_row = ((size_t)token * rows.num_heads + head) * parts.splits + split;
+        // Parts go to scratch by the copy engine, half a row at a time, from rows of shared memory that K and V have left.
+        constexpr int PITCH = SIDE * 4 + 16;
+        unsigned char* mine = &sm.k[0][0] + ((g * 4 + quadrant) * 32 + lane) * PITCH;
+        static_assert(2 * kTreeRows * PITCH <= kTreeKStages * kTreeKeys * D * 2 + kTreeVStages * kTreeKeys * D * 2);
 #pragma unroll 1
         for (int c0 = 0; c0 < SIDE; c0 += 16) {
           uint32_t a[16], b[16];
@@ -802,10 +809,17 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
               store8(to + i, part);
             }
           } else if (live) {
-            float* to = parts.o + part_row * D + g * SIDE + c0;
+            float* to = reinterpret_cast<float*>(mine) + c0;
 #pragma unroll
             for (int i = 0; i < 16; i += 4) store4(to + i, make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
           }
+        }
+        if (live && !alone) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(parts.o + part_row * D + g * SIDE), "r"(smem_u32(mine)),
+                       "r"(SIDE * 4) : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
         if (sm.bad && live) {  // values that are not finite join the sums of the rows that see them
 #pragma unroll 1
