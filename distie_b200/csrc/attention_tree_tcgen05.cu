@@ -607,7 +607,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
         // 32 keys at a time: 64 scores do not fit a thread's registers beside the rest, and what spills goes to L2 (shared memory
         // leaves L1 next to nothing).  P, two keys a column, takes the columns of scores that have been read.
         uint32_t next[32];
-#pragma unroll (E4M3 ? 1 : 2)
+#pragma unroll
         for (int piece = 0; piece < 2; ++piece) {
           uint32_t sv[32];  // scores in base-2 units, less the maximum in use
           if (E4M3 || piece == 0) tmem_load_32(s_addr + piece * 32, next);
