@@ -24,11 +24,12 @@
 // CTAs, are merged in the softmax's units: inside the cluster up to 8 splits, where every CTA sends its sums to the one that puts
 // them together (no CTA reads another's memory, none waits to leave), by a second kernel beyond.
 //
-// What bounds it: with many keys the bytes (13 requests of 30,011 keys, 8 key heads of 128: 824 MB in 130 us, 6.3 TB/s; 48 of
-// 4,099, 8 key heads of 64: 214 MB in 45 us inside the kernel, where a CTA's rounds of four groups take 1,600 cycles however
-// many of them an SM holds up to two).  With few keys a CTA's start (positions, seat, page ids, then q and the first rows: 5,000
-// cycles) and end (merge 1,200, cluster 3,500).  What was tried and took as long or longer: rings of 3, 4 and 6 groups and
-// CTAs of 8 warps (fewer CTAs fit an SM), boxes of 16 rows by the copy engine in place of cp.async.
+// What bounds it: with many long requests the bytes and the requests' uneven lengths (13 of 20,000 to 30,011 keys, 8 key heads of
+// 128: 634 MB in 130 us, 4.9 TB/s); with heads of 64 the instructions (48 requests of up to 4,099 keys, 8 key heads: 162 MB in 45 us
+// inside the kernel; 420 instructions a warp and group, 181 on the ALU pipe at half rate); with few keys a CTA's start
+// (positions, seat, page ids, then q and the first rows: 5,000 cycles) and end (merge 1,200, cluster 3,500).  What was tried
+// and took as long or longer: rings of 3, 4 and 6 groups and CTAs of 8 warps (fewer CTAs fit an SM), boxes of 16 rows by the copy
+// engine in place of cp.async.
 #include <cuda_fp16.h>
 
 #include "cached_rows.cuh"
