@@ -109,7 +109,8 @@ class Engine:
 
         ``knobs``: ``num_blocks`` or ``gpu_mem_fraction``, ``page_size``, ``max_seqs``, ``token_budget``,
         ``prefill_chunk``, ``max_model_len``, ``decode_graphs``, ``decode_ahead``, ``step_stats``,
-        ``float32_weights``, ``cache_dtype`` (``"float8_e4m3"``: keys and values in eight bits with a scale per row); the reference's ``WORKER_*`` environment variables give the defaults.
+        ``float32_weights``, ``cache_dtype`` (``"float8_e4m3"``: keys and values in eight bits with a scale per
+        row); the reference's ``WORKER_*`` environment variables give the defaults.
         """
         if device == "cuda":
             device = "cuda:0"
@@ -356,6 +357,7 @@ class Engine:
         """
         if not prompt_ids:
             raise ValueError("prompt_ids must be non-empty")
+        self.runner.check_drafted()
         limit = clamp_max_tokens(max_new_tokens)
         longest = self.cache.max_tokens_per_request
         if len(prompt_ids) + limit > longest:

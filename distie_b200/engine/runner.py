@@ -102,14 +102,19 @@ class ModelRunner:
         self.steps = 0
 
     # -- the step function ----------------------------------------------------
+    def check_drafted(self) -> None:
+        """Refuses steps of drafted tokens where a layer or the kernel set does not take them."""
+        if not self._takes_trees:
+            raise ValueError("drafted tokens branch: layers with per-request state and attention through a latent do not take them")
+
     @torch.inference_mode()
     def step(self, entries: Sequence[BatchEntry]) -> torch.Tensor | None:
         """Logits at the wanted places, in the order of entries and of ``want``.  Entries with ``parents`` make it a step of
         drafted tokens, for models all of whose layers are plain attention: the rows of all their tokens are in
         the cache afterwards, at the places behind the request's cached ones (``CacheManager.keep_places`` takes the accepted ones)."""
         drafted = any(entry.parents is not None for entry in entries)
-        if drafted and not self._takes_trees:
-            raise ValueError("drafted tokens branch: layers with per-request state and attention through a latent do not take them")
+        if drafted:
+            self.check_drafted()
         if not drafted and self.use_graphs and len(entries) <= self._sizes[-1] and all(len(e.tokens) == 1 for e in entries):
             logits = self._graph_logits(entries)
             if logits is not NotImplemented:

@@ -543,7 +543,8 @@ class DeviceKernels(CachedRows, KernelSet):
         projection's float32 slices itself (bias, rotation, the token's key and value into the cache and into
         its own tile), so the kernel between the projection and the attention is not launched."""
         merged = (
-            step.tree is None and kv.k_scale is None and step.slots is None and step.num_decode_tokens == step.num_tokens and self.dtype == torch.bfloat16 and head_dim in _PREFILL_HEAD_DIMS
+            step.tree is None and not self._apart(step, kv)
+            and step.num_decode_tokens == step.num_tokens and self.dtype == torch.bfloat16 and head_dim in _PREFILL_HEAD_DIMS
             and self._skinny(x, weight) and weight.shape[0] == (num_heads + 2 * num_kv_heads) * head_dim
             and (rotary is None or (rotary.rotary_dim == head_dim and not rotary.interleaved))
             and (bias is None or bias.dtype == torch.float32) and kv.k.dtype == torch.bfloat16

@@ -198,3 +198,17 @@ def test_shares_of_the_keys():
                 for many in (False, True):
                     assert 1 <= decode_splits(blocks, keys, 148, wide, many) <= max(1, min(64, keys // 256))
             assert 1 <= tree_splits(blocks, -(-keys // 128), 148) <= max(1, min(64, -(-keys // 128)))
+
+
+def test_drafted_generation_is_refused_before_the_prompt_runs():
+    from test_cached_engine import engine_for
+
+    engine, _, _ = engine_for("A")
+    engine.runner._takes_trees = False
+
+    def step(entries):
+        raise AssertionError("a step has run")
+
+    engine.runner.step = step
+    with pytest.raises(ValueError, match="drafted tokens branch"):
+        engine.generate_drafted([1, 2, 3], lambda ids: ([], []))
