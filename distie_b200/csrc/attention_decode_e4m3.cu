@@ -18,8 +18,8 @@
 //
 // Scales: s^k multiplies the finished score.  s^v cannot ride on V without rounding it; p_j s^v_j goes into the second product
 // in float16, in units of a running maximum m' of its own beside the softmax's m: p_j (s^v_j 2^(m - m')), however the scales
-// differ at most a few, and off by at most 2^-11 of itself (or of 2^-14).  Both maxima are whole numbers (what they scale,
-// they scale exactly) and are not searched for in every group, only in a head's first and where weights outgrow the ones in
+// differ at most a few, and off by at most 2^-11 of itself (or of 2^-14).  Both maxima are whole numbers, rounded down (what they
+// scale, they scale exactly), and are not searched for in every group, only in a head's first and where weights outgrow the ones in
 // use: no shuffles and no correction of O in most groups.  Sums and maxima are float32.  The warps, and with several splits the
 // CTAs, are merged in the softmax's units: inside the cluster up to 8 splits, where every CTA sends its sums to the one that puts
 // them together (no CTA reads another's memory, none waits to leave), by a second kernel beyond.
@@ -354,7 +354,7 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
               mo = fmaxf(mo, __shfl_xor_sync(0xffffffffu, mo, d));
             }
             const float shift = col_max[nh][e] == -INFINITY ? 0.f : col_max[nh][e];
-            const float o_new = fmaxf(out_max[nh][e], shift + ceilf(mo)), m_new = fmaxf(col_max[nh][e], shift + ceilf(m));
+            const float o_new = fmaxf(out_max[nh][e], shift + floorf(mo)), m_new = fmaxf(col_max[nh][e], shift + floorf(m));
             const float corr = o_new > out_max[nh][e] ? dec_exp2(out_max[nh][e] - o_new) : 1.f;  // (exp2(-inf) is 0)
             if (m_new > col_max[nh][e]) {
               col_sum[nh][e] *= dec_exp2(col_max[nh][e] - m_new);

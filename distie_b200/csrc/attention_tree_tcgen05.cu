@@ -26,8 +26,8 @@
 // element.  Rows of keys that belong to nobody are zeros.
 //
 // Running maxima are not searched for in every block, only in a row's first and where its weights outgrow the one in use;
-// then O, and what P of the block is there already, are read, scaled and written back.  The maxima are whole numbers, so that
-// scaling is exact.
+// then O, and what P of the block is there already, are read, scaled and written back.  The maxima are whole numbers (rounded down), so
+// that scaling is exact.
 //
 // What bounds it: the softmax warps.  Two trees of 64 new tokens over 16,001 keys (40 heads of 128, 8 key heads, bfloat16): 72 us
 // with the joining kernel, 144 CTAs of 44 blocks at 2,400 cycles a block, of which the products take 1,050 and each
@@ -662,10 +662,10 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                 }
               }
               // The maximum for the sum, and the one for O (of a 16-bit cache they are one).
-              const float m_new = fmaxf(m_used, shift + ceilf(mx));
+              const float m_new = fmaxf(m_used, shift + floorf(mx));
               float corr = 1.f;
               if (E4M3) {
-                const float o_new = fmaxf(o_used, shift + ceilf(ox));
+                const float o_new = fmaxf(o_used, shift + floorf(ox));
                 if (o_new > o_used) {
                   corr = exp2_approx(o_used - o_new);
                   o_used = o_new;
@@ -819,7 +819,9 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
           asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(parts.o + part_row * D + g * SIDE), "r"(smem_u32(mine)),
                        "r"(SIDE * 4) : "memory");
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+          // (read from here before the CTA leaves; written before anything else looks at them below)
+          if (sm.bad) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+          else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         }
         if (sm.bad && live) {  // values that are not finite join the sums of the rows that see them
 #pragma unroll 1
