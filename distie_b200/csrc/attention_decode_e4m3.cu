@@ -256,12 +256,14 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
 
   float o[NH][MT][4];  // O^T: dims 16 mt + 2 g (+ 1), heads 2 c (+ 1): [dim 2g: head, head + 1 | dim 2g + 1: head, head + 1]
   float col_max[NH][2], col_sum[NH][2], out_max[NH][2], units[NH][2];  // units: 2^(col_max - out_max)
+  bool unset[NH];  // a maximum of the lane's two heads is still to be found
 #pragma unroll
   for (int nh = 0; nh < NH; ++nh) {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[nh][i][r] = 0.f;
+    unset[nh] = true;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       col_max[nh][e] = out_max[nh][e] = -INFINITY;
@@ -319,6 +321,7 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
       ks_s[i] = scales[8 * i + g];
       vs_s[i] = scales[kDecKeys + 8 * i + g];
       keep[i] = !edge || (base + 8 * i + g >= lo_key && base + 8 * i + g <= hi_key);
+      if (edge && !keep[i]) vs_s[i] = 0.f;  // (a scale that is not finite would outlive its weight of 0)
     }
     uint32_t pb[kDecKeys / 16][NH][2];
 #pragma unroll
@@ -333,8 +336,13 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
           // (cap * tanh, by its exponential: off by 2^-22 of the cap)
           const float s = rows.extras.cap > 0.f ? cap * (1.f - __fdividef(2.f, dec_exp2(raw * each * 2.8853900817779268f) + 1.f)) - shift
                                                 : fmaf(raw, each, -shift);
-          x[i][e] = keep[i] ? s : -INFINITY;
+          x[i][e] = s;
         }
+      }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < RK; ++i)
+          if (!keep[i]) x[i][0] = x[i][1] = -INFINITY;
       }
       bool search = false;
 #pragma unroll 1
@@ -346,7 +354,7 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
 #pragma unroll
             for (int i = 0; i < RK; ++i) {
               m = fmaxf(m, x[i][e]);
-              mo = fmaxf(mo, keep[i] ? x[i][e] + dec_log2(vs_s[i]) : -INFINITY);
+              mo = fmaxf(mo, x[i][e] + dec_log2(vs_s[i]));
             }
 #pragma unroll
             for (int d = 4; d <= 16; d <<= 1) {
@@ -371,9 +379,10 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
               o[nh][mt][e + 2] *= corr;
             }
           }
+          unset[nh] = col_max[nh][0] == -INFINITY || col_max[nh][1] == -INFINITY || out_max[nh][0] == -INFINITY || out_max[nh][1] == -INFINITY;
           __syncwarp();
         }
-        bool outgrown = false;
+        float most = 0.f;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float weights = 0.f;
@@ -382,12 +391,12 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
           for (int i = 0; i < RK; ++i) {
             const float p = dec_exp2(x[i][e]);
             sum[e] += p;
-            w[i][e] = keep[i] ? p * (vs_s[i] * units[nh][e]) : 0.f;
+            w[i][e] = p * (vs_s[i] * units[nh][e]);
             weights += w[i][e];
           }
-          outgrown = outgrown || sum[e] > kDecMostSum || weights > kDecMostWeight || col_max[nh][e] == -INFINITY || out_max[nh][e] == -INFINITY;
+          most = fmaxf(most, fmaxf(weights, sum[e] * (kDecMostWeight / kDecMostSum)));
         }
-        if (search || !__any_sync(0xffffffffu, outgrown)) break;
+        if (search || !__any_sync(0xffffffffu, unset[nh] || most > kDecMostWeight)) break;
         search = true;
       }
       col_sum[nh][0] += sum[0];
