@@ -562,7 +562,7 @@ static cudaError_t launch_decode(const dim3& grid, const __nv_bfloat16* q, int q
 using namespace distie;
 
 // Single tokens over an 8-bit cache: q [tokens, >= heads * head_dim] and out bfloat16; heads of 64 or 128, keys and values
-// alike (else DISTIE_ERR_UNSUPPORTED, like rows that are not 8-byte aligned).  scratch: distie_attention_rows_scratch_floats, for more than 8 splits.
+// alike (else DISTIE_ERR_UNSUPPORTED, like rows that are not 8-byte aligned).  scratch: tokens * heads * splits * (value size + 2) floats, for more than 8 splits.
 extern "C" int distie_attention_decode_e4m3(const void* q, int q_stride, void* out, int out_stride, float* scratch, const int* positions,
                                             const int* token_seq, const int* seq_seat, int tokens, const void* k_cache, const void* v_cache,
                                             const float* k_scale, const float* v_scale, const int* block_table, int table_width,

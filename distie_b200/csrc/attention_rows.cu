@@ -331,12 +331,8 @@ int rows_merge_bf16(const Partials& parts, void* out, int out_stride, int tokens
 
 using namespace distie;
 
-extern "C" long long distie_attention_rows_scratch_floats(int tokens, int num_heads, int value_dim, int splits) {
-  return splits > 1 ? (long long)tokens * num_heads * splits * (value_dim + 2) : 0;
-}
-
 // q [tokens, >= heads * key_dim], out [tokens, heads * value_dim] of type `dtype`; seqs null: single tokens, `requests` of
-// them, else [requests, 3] with at most most_nodes new tokens each.  scratch: distie_attention_rows_scratch_floats.
+// them, else [requests, 3] with at most most_nodes new tokens each.  scratch: tokens * heads * splits * (value size + 2) floats.
 extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int out_stride, float* scratch, const int* positions,
                                      const int* token_seq, const int* seq_seat, const int* seqs, const int* bits, int words,
                                      int requests, int tokens, int most_nodes, const void* k_cache, const void* v_cache,

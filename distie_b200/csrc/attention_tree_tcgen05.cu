@@ -878,7 +878,7 @@ using namespace distie;
 
 // Drafted tokens: q [tokens, >= heads * head_dim] and out [tokens, heads * head_dim] bfloat16, a cache of bfloat16 or (with
 // scales) e4m3, heads of 64 or 128 (else DISTIE_ERR_UNSUPPORTED, like rows that are not aligned to what a thread moves), at most
-// 256 new tokens a request.  seqs [requests, 3], bits [tokens, words].  scratch: distie_attention_rows_scratch_floats.
+// 256 new tokens a request.  seqs [requests, 3], bits [tokens, words].  scratch: tokens * heads * splits * (value size + 2) floats.
 extern "C" int distie_attention_tree_tcgen05(const void* q, int q_stride, void* out, int out_stride, float* scratch, const int* positions,
                                              const int* seq_seat, const int* seqs, const int* bits, int words, int requests, int tokens,
                                              int most_nodes, const void* k_cache, const void* v_cache, const float* k_scale,

@@ -15,7 +15,7 @@ import functools
 import torch
 
 from .interface import E4M3, MOST_DRAFTED, KvSlot, first_visible
-from .library import KernelError, check, function, packed
+from .library import KernelError, check, packed
 
 _CACHE_CODE = {torch.float32: 0, torch.bfloat16: 1, E4M3: 2}
 _READ_ROWS = 256  # requests that one launch reads back
@@ -122,9 +122,10 @@ class CachedRows:
         coef, every = (float(q_temp[0]), float(q_temp[1])) if q_temp else (0.0, 0.0)
         code, splits, split_stride, q, q_stride, k, k_stride, v, v_stride = rows
         table, k_scale, v_scale = kv.block_table, kv.k_scale, kv.v_scale
+        launch, pack = packed("distie_rows_write")
         with self._here():
             check(
-                packed("distie_rows_write")(
+                launch(pack(
                     q, q_stride, k, k_stride, v, v_stride, code, splits, split_stride, *bias, norm_kind, norm_eps,
                     0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
                     frequencies, rotary_dim, interleaved, factor, coef, every, step.positions.data_ptr(),
@@ -133,7 +134,7 @@ class CachedRows:
                     0 if v_scale is None else v_scale.data_ptr(), step.num_tokens, num_heads if q else 0, num_kv_heads, head_dim, value_dim,
                     kv.page_size, kv.num_pages, 1, q_to, q_to_stride, _CACHE_CODE[self.dtype], cache_code,
                     self.error_flag.data_ptr(), self._stream(),
-                ),
+                )),
                 "rows_write",
             )
         self._ran("rows_write")
@@ -182,14 +183,15 @@ class CachedRows:
             v_out = torch.empty((total, num_kv_heads, page, value_dim), dtype=self.dtype, device=k.device)
         out = KvSlot(k_out, v_out, torch.empty_like(table), page, total)
         for numbers, count, first, size in plan:
+            launch, pack = packed("distie_rows_read")
             with self._here():
                 check(
-                    packed("distie_rows_read")(
+                    launch(pack(
                         ctypes.addressof(numbers), count, k.data_ptr(), v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
                         table.data_ptr(), table.shape[1], step.seq_seat.data_ptr(), num_kv_heads, key_dim, value_dim, page, pages,
                         k_out.data_ptr(), v_out.data_ptr(), out.block_table.data_ptr(), first, size,
                         _CACHE_CODE[self.dtype], self.error_flag.data_ptr(), self._stream(),
-                    ),
+                    )),
                     "rows_read",
                 )
             self._ran("rows_read")
@@ -221,6 +223,10 @@ class CachedRows:
         return made
 
     # -- attention ------------------------------------------------------------------------------------------------
+    def _parts(self, tokens: int, num_heads: int, value_dim: int, splits: int) -> torch.Tensor:
+        """Room for the parts that several shares of the keys leave: sums of values, a maximum and a sum of weights each."""
+        return torch.empty(tokens * num_heads * splits * (value_dim + 2), dtype=torch.float32, device=self.error_flag.device)
+
     def _attention_rows(self, q, out, step, kv, num_heads, num_kv_heads, head_dim, window, chunk, scale, keep_first, softcap, sink,
                         tokens: int, requests: int) -> None:
         """The first ``tokens`` tokens of the step: all of a step of drafted tokens, or its single tokens."""
@@ -250,13 +256,11 @@ class CachedRows:
             return
         blocks = requests * num_kv_heads * -(-most * group // 16)
         splits = max(1, min(4 * self.sm_count // blocks, step.max_kv_len // 64, 64))
-        scratch = None
-        if splits > 1:
-            floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, value_dim, splits)
-            scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        scratch = self._parts(tokens, num_heads, value_dim, splits) if splits > 1 else None
+        launch, pack = packed("distie_attention_rows")
         with self._here():
             check(
-                packed("distie_attention_rows")(
+                launch(pack(
                     q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
                     step.token_seq.data_ptr(), step.seq_seat.data_ptr(), _ptr(tree.seqs) if tree is not None else 0,
                     _ptr(tree.bits) if tree is not None else 0, tree.bits.shape[1] if tree is not None else 1, requests, tokens, most,
@@ -264,7 +268,7 @@ class CachedRows:
                     kv.block_table.shape[-1], num_heads, num_kv_heads, head_dim, value_dim, kv.page_size, kv.num_pages, window, chunk,
                     keep_first, float(scale), softcap, _ptr(sink), splits, _CACHE_CODE[self.dtype], cache_code,
                     self.error_flag.data_ptr(), self._stream(),
-                ),
+                )),
                 "attention_rows",
             )
         self._ran("attention_rows", 1 if splits == 1 else 2)
@@ -277,18 +281,16 @@ class CachedRows:
         blocks = tokens * num_kv_heads * -(-num_heads // num_kv_heads // 16)
         seen = min(step.max_kv_len, window or chunk or step.max_kv_len)
         splits = decode_splits(blocks, seen, self.sm_count, head_dim == 128, num_heads // num_kv_heads > 8)
-        scratch = None
-        if splits > 8:
-            floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, head_dim, splits)
-            scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        scratch = self._parts(tokens, num_heads, head_dim, splits) if splits > 8 else None
+        launch, pack = packed("distie_attention_decode_e4m3")
         with self._here():
-            code = packed("distie_attention_decode_e4m3")(
+            code = launch(pack(
                 q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
                 step.token_seq.data_ptr(), step.seq_seat.data_ptr(), tokens, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(),
                 kv.v_scale.data_ptr(), kv.block_table.data_ptr(), kv.block_table.shape[-1], num_heads, num_kv_heads, head_dim,
                 kv.page_size, kv.num_pages, window, chunk, keep_first, float(scale), softcap, _ptr(sink), splits,
                 self.error_flag.data_ptr(), self._stream(),
-            )
+            ))
         if code == -2:
             return False
         check(code, "attention_decode_e4m3")
@@ -303,18 +305,16 @@ class CachedRows:
         tree, group = step.tree, num_heads // num_kv_heads
         seen = min(step.max_kv_len, (window or chunk or step.max_kv_len) + most + 128)
         splits = tree_splits(requests * num_kv_heads * -(-most * group // 128), -(-seen // 128), self.sm_count)
-        scratch = None
-        if splits > 1:
-            floats = function("distie_attention_rows_scratch_floats")(tokens, num_heads, head_dim, splits)
-            scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        scratch = self._parts(tokens, num_heads, head_dim, splits) if splits > 1 else None
+        launch, pack = packed("distie_attention_tree_tcgen05")
         with self._here():
-            code = packed("distie_attention_tree_tcgen05")(
+            code = launch(pack(
                 q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
                 step.seq_seat.data_ptr(), tree.seqs.data_ptr(), tree.bits.data_ptr(), tree.bits.shape[1], requests, tokens, most,
                 kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.k_scale), _ptr(kv.v_scale), kv.block_table.data_ptr(),
                 kv.block_table.shape[-1], num_heads, num_kv_heads, head_dim, kv.page_size, kv.num_pages, window, chunk, keep_first,
                 float(scale), softcap, _ptr(sink), splits, self.error_flag.data_ptr(), self._stream(),
-            )
+            ))
         if code == -2:
             return False
         check(code, "attention_tree_tcgen05")

@@ -130,7 +130,6 @@ _SIGNATURES: dict[str, tuple[str, list]] = {
                    P, I, I, I, P, P]
     ),
     "distie_rows_read": ("cached", [P, I, P, P, P, P, P, I, P, I, I, I, I, I, P, P, P, I, I, I, P, P]),
-    "distie_attention_rows_scratch_floats": ("cached", [I, I, I, I]),
     "distie_attention_rows": (
         "cached", [P, I, P, I, P, P, P, P, P, P, I, I, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, F, P, I, I, I, P, P]
     ),
@@ -154,7 +153,7 @@ _SIGNATURES: dict[str, tuple[str, list]] = {
 _RESULT = {"distie_gemm_float32_scratch_floats": c_longlong, "distie_attention_prefill_pairs_scratch_floats": c_longlong, "distie_retention_scratch_floats": c_longlong, "distie_recurrence_chunks_scratch_floats": c_longlong,
            "distie_exp_gate_scratch_floats": c_longlong, "distie_attention_decode_scratch_floats": c_longlong, "distie_route_plan_words": c_longlong,
            "distie_latent_attention_scratch_floats": c_longlong, "distie_selective_scan_scratch_floats": c_longlong,
-           "distie_channel_delta_scratch_floats": c_longlong, "distie_attention_rows_scratch_floats": c_longlong}
+           "distie_channel_delta_scratch_floats": c_longlong}
 
 _libraries: dict[str, ctypes.CDLL] = {}
 _functions: dict[str, object] = {}
@@ -200,13 +199,14 @@ def function(name: str):
 
 
 _CODES = {P: "P", I: "i", F: "f", L: "q"}
-_packed: dict[str, object] = {}
+_packed: dict[str, tuple] = {}
 
 
 def packed(name: str):
-    """The launcher called with one block of memory instead of its many arguments (csrc/packed.h): pointers are integers, 0 for none."""
-    call = _packed.get(name)
-    if call is None:
+    """(launcher, pack): the launcher takes one block of memory instead of its many arguments (csrc/packed.h), ``launcher(pack(...))``;
+    pointers are integers, 0 for none."""
+    pair = _packed.get(name)
+    if pair is None:
         unit, argtypes = _SIGNATURES[name]
         lib = load_unit(unit)
         try:
@@ -214,13 +214,8 @@ def packed(name: str):
         except AttributeError as exc:
             raise KernelError(f"kernel library of unit {unit!r} has no symbol {name}_packed") from exc
         fn.argtypes, fn.restype = [ctypes.c_char_p], c_int
-        pack = struct.Struct("@" + "".join(_CODES[t] for t in argtypes)).pack
-
-        def call(*args):
-            return fn(pack(*args))
-
-        _packed[name] = call
-    return call
+        pair = _packed[name] = (fn, struct.Struct("@" + "".join(_CODES[t] for t in argtypes)).pack)
+    return pair
 
 
 _ARG_ERRORS = {-1: "invalid argument", -2: "size or dtype not supported by this kernel"}
