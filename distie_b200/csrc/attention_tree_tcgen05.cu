@@ -30,8 +30,8 @@
 // that scaling is exact.
 //
 // What bounds it: the softmax warps.  Two trees of 64 new tokens over 16,001 keys (40 heads of 128, 8 key heads, bfloat16): 72 us
-// with the joining kernel, 144 CTAs of 44 blocks at 2,400 cycles a block, of which the products take 1,050 and each
-// scheduler's 128 exponentials 1,024; over an 8-bit cache 103 us, 3,500 cycles a block (scales read and multiplied, weights summed
+// with the joining kernel, 144 CTAs of 44 blocks at 2,300 cycles a block, of which the products take 1,050 and each
+// scheduler's 128 exponentials 1,024; over an 8-bit cache 98 us, 3,400 cycles a block (scales read and multiplied, weights summed
 // once more for their limit).  Registers decide: 15 warps have 128 each, and a version that keeps 64 scores a thread spills.
 // With several shares of the keys, the parts go to scratch in float32 and attention_rows.cu joins them.
 //

@@ -28,11 +28,12 @@ def _ptr(x) -> int:
 @functools.lru_cache(maxsize=256)
 def tree_splits(tiles: int, blocks: int, sms: int) -> int:
     """Shares that the keys of ``tiles`` tiles of rows, ``blocks`` blocks of 128 keys each, are cut into
-    (attention_tree_tcgen05.cu): the number for which whole waves of CTAs take the least time, a CTA the time of its blocks
-    and of two more for its start and end; joining the parts takes another two."""
+    (attention_tree_tcgen05.cu): the number for which whole waves of CTAs, one an SM, take the least time, a CTA the time of its
+    blocks and of eight more for its start and end (1.2 and 10 us); joining the parts takes another two.  (8 tiles of 24 blocks:
+    45, 33, 28 and 26 us with 1 to 4 shares, 22 with 8 and 12; 64 of 17: 47, 38, 44, 44; 192 of 17: 60, 74, 80, 94.)"""
     best, least = 1, None
     for splits in range(1, max(1, min(blocks, 64)) + 1):
-        cost = -(-tiles * splits // sms) * (-(-blocks // splits) + 2) + (2 if splits > 1 else 0)
+        cost = -(-tiles * splits // sms) * (-(-blocks // splits) + 8) + (2 if splits > 1 else 0)
         if least is None or cost < least:
             best, least = splits, cost
     return best
