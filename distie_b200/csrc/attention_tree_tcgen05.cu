@@ -232,10 +232,10 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
   const int* table = cache.block_table + (size_t)request.seat * cache.table_width;
 
   grid_dependency_release();
-  int block0, blocks;
+  int block0, blocks, column0, columns;
+  const bool everything = rows.window == 0 && rows.chunk == 0;  // (no need to look at positions)
   {
     TreeSpan span;
-    const bool everything = rows.window == 0 && rows.chunk == 0;  // (no need to look at positions)
     int low = everything ? 0 : 0x7fffffff, high = 0;
     const int node0 = row0 / rows.group, node1 = (row0 + count - 1) / rows.group;
     for (int n = node0 + lane; n <= node1 && !everything; n += 32) {
@@ -259,6 +259,10 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
     const int share = (span.blocks + parts.splits - 1) / parts.splits;
     block0 = min(span.blocks, split * share);
     blocks = min(span.blocks, block0 + share) - block0;
+    // The page ids of the share's keys from its window's first block on.
+    column0 = cache.column_of(span.key0(max(block0, span.kept_blocks)));
+    columns = block0 + blocks > span.kept_blocks
+                  ? min(kTreePages, cache.column_of(min(span.keys - 1, span.key0(block0 + blocks - 1) + kTreeKeys - 1)) - column0 + 1) : 0;
     if (threadIdx.x == 0) sm.span = span;
   }
   if (blocks == 0) {  // a share without keys: its parts count nothing
@@ -275,52 +279,54 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
     return;
   }
 
-  if (threadIdx.x == 0) {
-    mbar_init(&sm.q_full, kTreeMmaWarp);
-    for (int s = 0; s < kTreeKStages; ++s) {
-      mbar_init(&sm.k_full[s], kTreeLoaders);
-      mbar_init(&sm.k_empty[s], 1);
-      mbar_init(&sm.k_landed[s], 1);
+  // Four jobs at once: barriers, tensor memory, what is known of the rows, page ids (they wait for one load each).
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_init(&sm.q_full, kTreeMmaWarp);
+      mbar_init(&sm.merge_ready, 2 * active);
+      sm.failed = 0;
+      sm.bad = 0;
     }
-    for (int s = 0; s < kTreeVStages; ++s) {
-      mbar_init(&sm.v_full[s], kTreeLoaders);
-      mbar_init(&sm.v_empty[s], 1);
-      mbar_init(&sm.v_landed[s], 1);
+    if (lane < kTreeKStages) {
+      mbar_init(&sm.k_full[lane], kTreeLoaders);
+      mbar_init(&sm.k_empty[lane], 1);
+      mbar_init(&sm.k_landed[lane], 1);
     }
-    for (int s = 0; s < kTreeScaleSlots; ++s) mbar_init(&sm.scale_full[s], kTreeLoaders);
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&sm.s_full[b], 1);
-      mbar_init(&sm.p_full[0][b], active);
-      mbar_init(&sm.p_full[1][b], active);
-      mbar_init(&sm.pv_done[b], 1);
+    if (lane < kTreeVStages) {
+      mbar_init(&sm.v_full[lane], kTreeLoaders);
+      mbar_init(&sm.v_empty[lane], 1);
+      mbar_init(&sm.v_landed[lane], 1);
     }
-    mbar_init(&sm.merge_ready, 2 * active);
-    sm.failed = 0;
-    sm.bad = 0;
+    if (lane < kTreeScaleSlots) mbar_init(&sm.scale_full[lane], kTreeLoaders);
+    if (lane < 2) {
+      mbar_init(&sm.s_full[lane], 1);
+      mbar_init(&sm.p_full[0][lane], active);
+      mbar_init(&sm.p_full[1][lane], active);
+      mbar_init(&sm.pv_done[lane], 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kTreeMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
   }
-  for (int n = threadIdx.x; n < request.nodes && n < kTreeMostNodes; n += kTreeThreads)
-    sm.node_position[n] = rows.positions[request.first + n];
-  for (int r = threadIdx.x; r < kTreeRows; r += kTreeThreads) {
-    const int token = r < count ? request.first + (row0 + r) / rows.group : -1;
-    sm.row_token[r] = token;
-    sm.row_first[r] = token < 0 ? 0 : first_visible_key(rows.positions[token], rows.window, rows.chunk);
-  }
+  if (warp >= kTreeCopyWarp)  // (the warps below alone look at them)
+    for (int i = threadIdx.x - kTreeCopyWarp * 32; i < columns; i += (kTreeLoaders + 2) * 32)
+      sm.pages[i] = column0 + i < cache.table_width ? table[column0 + i] : -1;
+  if (warp < kTreeMmaWarp)
+    for (int n = threadIdx.x; n < max(kTreeRows, min(request.nodes, kTreeMostNodes)); n += kTreeMmaWarp * 32) {
+      if (n < request.nodes) sm.node_position[n] = everything ? 0 : rows.positions[request.first + n];
+      if (n < kTreeRows) {
+        const int token = n < count ? request.first + (row0 + n) / rows.group : -1;
+        sm.row_token[n] = token;
+        sm.row_first[n] = token < 0 || everything ? 0 : first_visible_key(rows.positions[token], rows.window, rows.chunk);
+      }
+    }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const TreeSpan& span = sm.span;
   const int block1 = block0 + blocks;
-  // The page ids of the share's keys from its window's first block on.
-  const int column0 = cache.column_of(span.key0(max(block0, span.kept_blocks)));
-  const int columns = block1 > span.kept_blocks ? min(kTreePages, cache.column_of(min(span.keys - 1, span.key0(block1 - 1) + kTreeKeys - 1)) - column0 + 1) : 0;
-  if (warp >= kTreeCopyWarp)  // (the warps below alone look at them)
-    for (int i = threadIdx.x - kTreeCopyWarp * 32; i < columns; i += (kTreeLoaders + 2) * 32)
-      sm.pages[i] = column0 + i < cache.table_width ? table[column0 + i] : -1;
   const uint32_t tmem = sm.tmem_base;
   grid_dependency_wait();  // q and the newest rows come from the kernels before this one
 
@@ -329,7 +335,6 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
     // Packed rows: those of 32 keys land in the first 32 lines of 128 bytes that these keys will take, rows of 256 bytes in two
     // halves of 16 keys.
     constexpr int FIT = BYTES > 128 ? 16 : 32;
-    asm volatile("bar.sync 1, %0;" ::"n"((kTreeLoaders + 2) * 32) : "memory");  // the page ids are there
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_unless(bar, parity, failed)) != 0; };
     auto page_at = [&](int column) {
       const int index = column - column0;
@@ -548,34 +553,37 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
   } else {
     // ---- queries into shared memory: a warp takes 16 rows ---------------------------------------------------------------
     {
-      constexpr int PER_LANE = D / 32;  // 4 or 2 elements
+      constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;  // lanes of 8 elements to a row; rows that the warp takes at a time
       const float unit_times = rows.extras.cap > 0.f ? rows.extras.cap_pre : rows.scale_log2;
-      uint2 x[16];
+      uint2 x[16 / AT_ONCE][2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = min(warp * 16 + i, count - 1);  // (rows behind the last one are nobody's: copies of it)
+      for (int i = 0; i < 16 / AT_ONCE; ++i) {
+        const int r = min(warp * 16 + i * AT_ONCE + lane / LANES, count - 1);  // (rows behind the last one are nobody's: copies of it)
         const int token = sm.row_token[r], head = kv_head * rows.group + row0 + r - (token - request.first) * rows.group;
-        const __nv_bfloat16* from = q + (size_t)token * q_stride + (size_t)head * D + lane * PER_LANE;
-        if (PER_LANE == 4) x[i] = __ldcg(reinterpret_cast<const uint2*>(from));
-        else x[i] = make_uint2(__ldcg(reinterpret_cast<const unsigned int*>(from)), 0u);
+        const __nv_bfloat16* from = q + (size_t)token * q_stride + (size_t)head * D + lane % LANES * 8;
+        x[i][0] = __ldcg(reinterpret_cast<const uint2*>(from));
+        x[i][1] = __ldcg(reinterpret_cast<const uint2*>(from + 4));
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = warp * 16 + i;
-        uint32_t a = x[i].x, b = x[i].y;
+      for (int i = 0; i < 16 / AT_ONCE; ++i) {
+        const int r = warp * 16 + i * AT_ONCE + lane / LANES;
+        uint32_t w[4] = {x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y};
         if (E4M3) {  // times a power of two that brings the row's largest element to [1, 2): float16 then holds it
-          const float f[4] = {__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)};
-          const float most = warp_max(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))));
+          float most = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
+#pragma unroll
+          for (int d = LANES / 2; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
           const int exponent = most > 0.f ? min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126) : 0;
           const float down = __uint_as_float((uint32_t)(127 - exponent) << 23);
-          const __half2 lo = __floats2half2_rn(f[0] * down, f[1] * down), hi = __floats2half2_rn(f[2] * down, f[3] * down);
-          a = *reinterpret_cast<const uint32_t*>(&lo);
-          b = *reinterpret_cast<const uint32_t*>(&hi);
-          if (lane == 0) sm.q_times[r] = __uint_as_float((uint32_t)(127 + exponent) << 23) * unit_times;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const __half2 pair = __floats2half2_rn(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xffff0000u) * down);
+            w[e] = *reinterpret_cast<const uint32_t*>(&pair);
+          }
+          if (lane % LANES == 0) sm.q_times[r] = __uint_as_float((uint32_t)(127 + exponent) << 23) * unit_times;
         }
-        const uint32_t at = smem_u32(sm.q) + tree_offset(r, lane * PER_LANE / 8) + (lane * PER_LANE % 8) * 2;
-        if (PER_LANE == 4) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
-        else asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(a) : "memory");
+        store_shared16(smem_u32(sm.q) + tree_offset(r, lane % LANES), w[0], w[1], w[2], w[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -782,7 +790,8 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
           f[u] = sm.row_out[u][r] == -INFINITY ? sum - sum : exp2_approx(sm.row_out[u][r] - at_most);
         }
         const bool alone = parts.splits == 1, live = r < count;
-        const int token = max(sm.row_token[r], 0), head = kv_head * rows.group + (row0 + r) % rows.group;
+        // (rows behind the last one: nobody's, and not written)
+        const int token = live ? sm.row_token[r] : request.first, head = live ? kv_head * rows.group + row0 + r - (token - request.first) * rows.group : 0;
         float inv = 1.f;
         if (alone && live) inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
         const float f0 = f[0] * inv, f1 = f[1] * inv;
