@@ -225,6 +225,29 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
 
   const int split = blockIdx.z;
   const int tiles = gridDim.x / cache.num_kv_heads, kv_head = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+  if (warp == kTreeLoadWarp) {  // (a thousand cycles, while the others wait for the request)
+    if (lane == 0) {
+      mbar_init(&sm.q_full, kTreeMmaWarp);
+      sm.failed = 0;
+      sm.bad = 0;
+    }
+    if (lane < kTreeKStages) {
+      mbar_init(&sm.k_full[lane], kTreeLoaders);
+      mbar_init(&sm.k_empty[lane], 1);
+      mbar_init(&sm.k_landed[lane], 1);
+    }
+    if (lane < kTreeVStages) {
+      mbar_init(&sm.v_full[lane], kTreeLoaders);
+      mbar_init(&sm.v_empty[lane], 1);
+      mbar_init(&sm.v_landed[lane], 1);
+    }
+    if (lane < kTreeScaleSlots) mbar_init(&sm.scale_full[lane], kTreeLoaders);
+    if (lane < 2) {
+      mbar_init(&sm.s_full[lane], 1);
+      mbar_init(&sm.pv_done[lane], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   const Request request = request_of(rows, blockIdx.y);
   const int row0 = tile * kTreeRows, count = min(kTreeRows, request.nodes * rows.group - row0);
   if (count <= 0) return;
@@ -279,33 +302,9 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
     return;
   }
 
-  // Four jobs at once: barriers, tensor memory, what is known of the rows, page ids (they wait for one load each).
-  if (warp == 0) {
-    if (lane == 0) {
-      mbar_init(&sm.q_full, kTreeMmaWarp);
-      mbar_init(&sm.merge_ready, 2 * active);
-      sm.failed = 0;
-      sm.bad = 0;
-    }
-    if (lane < kTreeKStages) {
-      mbar_init(&sm.k_full[lane], kTreeLoaders);
-      mbar_init(&sm.k_empty[lane], 1);
-      mbar_init(&sm.k_landed[lane], 1);
-    }
-    if (lane < kTreeVStages) {
-      mbar_init(&sm.v_full[lane], kTreeLoaders);
-      mbar_init(&sm.v_empty[lane], 1);
-      mbar_init(&sm.v_landed[lane], 1);
-    }
-    if (lane < kTreeScaleSlots) mbar_init(&sm.scale_full[lane], kTreeLoaders);
-    if (lane < 2) {
-      mbar_init(&sm.s_full[lane], 1);
-      mbar_init(&sm.p_full[0][lane], active);
-      mbar_init(&sm.p_full[1][lane], active);
-      mbar_init(&sm.pv_done[lane], 1);
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
+  // Three jobs at once: tensor memory, what is known of the rows, page ids (they wait for one load each).
+  if (warp == 0 && lane < 4) mbar_init(&sm.p_full[lane >> 1][lane & 1], active);
+  if (warp == 0 && lane == 0) mbar_init(&sm.merge_ready, 2 * active);
   if (warp == kTreeMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -350,9 +349,9 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
       uint64_t* landed = is_k ? sm.k_landed : sm.v_landed;
       const CUtensorMap* map = is_k ? &map_k : &map_v;
       const unsigned char* rows_at = reinterpret_cast<const unsigned char*>(is_k ? cache.k : cache.v);
-      int requested = 0;
+      int requested = 0, stage = 0, turn = 0;
       for (; requested < blocks; ++requested) {
-        const int j = block0 + requested, stage = requested % stages;
+        const int j = block0 + requested;
         const int key0 = span.key0(j), end = min(key0 + kTreeKeys, span.key_end(j));
         const int first_column = cache.column_of(key0), last_column = end > key0 ? cache.column_of(end - 1) : first_column - 1;
         unsigned char* tile_at = (is_k ? sm.k[0] : sm.v[0]) + (size_t)stage * kTreeKeys * D * 2;
@@ -375,7 +374,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
             }
           }
           const int bytes = __reduce_add_sync(0xffffffffu, direct ? (to > from ? cache.page_size : 0) : to - from) * BYTES;
-          if (!waited && !wait(&empty[stage], ((requested / stages) & 1) ^ 1)) { ok = false; break; }
+          if (!waited && !wait(&empty[stage], turn ^ 1)) { ok = false; break; }
           waited = true;
           if (lane == 0) {
             if (round + 32 > last_column) mbar_expect_tx(&landed[stage], bytes);
@@ -402,6 +401,10 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
           __syncwarp();
         }
         if (!ok) break;
+        if (++stage == stages) {
+          stage = 0;
+          turn ^= 1;
+        }
       }
       // Copies still on their way must land before the CTA may leave.
       for (int i = max(0, requested - stages); !ok && i < requested; ++i) mbar_wait(&landed[i % stages], (i / stages) & 1);
