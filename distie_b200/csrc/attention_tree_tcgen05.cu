@@ -29,9 +29,9 @@
 // then O, and what P of the block is there already, are read, scaled and written back.  The maxima are whole numbers (rounded down), so
 // that scaling is exact.
 //
-// What bounds it: the softmax warps.  Two trees of 64 new tokens over 16,001 keys (40 heads of 128, 8 key heads, bfloat16): 72 us
-// with the joining kernel, 144 CTAs of 44 blocks at 2,300 cycles a block, of which the products take 1,050 and each
-// scheduler's 128 exponentials 1,024; over an 8-bit cache 98 us, 3,400 cycles a block (scales read and multiplied, weights summed
+// What bounds it: the softmax warps.  Two trees of 64 new tokens over 16,001 keys (40 heads of 128, 8 key heads, bfloat16): 68 us
+// with the joining kernel, 144 CTAs of 44 blocks at 2,200 cycles a block, of which the products take 1,050 and each
+// scheduler's 128 exponentials 1,024; over an 8-bit cache 96 us, 3,400 cycles a block (scales read and multiplied, weights summed
 // once more for their limit).  Registers decide: 15 warps have 128 each, and a version that keeps 64 scores a thread spills.
 // With several shares of the keys, the parts go to scratch in float32 and attention_rows.cu joins them.
 //
