@@ -18,6 +18,8 @@ constexpr int kRowsKeys = 32;
 constexpr int kRowsThreads = 128;
 constexpr int kRowsMostDim = 256;
 
+__host__ __device__ constexpr int rows_k_pitch(int dim) { return dim % 4 == 0 ? dim + 4 : dim + 1; }
+
 template <typename T, int CACHE>
 __global__ void __launch_bounds__(kRowsThreads)
 attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int out_stride, QueryRows rows, CachePages cache,
@@ -25,12 +27,13 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   extern __shared__ __align__(16) float dyn[];
   const int dim = cache.key_dim, vdim = cache.value_dim;
   float* q_s = dyn;                                 // [16][dim]
-  float* k_s = q_s + kRowsTile * dim;               // [32][dim + 1]
-  float* v_s = k_s + kRowsKeys * (dim + 1);         // [32][vdim]
-  __shared__ float p_s[kRowsKeys][kRowsTile + 4];   // weights, a key's rows side by side
+  const int k_pitch = rows_k_pitch(dim);            // (free of bank conflicts, by one element or by four a lane)
+  float* k_s = q_s + kRowsTile * dim;               // [32][k_pitch]
+  float* v_s = k_s + kRowsKeys * k_pitch;           // [32][vdim]
+  __shared__ alignas(16) float p_s[kRowsKeys][kRowsTile + 4];   // weights, a key's rows side by side
   __shared__ float corr_s[kRowsTile], m_s[kRowsTile], l_s[kRowsTile];
   __shared__ int bad_s;                             // a value of this tile is not finite
-  __shared__ int first_s[kRowsTile];                // a row's oldest visible key
+  __shared__ int first_s[kRowsTile], token_s[kRowsTile], head_s[kRowsTile];  // a row's oldest visible key, its token and head
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.y, split = blockIdx.z;
   const Request request = request_of(rows, b);
@@ -40,22 +43,19 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   const int count = min(kRowsTile, all_rows - row0);
   const int* table = cache.block_table + (size_t)request.seat * cache.table_width;
 
-  for (int i = threadIdx.x; i < kRowsTile * dim; i += kRowsThreads) {
-    const int r = i / dim, e = i % dim;
-    float x = 0.f;
-    if (r < count) {
-      const int token = request.first + (row0 + r) / rows.group, head = kv_head * rows.group + (row0 + r) % rows.group;
-      x = to_float(q[(size_t)token * q_stride + (size_t)head * dim + e]);
-    }
-    q_s[i] = x;
-  }
-  if (threadIdx.x < kRowsTile) {
-    m_s[threadIdx.x] = -INFINITY;
-    l_s[threadIdx.x] = 0.f;
-    const int token = request.first + (row0 + min((int)threadIdx.x, count - 1)) / rows.group;
+  if (threadIdx.x < kRowsTile) {  // (rows behind the last one are nobody's: copies of it, never written)
+    const int row = row0 + min((int)threadIdx.x, count - 1), node = row / rows.group, token = request.first + node;
+    token_s[threadIdx.x] = token;
+    head_s[threadIdx.x] = kv_head * rows.group + row - node * rows.group;
     first_s[threadIdx.x] = first_visible_key(rows.positions[token], rows.window, rows.chunk);
   }
   __syncthreads();
+  for (int e = lane; e < dim; e += 32)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = warp * 4 + u;
+      q_s[r * dim + e] = to_float(q[(size_t)token_s[r] * q_stride + (size_t)head_s[r] * dim + e]);
+    }
   // The oldest cached key that any row of the tile sees inside its window (all new tokens' keys are walked); the keys
   // before it are walked up to keep_first only.
   int oldest = request.past;
@@ -69,9 +69,18 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   const int share = (tiles + parts.splits - 1) / parts.splits;
   const int tile_end = min(tiles, (split + 1) * share);
 
-  float acc[kRowsTile][2];
+  // A warp keeps the maxima and sums of its four rows; of the sums of values a thread keeps a column of all 16 rows (two of
+  // values beyond 128), of 8 with up to 64 columns, of 4 with up to 32.
+  float m_mine[4], l_mine[4], acc[kRowsTile][2];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    m_mine[u] = -INFINITY;
+    l_mine[u] = 0.f;
+  }
 #pragma unroll
   for (int r = 0; r < kRowsTile; ++r) acc[r][0] = acc[r][1] = 0.f;
+  const int row_parts = vdim <= 32 ? 4 : vdim <= 64 ? 2 : 1, part_rows = kRowsTile / row_parts, part_threads = kRowsThreads / row_parts;
+  const int column = threadIdx.x & (part_threads - 1), row_first = threadIdx.x / part_threads * part_rows;
 
   for (int j = split * share; j < tile_end; ++j) {
     const int key0 = j < kept_tiles ? j * kRowsKeys : start + (j - kept_tiles) * kRowsKeys;
@@ -117,7 +126,7 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
       for (int i = 0; i < MINE; ++i) {
         const int r = warp * MINE + i;
         const bool live = (there >> r) & 1;
-        if (e < dim) k_s[r * (dim + 1) + e] = live ? kx[i] * ks[i] : 0.f;
+        if (e < dim) k_s[r * k_pitch + e] = live ? kx[i] * ks[i] : 0.f;
         if (e < vdim) {
           const float x = live ? vx[i] * vs[i] : 0.f;
           bad |= !(fabsf(x) <= 3.402823466e38f);
@@ -129,77 +138,109 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
     __syncthreads();
     {  // scores: key `lane`, rows 4 warp .. 4 warp + 3; then their softmax statistics over the warp
       float dot[4] = {0.f, 0.f, 0.f, 0.f};
-      const float* k_row = k_s + lane * (dim + 1);
+      const float* k_row = k_s + lane * k_pitch;
       const float* q_row = q_s + warp * 4 * dim;
-      for (int e = 0; e < dim; ++e) {
-        const float x = k_row[e];
+      if (dim % 4 == 0) {
+#pragma unroll 4
+        for (int e = 0; e < dim; e += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(k_row + e);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) dot[u] += x * q_row[u * dim + e];
+          for (int u = 0; u < 4; ++u) {
+            const float4 y = *reinterpret_cast<const float4*>(q_row + u * dim + e);
+            dot[u] += x.x * y.x;
+            dot[u] += x.y * y.y;
+            dot[u] += x.z * y.z;
+            dot[u] += x.w * y.w;
+          }
+        }
+      } else {
+        for (int e = 0; e < dim; ++e) {
+          const float x = k_row[e];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) dot[u] += x * q_row[u * dim + e];
+        }
       }
+      float x[4], most[4], p[4], sum[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int r = warp * 4 + u;
         bool seen = r < count && at >= 0 && (key_position >= first_s[r] || key_position < rows.keep_first);
-        if (seen && key >= request.past) seen = mask_bit(rows, request.first + (row0 + r) / rows.group, key - request.past);
-        const float x = seen ? score_log2(dot[u], rows) : -INFINITY;
-        const float m_old = m_s[r];
-        const float m_new = fmaxf(m_old, warp_max(x));
-        const float p = x == -INFINITY ? 0.f : exp2f(x - m_new);
-        const float corr = m_old == -INFINITY ? 0.f : exp2f(m_old - m_new);
-        const float sum = warp_sum(p);
-        p_s[lane][r] = p;
-        __syncwarp();
-        if (lane == 0) {
-          l_s[r] = l_s[r] * corr + sum;
-          m_s[r] = m_new;
-          corr_s[r] = corr;
-        }
+        if (seen && key >= request.past) seen = mask_bit(rows, token_s[r], key - request.past);
+        x[u] = most[u] = seen ? score_log2(dot[u], rows) : -INFINITY;
       }
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1)  // (the four rows' chains side by side)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) most[u] = fmaxf(most[u], __shfl_xor_sync(0xffffffffu, most[u], d));
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float m_old = m_mine[u], m_new = fmaxf(m_old, most[u]), corr = m_old == -INFINITY ? 0.f : exp2f(m_old - m_new);
+        p[u] = sum[u] = x[u] == -INFINITY ? 0.f : exp2f(x[u] - m_new);
+        m_mine[u] = m_new;
+        l_mine[u] *= corr;
+        if (lane == 0) corr_s[warp * 4 + u] = corr;
+      }
+      *reinterpret_cast<float4*>(&p_s[lane][warp * 4]) = make_float4(p[0], p[1], p[2], p[3]);
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], d);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) l_mine[u] += sum[u];
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int e = threadIdx.x + i * kRowsThreads;
+      const int e = column + i * kRowsThreads;
       if (e < vdim) {
 #pragma unroll
-        for (int r = 0; r < kRowsTile; ++r) acc[r][i] *= corr_s[r];
+        for (int r = 0; r < kRowsTile; ++r)
+          if (r < part_rows) acc[r][i] *= corr_s[row_first + r];
         if (!bad_s) {
-          for (int key = 0; key < kRowsKeys; ++key) {
-            const float v = v_s[key * vdim + e];
+#pragma unroll 8
+          for (int j = 0; j < kRowsKeys; ++j) {
+            const float v = v_s[j * vdim + e];
 #pragma unroll
             for (int r = 0; r < kRowsTile; r += 4) {
-              const float4 p = *reinterpret_cast<const float4*>(&p_s[key][r]);
-              acc[r][i] += p.x * v;
-              acc[r + 1][i] += p.y * v;
-              acc[r + 2][i] += p.z * v;
-              acc[r + 3][i] += p.w * v;
+              if (r >= part_rows) break;
+              const float4 w = *reinterpret_cast<const float4*>(&p_s[j][row_first + r]);
+              acc[r][i] += w.x * v;
+              acc[r + 1][i] += w.y * v;
+              acc[r + 2][i] += w.z * v;
+              acc[r + 3][i] += w.w * v;
             }
           }
         } else {  // 0 * NaN is not 0: a value that is not finite reaches the rows that see it alone
-          for (int key = 0; key < kRowsKeys; ++key) {
-            const float v = v_s[key * vdim + e];
+          for (int j = 0; j < kRowsKeys; ++j) {
+            const float v = v_s[j * vdim + e];
 #pragma unroll
-            for (int r = 0; r < kRowsTile; ++r) acc[r][i] += p_s[key][r] != 0.f ? p_s[key][r] * v : 0.f;
+            for (int r = 0; r < kRowsTile; ++r)
+              if (r < part_rows) acc[r][i] += p_s[j][row_first + r] != 0.f ? p_s[j][row_first + r] * v : 0.f;
           }
         }
       }
     }
   }
+  if (lane < 4) {
+    m_s[warp * 4 + lane] = lane == 0 ? m_mine[0] : lane == 1 ? m_mine[1] : lane == 2 ? m_mine[2] : m_mine[3];
+    l_s[warp * 4 + lane] = lane == 0 ? l_mine[0] : lane == 1 ? l_mine[1] : lane == 2 ? l_mine[2] : l_mine[3];
+  }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int e = threadIdx.x + i * kRowsThreads;
+    const int e = column + i * kRowsThreads;
     if (e >= vdim) continue;
 #pragma unroll
-    for (int r = 0; r < kRowsTile; ++r) {
-      if (r >= count) break;
-      const int token = request.first + (row0 + r) / rows.group, head = kv_head * rows.group + (row0 + r) % rows.group;
+    for (int x = 0; x < kRowsTile; ++x) {
+      const int r = row_first + x;
+      if (x >= part_rows || r >= count) break;
+      const int token = token_s[r], head = head_s[r];
       if (parts.splits == 1) {
         const float inv = rows.extras.sink ? sink_inverse_log2(m_s[r], l_s[r], rows.extras.sink[head]) : (l_s[r] == 0.f ? 0.f : 1.f / l_s[r]);
-        out[(size_t)token * out_stride + (size_t)head * vdim + e] = from_float<T>(acc[r][i] * inv);
+        out[(size_t)token * out_stride + (size_t)head * vdim + e] = from_float<T>(acc[x][i] * inv);
       } else {
         const size_t row = ((size_t)token * rows.num_heads + head) * parts.splits + split;
-        parts.o[row * vdim + e] = acc[r][i];
+        parts.o[row * vdim + e] = acc[x][i];
         if (e == 0) {
           parts.ml[row * 2] = m_s[r];
           parts.ml[row * 2 + 1] = l_s[r];
@@ -353,7 +394,7 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
   const Partials parts{scratch, scratch ? scratch + (size_t)tokens * num_heads * splits * value_dim : nullptr, splits};
   const int tiles = (most_nodes * rows.group + kRowsTile - 1) / kRowsTile;
   const dim3 grid(tiles * num_kv_heads, requests, splits);
-  const size_t shared = ((size_t)kRowsTile * key_dim + (size_t)kRowsKeys * (key_dim + 1 + value_dim)) * sizeof(float);
+  const size_t shared = ((size_t)kRowsTile * key_dim + (size_t)kRowsKeys * (rows_k_pitch(key_dim) + value_dim)) * sizeof(float);
   cudaError_t err;
 #define DISTIE_ROWS(T, CACHE)                                                                                                       \
   {                                                                                                                                 \
