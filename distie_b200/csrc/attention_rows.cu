@@ -16,9 +16,41 @@ namespace distie {
 constexpr int kRowsTile = 16;
 constexpr int kRowsKeys = 32;
 constexpr int kRowsThreads = 128;
+constexpr int kRowsPitch = kRowsTile + 4;  // of a key's weights in shared memory
 constexpr int kRowsMostDim = 256;
 
 __host__ __device__ constexpr int rows_k_pitch(int dim) { return dim % 4 == 0 ? dim + 4 : dim + 1; }
+
+// The sums of a column of values of ROWS rows (acc[..][i]), scaled down by `corr`, and a tile's weights times values joined to them.
+template <int ROWS>
+__device__ __forceinline__ void add_values(float (&acc)[kRowsTile][2], int i, const float* corr, const float* weights, const float* values,
+                                           int vdim, int bad) {
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) acc[r][i] *= corr[r];
+  if (!bad) {
+#pragma unroll 8
+    for (int j = 0; j < kRowsKeys; ++j) {
+      const float v = values[j * vdim];
+#pragma unroll
+      for (int r = 0; r < ROWS; r += 4) {
+        const float4 w = *reinterpret_cast<const float4*>(weights + j * kRowsPitch + r);
+        acc[r][i] += w.x * v;
+        acc[r + 1][i] += w.y * v;
+        acc[r + 2][i] += w.z * v;
+        acc[r + 3][i] += w.w * v;
+      }
+    }
+  } else {  // 0 * NaN is not 0: a value that is not finite reaches the rows that see it alone
+    for (int j = 0; j < kRowsKeys; ++j) {
+      const float v = values[j * vdim];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const float w = weights[j * kRowsPitch + r];
+        acc[r][i] += w != 0.f ? w * v : 0.f;
+      }
+    }
+  }
+}
 
 template <typename T, int CACHE>
 __global__ void __launch_bounds__(kRowsThreads)
@@ -30,7 +62,7 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   const int k_pitch = rows_k_pitch(dim);            // (free of bank conflicts, by one element or by four a lane)
   float* k_s = q_s + kRowsTile * dim;               // [32][k_pitch]
   float* v_s = k_s + kRowsKeys * k_pitch;           // [32][vdim]
-  __shared__ alignas(16) float p_s[kRowsKeys][kRowsTile + 4];   // weights, a key's rows side by side
+  __shared__ alignas(16) float p_s[kRowsKeys][kRowsPitch];   // weights, a key's rows side by side
   __shared__ float corr_s[kRowsTile], m_s[kRowsTile], l_s[kRowsTile];
   __shared__ int bad_s;                             // a value of this tile is not finite
   __shared__ int first_s[kRowsTile], token_s[kRowsTile], head_s[kRowsTile];  // a row's oldest visible key, its token and head
@@ -106,11 +138,13 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
     }
     constexpr int MINE = kRowsKeys / (kRowsThreads / 32);
     const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
-    long long from[MINE];
+    const long long k_at = max(at, 0ll) * dim, v_at = max(at, 0ll) * vdim;
+    long long k_from[MINE], v_from[MINE];
     float ks[MINE], vs[MINE];
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-      from[i] = max(__shfl_sync(0xffffffffu, at, warp * MINE + i), 0ll);
+      k_from[i] = __shfl_sync(0xffffffffu, k_at, warp * MINE + i);
+      v_from[i] = __shfl_sync(0xffffffffu, v_at, warp * MINE + i);
       ks[i] = __shfl_sync(0xffffffffu, k_scale, warp * MINE + i);
       vs[i] = __shfl_sync(0xffffffffu, v_scale, warp * MINE + i);
     }
@@ -119,8 +153,8 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
       float kx[MINE], vx[MINE];
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
-        kx[i] = cached_value<CACHE>(cache.k, (size_t)from[i] * dim + min(e, dim - 1));
-        vx[i] = cached_value<CACHE>(cache.v, (size_t)from[i] * vdim + min(e, vdim - 1));
+        kx[i] = cached_value<CACHE>(cache.k, (size_t)k_from[i] + min(e, dim - 1));
+        vx[i] = cached_value<CACHE>(cache.v, (size_t)v_from[i] + min(e, vdim - 1));
       }
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
@@ -193,31 +227,10 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
     for (int i = 0; i < 2; ++i) {
       const int e = column + i * kRowsThreads;
       if (e < vdim) {
-#pragma unroll
-        for (int r = 0; r < kRowsTile; ++r)
-          if (r < part_rows) acc[r][i] *= corr_s[row_first + r];
-        if (!bad_s) {
-#pragma unroll 8
-          for (int j = 0; j < kRowsKeys; ++j) {
-            const float v = v_s[j * vdim + e];
-#pragma unroll
-            for (int r = 0; r < kRowsTile; r += 4) {
-              if (r >= part_rows) break;
-              const float4 w = *reinterpret_cast<const float4*>(&p_s[j][row_first + r]);
-              acc[r][i] += w.x * v;
-              acc[r + 1][i] += w.y * v;
-              acc[r + 2][i] += w.z * v;
-              acc[r + 3][i] += w.w * v;
-            }
-          }
-        } else {  // 0 * NaN is not 0: a value that is not finite reaches the rows that see it alone
-          for (int j = 0; j < kRowsKeys; ++j) {
-            const float v = v_s[j * vdim + e];
-#pragma unroll
-            for (int r = 0; r < kRowsTile; ++r)
-              if (r < part_rows) acc[r][i] += p_s[j][row_first + r] != 0.f ? p_s[j][row_first + r] * v : 0.f;
-          }
-        }
+        const float* weights = &p_s[0][row_first];
+        if (part_rows == 4) add_values<4>(acc, i, corr_s + row_first, weights, v_s + e, vdim, bad_s);
+        else if (part_rows == 8) add_values<8>(acc, i, corr_s + row_first, weights, v_s + e, vdim, bad_s);
+        else add_values<16>(acc, i, corr_s + row_first, weights, v_s + e, vdim, bad_s);
       }
     }
   }
