@@ -6,6 +6,11 @@
 // into shared memory as float32 once for all rows, a thread makes the scores of one key with four rows, a warp the softmax
 // statistics of four rows (running maximum and sum), a thread the output columns of all rows.  With few rows the reads
 // of the cache bound it; keys are then split over blocks and the parts merged.
+//
+// What bounds it is latency: a block alone takes about 5,000 cycles a tile of 32 keys (its rows found 600, their loads 2,000,
+// scores 800, weights 1,200, sums 600; 8,000 before loads, reductions and sums were laid side by side).  So registers go to loads
+// in flight, two blocks an SM.  Two trees of 13 new tokens over 500 keys, 80 tiles of rows, heads of 32 in float32: 23 us with
+// the joining kernel; over 5,000 keys 119.
 #include <cuda_fp16.h>
 
 #include "cached_rows.cuh"
@@ -53,7 +58,7 @@ __device__ __forceinline__ void add_values(float (&acc)[kRowsTile][2], int i, co
 }
 
 template <typename T, int CACHE>
-__global__ void __launch_bounds__(kRowsThreads)
+__global__ void __launch_bounds__(kRowsThreads, 2)
 attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out, int out_stride, QueryRows rows, CachePages cache,
                       Partials parts, int* __restrict__ error) {
   extern __shared__ __align__(16) float dyn[];
@@ -66,6 +71,7 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   __shared__ float corr_s[kRowsTile], m_s[kRowsTile], l_s[kRowsTile];
   __shared__ int bad_s;                             // a value of this tile is not finite
   __shared__ int first_s[kRowsTile], token_s[kRowsTile], head_s[kRowsTile];  // a row's oldest visible key, its token and head
+  grid_dependency_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.y, split = blockIdx.z;
   const Request request = request_of(rows, b);
@@ -82,11 +88,12 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
     first_s[threadIdx.x] = first_visible_key(rows.positions[token], rows.window, rows.chunk);
   }
   __syncthreads();
+  grid_dependency_wait();  // q and the newest rows come from the kernels before this one
   for (int e = lane; e < dim; e += 32)
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int r = warp * 4 + u;
-      q_s[r * dim + e] = to_float(q[(size_t)token_s[r] * q_stride + (size_t)head_s[r] * dim + e]);
+      q_s[r * dim + e] = value_cg<sizeof(T) == 4 ? DISTIE_F32 : DISTIE_BF16>(q, (size_t)token_s[r] * q_stride + (size_t)head_s[r] * dim + e);
     }
   // The oldest cached key that any row of the tile sees inside its window (all new tokens' keys are walked); the keys
   // before it are walked up to keep_first only.
@@ -133,18 +140,16 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
     if (rows.seqs && key >= request.past && key < keys) key_position = rows.positions[request.first + key - request.past];
     float k_scale = 1.f, v_scale = 1.f;
     if (CACHE == DISTIE_E4M3) {
-      k_scale = cache.k_scale[max(at, 0ll)];
-      v_scale = cache.v_scale[max(at, 0ll)];
+      k_scale = __ldcg(cache.k_scale + max(at, 0ll));
+      v_scale = __ldcg(cache.v_scale + max(at, 0ll));
     }
     constexpr int MINE = kRowsKeys / (kRowsThreads / 32);
     const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
-    const long long k_at = max(at, 0ll) * dim, v_at = max(at, 0ll) * vdim;
-    long long k_from[MINE], v_from[MINE];
+    uint32_t from[MINE];  // (a cache has fewer than 2^32 rows)
     float ks[MINE], vs[MINE];
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-      k_from[i] = __shfl_sync(0xffffffffu, k_at, warp * MINE + i);
-      v_from[i] = __shfl_sync(0xffffffffu, v_at, warp * MINE + i);
+      from[i] = __shfl_sync(0xffffffffu, (uint32_t)max(at, 0ll), warp * MINE + i);
       ks[i] = __shfl_sync(0xffffffffu, k_scale, warp * MINE + i);
       vs[i] = __shfl_sync(0xffffffffu, v_scale, warp * MINE + i);
     }
@@ -153,8 +158,8 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
       float kx[MINE], vx[MINE];
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
-        kx[i] = cached_value<CACHE>(cache.k, (size_t)k_from[i] + min(e, dim - 1));
-        vx[i] = cached_value<CACHE>(cache.v, (size_t)v_from[i] + min(e, vdim - 1));
+        kx[i] = value_cg<CACHE>(cache.k, (size_t)from[i] * (uint32_t)dim + min(e, dim - 1));
+        vx[i] = value_cg<CACHE>(cache.v, (size_t)from[i] * (uint32_t)vdim + min(e, vdim - 1));
       }
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
@@ -400,6 +405,7 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
       splits > 65535 || requests > 65535 || num_heads > 65535 || (splits > 1 && scratch == nullptr) || (seqs != nullptr && bits == nullptr) ||
       (cache_type == DISTIE_E4M3 && (k_scale == nullptr || v_scale == nullptr)))
     return DISTIE_ERR_ARG;
+  if ((long long)num_pages * num_kv_heads * page_size > 0xffffffffLL) return DISTIE_ERR_UNSUPPORTED;
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, key_dim, value_dim,
                                       page_size, num_pages);
   const QueryRows rows{positions, token_seq, seq_seat, seqs, bits, words, tokens, num_heads / num_kv_heads, num_heads, window, chunk, keep_first,
@@ -414,9 +420,9 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
     if (shared > 48 * 1024 && (err = cudaFuncSetAttribute(attention_rows_kernel<T, CACHE>,                                           \
                                                           cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024)) != cudaSuccess)  \
       return (int)err;                                                                                        \
-    attention_rows_kernel<T, CACHE><<<grid, kRowsThreads, shared, stream>>>((const T*)q, q_stride, (T*)out, out_stride, rows, cache,   \
-                                                                            parts, error);                                          \
-    DISTIE_LAUNCH_CHECK();                                                                                                          \
+    err = launch_dependent(attention_rows_kernel<T, CACHE>, grid, dim3(kRowsThreads), shared, stream, (const T*)q, q_stride, (T*)out,         \
+                           out_stride, rows, cache, parts, error);                                                                   \
+    if (err != cudaSuccess) return (int)err;                                                                                        \
     if (splits > 1) return rows_merge<T>(parts, out, out_stride, tokens, num_heads, value_dim, sink, stream);                          \
     return 0;                                                                                                                       \
   }

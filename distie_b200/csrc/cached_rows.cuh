@@ -115,12 +115,12 @@ __device__ __forceinline__ float e4m3_to_float(uint8_t x) {
   return __half2float(__low2half(*reinterpret_cast<const __half2*>(&h)));
 }
 
-// A cached element as a float32 number (CACHE: the cache's element type), without its row's scale.
-template <int CACHE>
-__device__ __forceinline__ float cached_value(const void* rows, size_t at) {
-  if (CACHE == DISTIE_E4M3) return e4m3_to_float(reinterpret_cast<const uint8_t*>(rows)[at]);
-  if (CACHE == DISTIE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(rows)[at]);
-  return reinterpret_cast<const float*>(rows)[at];
+// An element as a float32 number (TYPE: its type), without its row's scale; through L2, for kernels that start early.
+template <int TYPE>
+__device__ __forceinline__ float value_cg(const void* rows, size_t at) {
+  if (TYPE == DISTIE_E4M3) return e4m3_to_float(__ldcg(reinterpret_cast<const uint8_t*>(rows) + at));
+  if (TYPE == DISTIE_BF16) return __uint_as_float((uint32_t)__ldcg(reinterpret_cast<const unsigned short*>(rows) + at) << 16);
+  return __ldcg(reinterpret_cast<const float*>(rows) + at);
 }
 
 // The partial results of split key ranges: scratch holds o [tokens * heads * splits, value_dim] and behind it (maximum in

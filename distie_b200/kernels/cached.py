@@ -60,6 +60,20 @@ def decode_splits(blocks: int, keys: int, sms: int, wide: bool, many: bool) -> i
     return best
 
 
+@functools.lru_cache(maxsize=256)
+def rows_splits(blocks: int, keys: int, sms: int) -> int:
+    """Shares that the keys of ``blocks`` tiles of 16 rows are cut into (attention_rows.cu): the number for which whole waves of
+    blocks, two an SM, take the least time, a block that of its tiles of 32 keys and of one more for its start and end; joining
+    the parts takes another.  (80 blocks, heads of 32: over 500 keys 45 us with one share, 23 with 3, 25 with 7; over 5,000
+    356, 147 and 119.)"""
+    best, least = 1, None
+    for splits in range(1, max(1, min(keys // 64, 64)) + 1):
+        cost = -(-blocks * splits // (2 * sms)) * (-(-keys // (32 * splits)) + 1) + (1 if splits > 1 else 0)
+        if least is None or cost < least:
+            best, least = splits, cost
+    return best
+
+
 class CachedRows:
     caches_in_8_bits = True
     drafted_tokens = True
@@ -256,7 +270,7 @@ class CachedRows:
                                                    softcap, sink, tokens, requests, most):
             return
         blocks = requests * num_kv_heads * -(-most * group // 16)
-        splits = max(1, min(4 * self.sm_count // blocks, step.max_kv_len // 64, 64))
+        splits = rows_splits(blocks, step.max_kv_len, self.sm_count)
         scratch = self._parts(tokens, num_heads, value_dim, splits) if splits > 1 else None
         launch, pack = packed("distie_attention_rows")
         with self._here():

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from distie_b200.kernels import DraftTree, cached
-from distie_b200.kernels.cached import CachedRows, decode_splits, tree_splits
+from distie_b200.kernels.cached import CachedRows, decode_splits, rows_splits, tree_splits
 from distie_b200.kernels.interface import E4M3, KvSlot, RotaryTable, StepTensors
 from distie_b200.kernels.library import KernelError
 
@@ -197,6 +197,7 @@ def test_shares_of_the_keys():
             for wide in (False, True):
                 for many in (False, True):
                     assert 1 <= decode_splits(blocks, keys, 148, wide, many) <= max(1, min(64, keys // 256))
+            assert 1 <= rows_splits(blocks, keys, 148) <= max(1, min(64, keys // 64))
             assert 1 <= tree_splits(blocks, -(-keys // 128), 148) <= max(1, min(64, -(-keys // 128)))
 
 
