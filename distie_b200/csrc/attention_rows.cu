@@ -4,8 +4,8 @@
 // The rows of a request that share a kv head, (new token, query head of the group), are packed: row r is head r % group of
 // new token r / group.  A block takes up to 16 rows and walks its share of the keys in tiles of 32: keys and values come
 // into shared memory as float32 once for all rows, a thread makes the scores of one key with four rows, a warp the softmax
-// statistics of four rows (running maximum and sum), a thread the output columns of all rows.  With few rows the reads
-// of the cache bound it; keys are then split over blocks and the parts merged.
+// statistics of four rows (running maximum and sum), a thread a column of the sums of 4, 8 or 16 rows, so that all threads have
+// one.  Keys are split over blocks (rows_splits in kernels/cached.py) and the parts joined.
 //
 // What bounds it is latency: a block alone takes about 5,000 cycles a tile of 32 keys (its rows found 600, their loads 2,000,
 // scores 800, weights 1,200, sums 600; 8,000 before loads, reductions and sums were laid side by side).  So registers go to loads
