@@ -371,7 +371,7 @@ constexpr int kReadRows = 256, kReadFewRows = 8;  // (a launch copies the whole 
 template <int ROWS>
 struct ReadPlan {
   int count;
-  int batch_row[ROWS];    // of the step: its seat is read, and that seat's row of the result's table filled
+  int batch_row[ROWS];    // of the step: its seat is read
   int first_page[ROWS];   // pages of the result before this request's
   int first_column[ROWS]; // its first logical page that is read
   int hole[ROWS];         // logical pages hole .. hole_end - 1 are not read: a window has passed them
@@ -390,6 +390,21 @@ __device__ __forceinline__ void store_row16(T* to, const float (&v)[16]) {
   }
 }
 
+// The rows of the result's table that belong to the requests' seats.  The attention that follows starts early and looks at its
+// block table before it waits, as at an input of the step (common.cuh).  So this is a kernel of its own, launched the ordinary
+// way before the pages are read and releasing nobody: rows_read_kernel does not start before it has ended, and releases the
+// attention only once it has seen that.
+template <int ROWS>
+__global__ void __launch_bounds__(128)
+rows_table_kernel(const __grid_constant__ ReadPlan<ROWS> plan, const int* __restrict__ seq_seat, int page_size, int* __restrict__ table_out,
+                  int table_width) {
+  const int i = blockIdx.x, columns = (plan.length[i] + page_size - 1) / page_size;
+  int* row = table_out + (size_t)seq_seat[plan.batch_row[i]] * table_width;
+  for (int c = threadIdx.x; c < table_width; c += blockDim.x)
+    row[c] = c >= plan.first_column[i] && c < columns && (c < plan.hole[i] || c >= plan.hole_end[i])
+                 ? plan.first_page[i] + c - plan.first_column[i] : -1;
+}
+
 constexpr int kReadThreads = 256;
 constexpr int kReadPieces = 4;  // 16 numbers each, per thread: all requested before the first is stored
 
@@ -397,19 +412,7 @@ constexpr int kReadPieces = 4;  // 16 numbers each, per thread: all requested be
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(kReadThreads)
 rows_read_kernel(const __grid_constant__ ReadPlan<ROWS> plan, CachePages cache, const int* __restrict__ seq_seat, T* __restrict__ k_out,
-                 T* __restrict__ v_out, int* __restrict__ table_out, int page0, int pages, int* __restrict__ error) {
-  grid_dependency_release();
-  if ((int)blockIdx.x >= pages) {  // blocks behind the pages: a row of the result's table each
-    if (blockIdx.y > 0) return;
-    grid_dependency_wait();
-    const int i = blockIdx.x - pages;
-    const int columns = (plan.length[i] + cache.page_size - 1) / cache.page_size;
-    int* row = table_out + (size_t)seq_seat[plan.batch_row[i]] * cache.table_width;
-    for (int c = threadIdx.x; c < cache.table_width; c += blockDim.x)
-      row[c] = c >= plan.first_column[i] && c < columns && (c < plan.hole[i] || c >= plan.hole_end[i])
-                   ? plan.first_page[i] + c - plan.first_column[i] : -1;
-    return;
-  }
+                 T* __restrict__ v_out, int page0, int* __restrict__ error) {
   const int page_out = page0 + blockIdx.x;
   int i = 0;
   for (int step = ROWS / 2; step > 0; step >>= 1)
@@ -423,6 +426,7 @@ rows_read_kernel(const __grid_constant__ ReadPlan<ROWS> plan, CachePages cache, 
   const int rows = cache.num_kv_heads * cache.page_size;
   const size_t from = (size_t)(held ? page : 0) * rows, to = (size_t)page_out * rows;
   grid_dependency_wait();  // the newest rows come from the kernels before this one
+  grid_dependency_release();  // (not before the wait: see rows_table_kernel)
   if (!held && threadIdx.x == 0 && blockIdx.y == 0 && error) atomicExch(error, 5);
   auto live_row = [&](int row) { return (cache.page_shift >= 0 ? row & (cache.page_size - 1) : row % cache.page_size) < live; };
   if (((cache.key_dim | cache.value_dim) & 15) == 0) {
@@ -553,9 +557,8 @@ extern "C" int distie_rows_write(const void* q, int q_stride, const void* k, int
   return DISTIE_ERR_UNSUPPORTED;
 }
 
-template <typename T, int ROWS>
-static int launch_read(const int* plan, int count, const dim3& grid, const CachePages& cache, const int* seq_seat, void* k_out, void* v_out,
-                       int* table_out, int page0, int pages, int* error, cudaStream_t stream) {
+template <int ROWS>
+static ReadPlan<ROWS> read_plan(const int* plan, int count) {
   ReadPlan<ROWS> p;
   p.count = count;
   for (int i = 0; i < count; ++i) {
@@ -566,16 +569,25 @@ static int launch_read(const int* plan, int count, const dim3& grid, const Cache
     p.hole_end[i] = plan[6 * i + 4];
     p.length[i] = plan[6 * i + 5];
   }
-  return (int)launch_dependent(rows_read_kernel<T, ROWS>, grid, dim3(kReadThreads), 0, stream, p, cache, seq_seat, (T*)k_out, (T*)v_out, table_out,
-                               page0, pages, error);
+  return p;
+}
+
+template <typename T>
+static int launch_read(const int* plan, int count, const dim3& grid, const CachePages& cache, const int* seq_seat, void* k_out, void* v_out,
+                       int page0, int* error, cudaStream_t stream) {
+  if (count <= kReadFewRows)
+    return (int)launch_dependent(rows_read_kernel<T, kReadFewRows>, grid, dim3(kReadThreads), 0, stream, read_plan<kReadFewRows>(plan, count),
+                                 cache, seq_seat, (T*)k_out, (T*)v_out, page0, error);
+  return (int)launch_dependent(rows_read_kernel<T, kReadRows>, grid, dim3(kReadThreads), 0, stream, read_plan<kReadRows>(plan, count), cache,
+                               seq_seat, (T*)k_out, (T*)v_out, page0, error);
 }
 
 // plan: `count` rows (batch row, first page of the result, first logical page, hole, end of the hole, keys) on the host; their
-// pages of the result are page0 .. page0 + pages - 1.  table_out: of the shape of block_table.
+// pages of the result are page0 .. page0 + pages - 1.
 extern "C" int distie_rows_read(const int* plan, int count, const void* k_cache, const void* v_cache, const float* k_scale,
                                 const float* v_scale, const int* block_table, int table_width, const int* seq_seat, int num_kv_heads,
-                                int key_dim, int value_dim, int page_size, int num_pages, void* k_out, void* v_out, int* table_out,
-                                int page0, int pages, int out_type, int* error, cudaStream_t stream) {
+                                int key_dim, int value_dim, int page_size, int num_pages, void* k_out, void* v_out, int page0, int pages,
+                                int out_type, int* error, cudaStream_t stream) {
   if (count <= 0 || pages <= 0) return 0;
   if (count > kReadRows || num_kv_heads < 1 || key_dim < 1 || value_dim < 1 || page_size < 1 || table_width < 1 || k_scale == nullptr || v_scale == nullptr ||
       (long long)num_kv_heads * page_size * (key_dim + value_dim) > 1 << 30)
@@ -584,15 +596,26 @@ extern "C" int distie_rows_read(const int* plan, int count, const void* k_cache,
                                       page_size, num_pages);
   const long long pieces = (long long)num_kv_heads * page_size * (key_dim / 16 + value_dim / 16);
   const int per_block = kReadThreads * kReadPieces;
-  const dim3 grid(pages + count, ((key_dim | value_dim) & 15) == 0 ? (unsigned)((pieces + per_block - 1) / per_block) : 1);
+  const dim3 grid(pages, ((key_dim | value_dim) & 15) == 0 ? (unsigned)((pieces + per_block - 1) / per_block) : 1);
   if (out_type == DISTIE_BF16)
-    return count <= kReadFewRows ? launch_read<__nv_bfloat16, kReadFewRows>(plan, count, grid, cache, seq_seat, k_out, v_out, table_out, page0, pages, error, stream)
-                                 : launch_read<__nv_bfloat16, kReadRows>(plan, count, grid, cache, seq_seat, k_out, v_out, table_out, page0, pages, error, stream);
-  if (out_type == DISTIE_F32)
-    return count <= kReadFewRows ? launch_read<float, kReadFewRows>(plan, count, grid, cache, seq_seat, k_out, v_out, table_out, page0, pages, error, stream)
-                                 : launch_read<float, kReadRows>(plan, count, grid, cache, seq_seat, k_out, v_out, table_out, page0, pages, error, stream);
+    return launch_read<__nv_bfloat16>(plan, count, grid, cache, seq_seat, k_out, v_out, page0, error, stream);
+  if (out_type == DISTIE_F32) return launch_read<float>(plan, count, grid, cache, seq_seat, k_out, v_out, page0, error, stream);
   return DISTIE_ERR_UNSUPPORTED;
+}
+
+// Of the table [seats, table_width] of the pages read back, the rows of the plan's requests.
+extern "C" int distie_rows_table(const int* plan, int count, const int* seq_seat, int page_size, int* table_out, int table_width,
+                                 cudaStream_t stream) {
+  if (count <= 0) return 0;
+  if (count > kReadRows || page_size < 1 || table_width < 1) return DISTIE_ERR_ARG;
+  if (count <= kReadFewRows)
+    rows_table_kernel<kReadFewRows><<<count, 128, 0, stream>>>(read_plan<kReadFewRows>(plan, count), seq_seat, page_size, table_out, table_width);
+  else
+    rows_table_kernel<kReadRows><<<count, 128, 0, stream>>>(read_plan<kReadRows>(plan, count), seq_seat, page_size, table_out, table_width);
+  DISTIE_LAUNCH_CHECK();
+  return 0;
 }
 
 DISTIE_PACKED(distie_rows_write)
 DISTIE_PACKED(distie_rows_read)
+DISTIE_PACKED(distie_rows_table)

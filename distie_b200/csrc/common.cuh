@@ -230,7 +230,8 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
 
 // Programmatic dependent launch.  A kernel launched with `launch_dependent` may start while the
 // kernel before it in the stream is still running; it may read data that no kernel of the step
-// writes (weights, the step's index arrays, block tables) at once, and must call
+// writes (weights, the step's index arrays, block tables; the table of pages read back is made by a
+// launch that starts late and releases nobody: rows_table_kernel) at once, and must call
 // `grid_dependency_wait()` before it reads anything an earlier kernel produced and before it
 // writes global memory (a buffer it writes may still be read by an earlier kernel).  The wait
 // returns when all earlier kernels have finished and their writes are visible.  Calling

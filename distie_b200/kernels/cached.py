@@ -196,7 +196,7 @@ class CachedRows:
         else:
             k_out = torch.empty((total, num_kv_heads, page, key_dim), dtype=self.dtype, device=k.device)
             v_out = torch.empty((total, num_kv_heads, page, value_dim), dtype=self.dtype, device=k.device)
-        out = KvSlot(k_out, v_out, torch.empty_like(table), page, total)
+        out = KvSlot(k_out, v_out, self._read_table(step, table, page, plan, (int(window or 0), int(chunk or 0), int(keep_first or 0))), page, total)
         for numbers, count, first, size in plan:
             launch, pack = packed("distie_rows_read")
             with self._here():
@@ -204,8 +204,7 @@ class CachedRows:
                     launch(pack(
                         ctypes.addressof(numbers), count, k.data_ptr(), v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
                         table.data_ptr(), table.shape[1], step.seq_seat.data_ptr(), num_kv_heads, key_dim, value_dim, page, pages,
-                        k_out.data_ptr(), v_out.data_ptr(), out.block_table.data_ptr(), first, size,
-                        _CACHE_CODE[self.dtype], self.error_flag.data_ptr(), self._stream(),
+                        k_out.data_ptr(), v_out.data_ptr(), first, size, _CACHE_CODE[self.dtype], self.error_flag.data_ptr(), self._stream(),
                     )),
                     "rows_read",
                 )
@@ -235,6 +234,25 @@ class CachedRows:
                 numbers = (ctypes.c_int * (6 * len(part)))(*[n for entry in part for n in entry])
                 plan.append((numbers, len(part), part[0][1], end - part[0][1]))
             made = step.derived[key] = (plan, total)
+        return made
+
+    def _read_table(self, step, table, page: int, plan, what) -> torch.Tensor:
+        """The block table of the pages that ``plan`` reads back, made before any of them is read (csrc/cached_rows.cu says why) and kept
+        with the step for all layers of a kind.  Into a graph it is captured with every call: a replay may bring other seats."""
+        with self._here():
+            capturing = table.is_cuda and torch.cuda.is_current_stream_capturing()
+        key = ("read_table", page, *what, table.shape, self._stream())
+        made = None if capturing else step.derived.get(key)
+        if made is None:
+            made = torch.empty_like(table)
+            for numbers, count, _first, _size in plan:
+                launch, pack = packed("distie_rows_table")
+                with self._here():
+                    check(launch(pack(ctypes.addressof(numbers), count, step.seq_seat.data_ptr(), page, made.data_ptr(), table.shape[1],
+                                      self._stream())), "rows_table")
+                self._ran("rows_table")
+            if not capturing:
+                step.derived[key] = made
         return made
 
     # -- attention ------------------------------------------------------------------------------------------------

@@ -129,7 +129,8 @@ _SIGNATURES: dict[str, tuple[str, list]] = {
         "cached", [P, I, P, I, P, I, I, I, L, P, P, P, I, F, P, P, P, I, I, F, F, F, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I,
                    P, I, I, I, P, P]
     ),
-    "distie_rows_read": ("cached", [P, I, P, P, P, P, P, I, P, I, I, I, I, I, P, P, P, I, I, I, P, P]),
+    "distie_rows_read": ("cached", [P, I, P, P, P, P, P, I, P, I, I, I, I, I, P, P, I, I, I, P, P]),
+    "distie_rows_table": ("cached", [P, I, P, I, P, I, P]),
     "distie_attention_rows": (
         "cached", [P, I, P, I, P, P, P, P, P, P, I, I, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, F, F, P, I, I, I, P, P]
     ),
