@@ -32,6 +32,7 @@ struct RowsNorm {
 struct RowsTurn {
   const float* inv_freq;  // null: nothing is rotated
   int rotary_dim, interleaved;
+  int rounded;            // whether position * frequency is rounded to float32, as by the kernels for rows at their positions
   float factor;
   float temp_coef, temp_every;  // temp_every > 0: q at position p times 1 + coef ln(floor((p + 1) / every) + 1)
 };
@@ -42,10 +43,12 @@ struct RowsPlace {
   const int* seq_seat;
 };
 
-// cos and sin of position * frequency as the exact product: the product's rounding error, up to 2^-24 of an angle of many
-// turns, comes back as a small rotation.  (A float32 product alone is off by 4e-3 at position 65,536.)
-__device__ __forceinline__ void exact_angle(int position, float frequency, float& sn, float& cs) {
-  const float p = (float)position, high = __fmul_rn(p, frequency), low = __fmaf_rn(p, frequency, -high);
+// cos and sin of position * frequency: of the float32 product (`rounded`), as the rotations of all other steps and of the
+// checkpoints' own code take it, so that rows of drafted tokens fit the rows they stand beside; or of the exact product.  There
+// the product's rounding error e, up to 2^-24 of an angle of many turns, comes back as a small rotation, without its terms from
+// e^3 / 6 on: 8e-8 up to position 2^18.  (A float32 product alone is off by 4e-3 at position 65,536.)
+__device__ __forceinline__ void turn_angle(int position, float frequency, int rounded, float& sn, float& cs) {
+  const float p = (float)position, high = __fmul_rn(p, frequency), low = rounded ? 0.f : __fmaf_rn(p, frequency, -high);
   float s, c;
   sincosf(high, &s, &c);
   const float half = 0.5f * low * low;
@@ -82,7 +85,7 @@ rows_write_kernel(RowsInput in, RowsNorm norm, RowsTurn turn, RowsPlace place, T
   const int position = place.positions[t];
   for (int i = threadIdx.x; i < half; i += blockDim.x) {
     float sn, cs;
-    exact_angle(position, turn.inv_freq[i], sn, cs);
+    turn_angle(position, turn.inv_freq[i], turn.rounded, sn, cs);
     cos_s[i] = cs * turn.factor;
     sin_s[i] = sn * turn.factor;
   }
@@ -246,7 +249,7 @@ rows_write_fast_kernel(RowsInput in, RowsNorm norm, RowsTurn turn, RowsPlace pla
   if (turn.inv_freq) {
     for (int i = threadIdx.x; i < count * HALF; i += kFastThreads) {
       float sn, cs;
-      exact_angle(place.positions[t0 + i / HALF], turn.inv_freq[i % HALF], sn, cs);
+      turn_angle(place.positions[t0 + i / HALF], turn.inv_freq[i % HALF], turn.rounded, sn, cs);
       cos_s[i / HALF][i % HALF] = cs * turn.factor;
       sin_s[i / HALF][i % HALF] = sn * turn.factor;
     }
@@ -520,7 +523,7 @@ using namespace distie;
 extern "C" int distie_rows_write(const void* q, int q_stride, const void* k, int k_stride, const void* v, int v_stride, int in_type,
                                  int splits, long long split_stride, const float* q_bias, const float* k_bias, const float* v_bias,
                                  int norm_mode, float norm_eps, const float* q_weight, const float* k_weight, const float* inv_freq,
-                                 int rotary_dim, int interleaved, float factor, float temp_coef, float temp_every,
+                                 int rotary_dim, int interleaved, int rounded, float factor, float temp_coef, float temp_every,
                                  const int* positions, const int* slots, const int* token_seq, const int* seq_seat,
                                  const int* block_table, int table_width, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
                                  int tokens, int num_heads, int num_kv_heads, int key_dim, int value_dim, int page_size, int num_pages,
@@ -536,7 +539,7 @@ extern "C" int distie_rows_write(const void* q, int q_stride, const void* k, int
     return DISTIE_ERR_ARG;
   const RowsInput in{q, k, v, q_stride, k_stride, v_stride, splits, split_stride, q_bias, k_bias, v_bias};
   const RowsNorm norm{norm_mode, norm_eps, q_weight, k_weight};
-  const RowsTurn turn{rotary_dim > 0 ? inv_freq : nullptr, rotary_dim, interleaved, factor, temp_coef, temp_every};
+  const RowsTurn turn{rotary_dim > 0 ? inv_freq : nullptr, rotary_dim, interleaved, rounded, factor, temp_coef, temp_every};
   const RowsPlace place{positions, slots, token_seq, seq_seat};
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, key_dim, value_dim,
                                       page_size, num_pages);

@@ -119,12 +119,12 @@ class CachedRows:
         slots, norm_kind, norm_eps, q_weight, k_weight = step.slots, *norm
         if slots is not None:
             self._check_slots(what, step)
-        frequencies, rotary_dim, interleaved, factor = 0, 0, 0, 1.0
+        frequencies, rotary_dim, interleaved, rounded, factor = 0, 0, 0, 0, 1.0
         if rotary is not None:
             rotary_dim, inv_freq = rotary.rotary_dim, rotary.inv_freq
             if rotary_dim > head_dim or rotary_dim % 2 or inv_freq.dtype != torch.float32 or inv_freq.numel() * 2 < rotary_dim:
                 raise KernelError(f"{what}: a rotary table of float32 frequencies for an even number of a head's elements is expected")
-            frequencies, interleaved, factor = inv_freq.data_ptr(), int(rotary.interleaved), rotary.factor
+            frequencies, interleaved, rounded, factor = inv_freq.data_ptr(), int(rotary.interleaved), int(rotary.rounded), rotary.factor
         for vector in (q_weight, k_weight):
             if vector is not None and (vector.dtype != torch.float32 or vector.numel() != head_dim or not vector.is_contiguous()):
                 raise KernelError(f"{what}: float32 weights of {head_dim} elements are expected")
@@ -143,7 +143,7 @@ class CachedRows:
                 launch(pack(
                     q, q_stride, k, k_stride, v, v_stride, code, splits, split_stride, *bias, norm_kind, norm_eps,
                     0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
-                    frequencies, rotary_dim, interleaved, factor, coef, every, step.positions.data_ptr(),
+                    frequencies, rotary_dim, interleaved, rounded, factor, coef, every, step.positions.data_ptr(),
                     0 if slots is None else slots.data_ptr(), step.token_seq.data_ptr(), step.seq_seat.data_ptr(),
                     table.data_ptr(), table.shape[1], kv.k.data_ptr(), kv.v.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
                     0 if v_scale is None else v_scale.data_ptr(), step.num_tokens, num_heads if q else 0, num_kv_heads, head_dim, value_dim,

@@ -174,6 +174,10 @@ class RotaryTable:
     rotary_dim: int
     interleaved: bool = False
     factor: float = 1.0  # cos and sin are multiplied by it (the attention factor of scaled rotary encodings)
+    # Angles are position * frequency rounded to float32, off by 4e-3 at position 65,536.  The kernel that writes rows of 8-bit
+    # caches and of tokens at places of their own can take the exact product instead, and does unless ``rounded``.  The rows of
+    # a request have to agree: the tables of a model's layers are ``rounded``.
+    rounded: bool = False
 
 
 class KernelSet(ABC):

@@ -126,7 +126,7 @@ _SIGNATURES: dict[str, tuple[str, list]] = {
     "distie_latent_gate": ("latent", [P, I, I, I, P, I, I, L, P, I, I, P]),
     "distie_glu_act": ("latent", [P, I, I, L, I, I, I, F, F, F, P, I, I, L, P, I, I, P]),
     "distie_rows_write": (
-        "cached", [P, I, P, I, P, I, I, I, L, P, P, P, I, F, P, P, P, I, I, F, F, F, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I,
+        "cached", [P, I, P, I, P, I, I, I, L, P, P, P, I, F, P, P, P, I, I, I, F, F, F, P, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I,
                    P, I, I, I, P, P]
     ),
     "distie_rows_read": ("cached", [P, I, P, P, P, P, P, I, P, I, I, I, I, I, P, P, I, I, I, P, P]),

@@ -2,8 +2,8 @@
 
 ``rotary``: the reference's default RoPE (worker/src/inference/qwen2/model.py:93-117):
 ``inv_freq[j] = 1 / theta**(2j / d)`` computed in float32 exactly as there, angles
-``pos * inv_freq`` and their cos/sin evaluated in float32 inside the fused kernel,
-pairs ``(j, j + d/2)`` (rotate-half).  ``rotary_dim < head_dim``, interleaved pairs and
+``pos * inv_freq`` and their cos/sin evaluated in float32 inside the fused kernel (in every step alike:
+``RotaryTable.rounded``), pairs ``(j, j + d/2)`` (rotate-half).  ``rotary_dim < head_dim``, interleaved pairs and
 a factor on cos and sin are parameters for other layer kinds, and so is ``scaling``, which divides the
 frequencies of long waves: with wavelength ``l = 2 pi / f``, ``f`` stays where ``l < original / high``, becomes
 ``f / factor`` where ``l > original / low``, and in between ``(1 - s) f / factor + s f`` with
@@ -92,7 +92,7 @@ class RotaryEncoding:
                 inv_freq = ramped_frequencies(theta, rotary_dim, *scaled[:4])
             else:
                 inv_freq = scaled_frequencies(theta, rotary_dim, *scaled[:4])
-            table = _TABLES[key] = RotaryTable(inv_freq.to(ctx.device), *key[1:4])
+            table = _TABLES[key] = RotaryTable(inv_freq.to(ctx.device), *key[1:4], rounded=True)
         return cls(table)
 
     def rotary_table(self) -> RotaryTable | None:
