@@ -17,8 +17,8 @@
 // element to [1, 2), so that float16 holds it exactly down to 2^-24 of that.
 //
 // Scales: s^k multiplies the finished score.  s^v cannot ride on V without rounding it; p_j s^v_j goes into the second product
-// in float16, in units of a running maximum m' of its own beside the softmax's m: p_j (s^v_j 2^(m - m')), however the scales
-// differ at most a few, and off by at most 2^-11 of itself (or of 2^-14).  Both maxima are whole numbers, rounded down (what they
+// in float16, in units of a running maximum m' of its own beside the softmax's m: (p_j s^v_j) 2^(m - m'), however the scales
+// differ at most a few, and off by at most 2^-11 of itself (or of 2^-14); p_j below 2^-126 is 0 whatever its value's scale.  Both maxima are whole numbers, rounded down (what they
 // scale, they scale exactly), and are not searched for in every group, only in a head's first and where weights outgrow the ones in
 // use: no shuffles and no correction of O in most groups.  Sums and maxima are float32.  The warps, and with several splits the
 // CTAs, are merged in the softmax's units: inside the cluster up to 8 splits, where every CTA sends its sums to the one that puts
@@ -371,7 +371,8 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
             }
             col_max[nh][e] = m_new;
             out_max[nh][e] = o_new;
-            // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0)
+            // (2^(m - m') outgrows float32 only where every value so far is below 2^-126; those weights are 0.  Weight times scale
+            // comes first in the products below: scale times 2^(m - m') can be infinite beside a weight of 0)
             units[nh][e] = o_new == -INFINITY ? 0.f : dec_exp2(fminf((m_new == -INFINITY ? 0.f : m_new) - o_new, 126.f));
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
@@ -391,7 +392,7 @@ attention_decode_e4m3_kernel(const __nv_bfloat16* __restrict__ q, int q_stride, 
           for (int i = 0; i < RK; ++i) {
             const float p = dec_exp2(x[i][e]);
             sum[e] += p;
-            w[i][e] = p * (vs_s[i] * units[nh][e]);
+            w[i][e] = (p * vs_s[i]) * units[nh][e];
             weights += w[i][e];
           }
           most = fmaxf(most, fmaxf(weights, sum[e] * (kDecMostWeight / kDecMostSum)));

@@ -17,7 +17,7 @@
 // a block, each step waiting for the one before.)  So Q (times a power of two a row, float16), K, P and V are float16 there
 // and bfloat16 of a 16-bit cache.  The
 // scales of the rows go beside the tiles: s^k multiplies the finished score; the weights of the second product are p s^v over
-// a running maximum m' of their own, p (s^v 2^(m - m')), so that float16 holds the largest of a row near 1 whatever
+// a running maximum m' of their own, (p s^v) 2^(m - m'), so that float16 holds the largest of a row near 1 whatever
 // the scales.
 //
 // Masks: a block that lies before every row's new tokens and inside every row's window needs none; the others get 64 bits a
@@ -739,7 +739,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
                 float w0, w1;
                 if (E4M3) {
                   total = add_pairs(total, p);
-                  const uint64_t w = mul_pairs(p, mul_pairs(scale2[e >> 1], units2));
+                  const uint64_t w = mul_pairs(mul_pairs(p, scale2[e >> 1]), units2);  // (scale times units can be infinite beside a weight of 0)
                   weight4[e >> 1] = add_pairs(weight4[e >> 1], w);
                   halves_of(w, w0, w1);
                   const __half2 pair = __floats2half2_rn(w0, w1);
