@@ -324,14 +324,9 @@ rows_write_fast_kernel(RowsInput in, RowsNorm norm, RowsTurn turn, RowsPlace pla
           const bool bad = nothing != nothing;
           const float scale = row_scale(most, bad);
           if (e0 == 0) (is_value ? v_scale : k_scale)[row] = scale;
-          if (scale >= 1e-37f) {  // (the reciprocal of a smaller one is not a number)
-            const float inv = 1.f / scale;
+          const bool nothing_held = bad || scale == 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] *= inv;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = bad || scale == 0.f ? 0.f : v[e] / scale;
-          }
+          for (int e = 0; e < 16; ++e) v[e] = nothing_held ? 0.f : v[e] / scale;  // (times 1 / scale, numbers next to a border fell on its other side)
           uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(out) + (size_t)row * D + e0);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
