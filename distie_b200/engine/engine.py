@@ -373,6 +373,7 @@ class Engine:
                     raise CacheExhausted("out of KV blocks for the prompt")
                 logits = self.runner.step([BatchEntry(seat, part, at, (len(part) - 1,))])
                 cached = at + len(part)
+                self.cache.trim(seat, cached)
             pick = int(torch.argmax(logits[0]))
             self.runner.finish_step()
             while True:

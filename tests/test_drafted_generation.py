@@ -1,0 +1,35 @@
+"""Drafted generation beside other requests, near its end, and with drafters that are wrong."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import helpers
+import test_fovudra as fovudra
+from ref_cached import RefCached
+from test_cached_engine import engine_for
+
+NONE = lambda ids: ([], [])  # noqa: E731
+
+
+@pytest.mark.parametrize("budget", [4096, 8])
+def test_pages_behind_a_window_go_back_before_the_first_guess(budget):
+    """Layers with a window of 8 over pages of 4: behind a prompt of 32 tokens they hold three pages, not eight, and the request
+    goes on beside another one that holds the last."""
+    layer = fovudra._attention(4, 2, 16, 8, 0, 16, 1e4, None, 0.25, fovudra._moe(3, 1, 20, None))
+    cfg = {"architecture": "Fovudra", "vocab": 101, "width": 48, "norm": {"eps": 1e-5}, "layers": [layer, layer]}
+    weights = fovudra.pf.random_weights(cfg, 5)
+    prompt = helpers.random_ids(101, 32, 8)
+    made = []
+    for drafted in (False, True):
+        engine = fovudra.engine_of(cfg, weights, 4, RefCached(torch.float32), 9, token_budget=budget, max_model_len=40)
+        other = engine.cache.open_seat()
+        assert engine.cache.grow(other, 1)
+        if drafted:
+            made.append(engine.generate_drafted(prompt, NONE, 4, eos_id=None).token_ids)
+        else:
+            made.append(engine.generate([prompt], max_new_tokens=4, ignore_eos=True)[0].token_ids)
+        engine.cache.close_seat(other)
+        assert engine.cache.free_pages() == engine.cache.total_pages()
+    assert made[0] == made[1] and len(made[0]) == 4
