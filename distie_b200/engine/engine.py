@@ -31,7 +31,7 @@ from ..kernels import make_kernels
 from ..kernels.interface import E4M3, MOST_DRAFTED
 from ..models.decoder import DecoderModel, model_tensor_specs, slot_needs
 from ..weights.loader import open_weights
-from .batch import BatchEntry
+from .batch import BatchEntry, tree_of
 from .runner import ModelRunner
 from .scheduler import Emission, Scheduler, Sequence as Seq
 from .step_stats import StepStats
@@ -385,12 +385,13 @@ class Engine:
                     made.finish_reason = "length"
                 if made.finish_reason:
                     return made
-                tokens, parents = drafter(list(ids))
+                tokens, parents = (list(map(int, numbers)) for numbers in drafter(list(ids)))
                 if len(tokens) != len(parents):
                     raise ValueError(f"{len(tokens)} drafted tokens with {len(parents)} parents")
+                tree_of(parents)  # (refuses parents that are none, before they are numbered behind the last token)
                 # No more than a step takes, the tables hold or the request still wants behind the token it has.
                 room = min(MOST_DRAFTED, self.runner.max_step_tokens, longest - cached) - 1
-                tokens, parents = [pick, *map(int, tokens[:room])], [-1, *(int(p) + 1 for p in parents[:room])]
+                tokens, parents = [pick, *tokens[:room]], [-1, *(p + 1 for p in parents[:room])]
                 if not self.cache.grow(seat, cached + len(tokens)):
                     tokens, parents = tokens[:1], parents[:1]
                     if not self.cache.grow(seat, cached + 1):

@@ -33,3 +33,13 @@ def test_pages_behind_a_window_go_back_before_the_first_guess(budget):
         engine.cache.close_seat(other)
         assert engine.cache.free_pages() == engine.cache.total_pages()
     assert made[0] == made[1] and len(made[0]) == 4
+
+
+@pytest.mark.parametrize("parents, word", [([-2], "parent"), ([-1, -2, 0], "parent"), ([-1, 1], "parent"), ([-1] * 300 + [300], "parent")])
+def test_parents_that_are_none_are_refused(parents, word):
+    """-2 is no parent: as the number behind the last token's it would have been taken for a second root.  The guesses that a step
+    has no room for are looked at too."""
+    engine, _, _ = engine_for("A")
+    with pytest.raises(ValueError, match=word):
+        engine.generate_drafted([1, 2], lambda ids: ([5] * len(parents), parents), 40, eos_id=None)
+    assert engine.cache.free_pages() == engine.cache.total_pages() and engine.cache.free_seats == 8
