@@ -55,13 +55,20 @@ class StepLayout:
     most_nodes: int = 0
 
 
-def tree_of(parents: Sequence[int]) -> tuple[list[int], list[int]]:
-    """(depth of every node, its ancestors and itself as the bits of a number)."""
-    depths, seen = [], []
+def depths_of(parents: Sequence[int]) -> list[int]:
+    """The depth of every node of a tree, 0 for roots; refuses parents that are none."""
+    depths = []
     for node, parent in enumerate(parents):
         if not -1 <= parent < node:
             raise ValueError(f"a drafted token's parent is one of those before it or -1, got {parent} for token {node}")
         depths.append(0 if parent < 0 else depths[parent] + 1)
+    return depths
+
+
+def tree_of(parents: Sequence[int]) -> tuple[list[int], list[int]]:
+    """(depth of every node, its ancestors and itself as the bits of a number)."""
+    depths, seen = depths_of(parents), []
+    for node, parent in enumerate(parents):
         seen.append((1 << node) | (seen[parent] if parent >= 0 else 0))
     return depths, seen
 

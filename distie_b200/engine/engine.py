@@ -31,7 +31,7 @@ from ..kernels import make_kernels
 from ..kernels.interface import E4M3, MOST_DRAFTED
 from ..models.decoder import DecoderModel, model_tensor_specs, slot_needs
 from ..weights.loader import open_weights
-from .batch import BatchEntry, tree_of
+from .batch import BatchEntry, depths_of
 from .runner import ModelRunner
 from .scheduler import Emission, Scheduler, Sequence as Seq
 from .step_stats import StepStats
@@ -388,10 +388,13 @@ class Engine:
                 tokens, parents = (list(map(int, numbers)) for numbers in drafter(list(ids)))
                 if len(tokens) != len(parents):
                     raise ValueError(f"{len(tokens)} drafted tokens with {len(parents)} parents")
-                tree_of(parents)  # (refuses parents that are none, before they are numbered behind the last token)
-                # No more than a step takes, the tables hold or the request still wants behind the token it has.
+                # No more guesses than a step takes and the tables hold, and none too deep to become output: of the tokens that the
+                # request still wants the last follows the last guess.
                 room = min(MOST_DRAFTED, self.runner.max_step_tokens, longest - cached) - 1
-                tokens, parents = [pick, *tokens[:room]], [-1, *(p + 1 for p in parents[:room])]
+                deepest = limit - len(made.token_ids) - 2
+                kept = [guess for guess, depth in enumerate(depths_of(parents)) if depth <= deepest][:room]
+                node_of = {-1: 0, **{guess: node for node, guess in enumerate(kept, start=1)}}
+                tokens, parents = [pick, *(tokens[g] for g in kept)], [-1, *(node_of[parents[g]] for g in kept)]
                 if not self.cache.grow(seat, cached + len(tokens)):
                     tokens, parents = tokens[:1], parents[:1]
                     if not self.cache.grow(seat, cached + 1):

@@ -43,3 +43,37 @@ def test_parents_that_are_none_are_refused(parents, word):
     with pytest.raises(ValueError, match=word):
         engine.generate_drafted([1, 2], lambda ids: ([5] * len(parents), parents), 40, eos_id=None)
     assert engine.cache.free_pages() == engine.cache.total_pages() and engine.cache.free_seats == 8
+
+
+def checked(engine):
+    """The numbers of guesses that each step of an engine brings."""
+    seen, run = [], engine.runner.step
+
+    def step(entries):
+        if entries[0].parents is not None:
+            seen.append(len(entries[0].tokens) - 1)
+        return run(entries)
+
+    engine.runner.step = step
+    return seen
+
+
+def test_guesses_that_the_request_has_no_use_for_are_not_checked():
+    """With n tokens still wanted behind the one that a step begins with, guesses below depth n - 1 cannot become output."""
+    engine, cfg, _ = engine_for("A")
+    prompt, vocab = helpers.random_ids(cfg["vocab_size"], 9, 3), cfg["vocab_size"]
+    answer = engine.generate([prompt], max_new_tokens=12, ignore_eos=True)[0].token_ids
+
+    def drafter(ids):  # a chain of five right guesses, and two wrong ones beside its second and at its end
+        at = len(ids) - len(prompt)
+        right = (answer + answer)[at : at + 5]
+        return [*right[:2], (right[1] + 1) % vocab, *right[2:], (right[4] + 1) % vocab], [-1, 0, 0, 1, 3, 4, 4]
+
+    seen = checked(engine)
+    made = engine.generate_drafted(prompt, drafter, 9, eos_id=None)
+    # Nine tokens: the prompt's, five guesses and the one behind them, then two more, of which one can be a guess.
+    assert made.token_ids == answer[:9] and seen == [7, 1] and made.drafted == 8 and made.accepted == 6
+    engine, _, _ = engine_for("A")
+    seen = checked(engine)
+    made = engine.generate_drafted(prompt, lambda ids: ([answer[len(ids) - len(prompt)]] * 300, [-1] * 300), 2, eos_id=None)
+    assert made.token_ids == answer[:2] and seen == [0] and made.drafted == 0
