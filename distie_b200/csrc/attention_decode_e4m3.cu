@@ -580,7 +580,7 @@ extern "C" int distie_attention_decode_e4m3(const void* q, int q_stride, void* o
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, head_dim, head_dim,
                                       page_size, num_pages);
   const int group = num_heads / num_kv_heads, chunks = (group + 15) / 16;
-  const QueryRows rows{positions, token_seq, seq_seat, nullptr, nullptr, 1, tokens, group, num_heads, window, chunk, keep_first,
+  const QueryRows rows{positions, token_seq, seq_seat, nullptr, nullptr, 1, tokens, tokens, 1, group, num_heads, window, chunk, keep_first,
                        scale * 1.4426950408889634f, make_score_extras(scale, softcap, sink)};
   const Partials parts{scratch, scratch ? scratch + (size_t)tokens * num_heads * splits * head_dim : nullptr, splits};
   const int cluster_merge = splits > 1 && splits <= kDecClusterSplits;
@@ -599,7 +599,7 @@ extern "C" int distie_attention_decode_e4m3(const void* q, int q_stride, void* o
   }
 #undef DISTIE_DECODE_E4M3
   if (err != cudaSuccess) return (int)err;
-  if (splits > 1 && !cluster_merge) return rows_merge_bf16(parts, out, out_stride, tokens, num_heads, head_dim, sink, stream);
+  if (splits > 1 && !cluster_merge) return rows_merge_bf16(parts, rows, out, out_stride, head_dim, stream);
   return 0;
 }
 

@@ -77,7 +77,10 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
   const Request request = request_of(rows, b);
   const int kv_head = blockIdx.x % cache.num_kv_heads, tile = blockIdx.x / cache.num_kv_heads;
   const int row0 = tile * kRowsTile, all_rows = request.nodes * rows.group;
-  if (row0 >= all_rows) return;
+  if (row0 >= all_rows) {
+    if (blockIdx.x == 0 && b == 0 && split == 0) grid_dependency_wait();  // (some block of the grid always waits: kernels end in order)
+    return;
+  }
   const int count = min(kRowsTile, all_rows - row0);
   const int* table = cache.block_table + (size_t)request.seat * cache.table_width;
 
@@ -278,7 +281,7 @@ constexpr int kMergeThreads = 128;
 
 template <typename T, int SHARE>
 __global__ void __launch_bounds__(kMergeThreads)
-attention_rows_merge_kernel(Partials parts, T* __restrict__ out, int out_stride, int num_rows, int num_heads, int value_dim, const float* __restrict__ sink) {
+attention_rows_merge_kernel(Partials parts, QueryRows rows, T* __restrict__ out, int out_stride, int num_rows, int value_dim) {
   constexpr int ROWS = kMergeThreads / 32 / SHARE, PASSES = kRowsMostDim / 128;
   __shared__ float sh_acc[SHARE][PASSES * 128 + 4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % SHARE;
@@ -290,7 +293,10 @@ attention_rows_merge_kernel(Partials parts, T* __restrict__ out, int out_stride,
   const int groups = 32 / across, mine = lane / across, column = lane % across * 4;
   const bool whole = value_dim % 4 == 0;
   const size_t part0 = (size_t)row * parts.splits;
+  const int token = row / rows.num_heads, head = row % rows.num_heads;
+  const bool somebodys = token_is_somebodys(rows, token);
   grid_dependency_wait();
+  if (!somebodys) return;  // (a block's warps that meet at a barrier share their row)
   // A part without a key has a sum of 0, one whose scores are all NaN a sum of NaN; both have no maximum.
   float m_mine = lane < parts.splits ? __ldcg(parts.ml + (part0 + lane) * 2) : -INFINITY, l_mine = lane < parts.splits ? __ldcg(parts.ml + (part0 + lane) * 2 + 1) : 0.f;
   float m_all = m_mine;
@@ -359,8 +365,7 @@ attention_rows_merge_kernel(Partials parts, T* __restrict__ out, int out_stride,
         for (int w = 1; w < SHARE; ++w) acc[pass][e] += sh_acc[w][pass * 128 + column + e];
   }
   if (mine != 0) return;
-  const int token = row / num_heads, head = row % num_heads;
-  const float inv = sink ? sink_inverse_log2(m_all, l_all, sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
+  const float inv = rows.extras.sink ? sink_inverse_log2(m_all, l_all, rows.extras.sink[head]) : (l_all == 0.f ? 0.f : 1.f / l_all);
 #pragma unroll
   for (int pass = 0; pass < PASSES; ++pass)
 #pragma unroll
@@ -371,19 +376,17 @@ attention_rows_merge_kernel(Partials parts, T* __restrict__ out, int out_stride,
 }
 
 template <typename T>
-static int rows_merge(const Partials& parts, void* out, int out_stride, int tokens, int num_heads, int value_dim, const float* sink,
-                      cudaStream_t stream) {
-  const int rows = tokens * num_heads;
-  if (parts.splits > 16 || (parts.splits > 4 && rows <= 512))
-    return (int)launch_dependent(attention_rows_merge_kernel<T, 4>, dim3(rows), dim3(kMergeThreads), 0, stream, parts, (T*)out, out_stride, rows,
-                                 num_heads, value_dim, sink);
-  return (int)launch_dependent(attention_rows_merge_kernel<T, 1>, dim3((rows + 3) / 4), dim3(kMergeThreads), 0, stream, parts, (T*)out, out_stride, rows,
-                               num_heads, value_dim, sink);
+static int rows_merge(const Partials& parts, const QueryRows& rows, void* out, int out_stride, int value_dim, cudaStream_t stream) {
+  const int count = rows.tokens * rows.num_heads;
+  if (parts.splits > 16 || (parts.splits > 4 && count <= 512))
+    return (int)launch_dependent(attention_rows_merge_kernel<T, 4>, dim3(count), dim3(kMergeThreads), 0, stream, parts, rows, (T*)out, out_stride,
+                                 count, value_dim);
+  return (int)launch_dependent(attention_rows_merge_kernel<T, 1>, dim3((count + 3) / 4), dim3(kMergeThreads), 0, stream, parts, rows, (T*)out,
+                               out_stride, count, value_dim);
 }
 
-int rows_merge_bf16(const Partials& parts, void* out, int out_stride, int tokens, int num_heads, int value_dim, const float* sink,
-                    cudaStream_t stream) {
-  return rows_merge<__nv_bfloat16>(parts, out, out_stride, tokens, num_heads, value_dim, sink, stream);
+int rows_merge_bf16(const Partials& parts, const QueryRows& rows, void* out, int out_stride, int value_dim, cudaStream_t stream) {
+  return rows_merge<__nv_bfloat16>(parts, rows, out, out_stride, value_dim, stream);
 }
 
 }  // namespace distie
@@ -408,7 +411,7 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
   if ((long long)num_pages * num_kv_heads * page_size > 0xffffffffLL) return DISTIE_ERR_UNSUPPORTED;
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, key_dim, value_dim,
                                       page_size, num_pages);
-  const QueryRows rows{positions, token_seq, seq_seat, seqs, bits, words, tokens, num_heads / num_kv_heads, num_heads, window, chunk, keep_first,
+  const QueryRows rows{positions, token_seq, seq_seat, seqs, bits, words, tokens, requests, most_nodes, num_heads / num_kv_heads, num_heads, window, chunk, keep_first,
                        scale * 1.4426950408889634f, make_score_extras(scale, softcap, sink)};
   const Partials parts{scratch, scratch ? scratch + (size_t)tokens * num_heads * splits * value_dim : nullptr, splits};
   const int tiles = (most_nodes * rows.group + kRowsTile - 1) / kRowsTile;
@@ -423,7 +426,7 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
     err = launch_dependent(attention_rows_kernel<T, CACHE>, grid, dim3(kRowsThreads), shared, stream, (const T*)q, q_stride, (T*)out,         \
                            out_stride, rows, cache, parts, error);                                                                   \
     if (err != cudaSuccess) return (int)err;                                                                                        \
-    if (splits > 1) return rows_merge<T>(parts, out, out_stride, tokens, num_heads, value_dim, sink, stream);                          \
+    if (splits > 1) return rows_merge<T>(parts, rows, out, out_stride, value_dim, stream);                                             \
     return 0;                                                                                                                       \
   }
   if (dtype == DISTIE_BF16 && cache_type == DISTIE_E4M3) DISTIE_ROWS(__nv_bfloat16, DISTIE_E4M3)

@@ -250,7 +250,10 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap map_k, const _
   }
   const Request request = request_of(rows, blockIdx.y);
   const int row0 = tile * kTreeRows, count = min(kTreeRows, request.nodes * rows.group - row0);
-  if (count <= 0) return;
+  if (count <= 0) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && split == 0) grid_dependency_wait();  // (some CTA of the grid always waits: kernels end in order)
+    return;
+  }
   const int active = (count + 31) / 32;  // warps of a softmax group that have rows
   const int* table = cache.block_table + (size_t)request.seat * cache.table_width;
 
@@ -892,7 +895,7 @@ using namespace distie;
 // scales) e4m3, heads of 64 or 128 (else DISTIE_ERR_UNSUPPORTED, like rows that are not aligned to what a thread moves), at most
 // 256 new tokens a request.  seqs [requests, 3], bits [tokens, words].  scratch: tokens * heads * splits * (value size + 2) floats.
 extern "C" int distie_attention_tree_tcgen05(const void* q, int q_stride, void* out, int out_stride, float* scratch, const int* positions,
-                                             const int* seq_seat, const int* seqs, const int* bits, int words, int requests, int tokens,
+                                             const int* token_seq, const int* seq_seat, const int* seqs, const int* bits, int words, int requests, int tokens,
                                              int most_nodes, const void* k_cache, const void* v_cache, const float* k_scale,
                                              const float* v_scale, const int* block_table, int table_width, int num_heads, int num_kv_heads,
                                              int head_dim, int page_size, int num_pages, int window, int chunk, int keep_first, float scale,
@@ -908,7 +911,7 @@ extern "C" int distie_attention_tree_tcgen05(const void* q, int q_stride, void* 
   const CachePages cache = make_pages(k_cache, v_cache, k_scale, v_scale, block_table, table_width, num_kv_heads, head_dim, head_dim,
                                       page_size, num_pages);
   const int group = num_heads / num_kv_heads;
-  const QueryRows rows{positions, nullptr, seq_seat, seqs, bits, words, tokens, group, num_heads, window, chunk, keep_first,
+  const QueryRows rows{positions, token_seq, seq_seat, seqs, bits, words, tokens, requests, most_nodes, group, num_heads, window, chunk, keep_first,
                        scale * 1.4426950408889634f, make_score_extras(scale, softcap, sink)};
   const Partials parts{scratch, scratch ? scratch + (size_t)tokens * num_heads * splits * head_dim : nullptr, splits};
   const dim3 grid((unsigned)(((long long)most_nodes * group + kTreeRows - 1) / kTreeRows * num_kv_heads), requests, splits);
@@ -920,7 +923,7 @@ extern "C" int distie_attention_tree_tcgen05(const void* q, int q_stride, void* 
     status = k_scale ? launch_tree<128, true>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts, error, stream)
                      : launch_tree<128, false>(grid, (const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride, rows, cache, parts, error, stream);
   if (status != 0 || splits == 1) return status;
-  return rows_merge_bf16(parts, out, out_stride, tokens, num_heads, head_dim, sink, stream);
+  return rows_merge_bf16(parts, rows, out, out_stride, head_dim, stream);
 }
 
 DISTIE_PACKED(distie_attention_tree_tcgen05)

@@ -52,8 +52,9 @@ __host__ inline CachePages make_pages(const void* k, const void* v, const float*
 
 // The query rows of a step, request by request.  Request b has `nodes` new tokens, tokens first .. first + nodes - 1 of the
 // step, whose keys and values stand behind its `past` cached ones (new token j at place past + j).  A new token sees the
-// cached places that its window allows and new token j when bit j of its mask is set.  Without `seqs` every token is a
-// request of its own: a single token behind positions[t] cached ones, which sees itself.
+// cached places that its window allows and new token j when bit j of its mask is set.  Tokens of no request are nobody's: nothing
+// is written for them.  Without `seqs` every token is a request of its own: a single token behind positions[t] cached ones, which
+// sees itself.
 struct QueryRows {
   const int* positions;   // [tokens]
   const int* token_seq;   // [tokens]
@@ -62,6 +63,8 @@ struct QueryRows {
   const int* bits;        // [tokens, words]
   int words;
   int tokens;             // of the step
+  int requests;
+  int most_nodes;         // new tokens of a request that the grid has tiles for
   int group;              // query heads per kv head
   int num_heads;
   int window, chunk, keep_first;
@@ -76,9 +79,9 @@ struct Request {
 __device__ __forceinline__ Request request_of(const QueryRows& rows, int b) {
   Request r;
   if (rows.seqs) {
-    // (held to the step's tokens and to the masks' words, whatever the rows say)
+    // (held to the step's tokens, the masks' words and the grid, whatever the rows say)
     r.first = min(max(rows.seqs[3 * b], 0), rows.tokens);
-    r.nodes = min(min(max(rows.seqs[3 * b + 1], 0), rows.words * 32), rows.tokens - r.first);
+    r.nodes = min(min(max(rows.seqs[3 * b + 1], 0), min(rows.words * 32, rows.most_nodes)), rows.tokens - r.first);
     r.past = max(rows.seqs[3 * b + 2], 0);
     r.seat = rows.seq_seat[b];
   } else {
@@ -88,6 +91,15 @@ __device__ __forceinline__ Request request_of(const QueryRows& rows, int b) {
     r.seat = rows.seq_seat[rows.token_seq[b]];
   }
   return r;
+}
+
+// Whether a token belongs to a request.
+__device__ __forceinline__ bool token_is_somebodys(const QueryRows& rows, int token) {
+  if (rows.seqs == nullptr) return true;
+  const int b = rows.token_seq[token];
+  if (b < 0 || b >= rows.requests) return false;
+  const Request r = request_of(rows, b);
+  return token >= r.first && token < r.first + r.nodes;
 }
 
 // Whether new token `node` of its request sees new token j (bit j of its mask).
@@ -132,7 +144,6 @@ struct Partials {
 };
 
 // Joins the parts of every (token, head) into 16-bit rows (attention_rows.cu).
-int rows_merge_bf16(const Partials& parts, void* out, int out_stride, int tokens, int num_heads, int value_dim, const float* sink,
-                    cudaStream_t stream);
+int rows_merge_bf16(const Partials& parts, const QueryRows& rows, void* out, int out_stride, int value_dim, cudaStream_t stream);
 
 }  // namespace distie

@@ -345,7 +345,7 @@ class CachedRows:
         with self._here():
             code = launch(pack(
                 q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), _ptr(scratch), step.positions.data_ptr(),
-                step.seq_seat.data_ptr(), tree.seqs.data_ptr(), tree.bits.data_ptr(), tree.bits.shape[1], requests, tokens, most,
+                step.token_seq.data_ptr(), step.seq_seat.data_ptr(), tree.seqs.data_ptr(), tree.bits.data_ptr(), tree.bits.shape[1], requests, tokens, most,
                 kv.k.data_ptr(), kv.v.data_ptr(), _ptr(kv.k_scale), _ptr(kv.v_scale), kv.block_table.data_ptr(),
                 kv.block_table.shape[-1], num_heads, num_kv_heads, head_dim, kv.page_size, kv.num_pages, window, chunk, keep_first,
                 float(scale), softcap, _ptr(sink), splits, self.error_flag.data_ptr(), self._stream(),

@@ -48,7 +48,8 @@ class DraftTree:
     of the step, behind ``past`` cached ones; new token j stands in the cache's place ``past + j`` (``StepTensors.slots``)
     whatever its position, ``past`` plus its depth.  A new token sees the cached keys that its window or chunk allows, and of
     its request's new tokens those whose bits are set in its mask: itself and its ancestors, or any others; a token whose
-    mask is empty and that has no cached key gets zeros.  Windows and chunks count positions, not places."""
+    mask is empty and that has no cached key gets zeros.  Tokens of no request are left as they were.  Windows and chunks count
+    positions, not places."""
 
     bits: torch.Tensor  # [T, words] int32: bit j % 32 of word j / 32 is new token j of the same request
     seqs: torch.Tensor  # [B, 3] int32: first, nodes, past

@@ -138,7 +138,7 @@ _SIGNATURES: dict[str, tuple[str, list]] = {
         "cached", [P, I, P, I, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, F, P, I, P, P]
     ),
     "distie_attention_tree_tcgen05": (
-        "cached", [P, I, P, I, P, P, P, P, P, I, I, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, F, P, I, P, P]
+        "cached", [P, I, P, I, P, P, P, P, P, P, I, I, I, I, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, F, P, I, P, P]
     ),
     "distie_gated_rmsnorm": ("state", [P, I, P, I, I, L, P, I, P, I, I, I, I, F, I, I, P]),
     "distie_gemm_tcgen05": ("bf16", [P, I, P, P, I, I, I, I, I, I, I, P, P]),
