@@ -420,7 +420,7 @@ extern "C" int distie_attention_rows(const void* q, int q_stride, void* out, int
   cudaError_t err;
 #define DISTIE_ROWS(T, CACHE)                                                                                                       \
   {                                                                                                                                 \
-    if (shared > 48 * 1024 && (err = cudaFuncSetAttribute(attention_rows_kernel<T, CACHE>,                                           \
+    if (shared > 40 * 1024 && (err = cudaFuncSetAttribute(attention_rows_kernel<T, CACHE>, /* (48 KB hold the static arrays too) */  \
                                                           cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024)) != cudaSuccess)  \
       return (int)err;                                                                                        \
     err = launch_dependent(attention_rows_kernel<T, CACHE>, grid, dim3(kRowsThreads), shared, stream, (const T*)q, q_stride, (T*)out,         \
