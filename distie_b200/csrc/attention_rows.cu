@@ -45,7 +45,7 @@ __device__ __forceinline__ void add_values(float (&acc)[kRowsTile][2], int i, co
         acc[r + 3][i] += w.w * v;
       }
     }
-  } else {  // 0 * NaN is not 0: a value that is not finite reaches the rows that see it alone
+  } else {  // 0 * NaN is not 0: a value that is not finite reaches the rows that see it (their weights are above 0), and no others
     for (int j = 0; j < kRowsKeys; ++j) {
       const float v = values[j * vdim];
 #pragma unroll
@@ -217,7 +217,9 @@ attention_rows_kernel(const T* __restrict__ q, int q_stride, T* __restrict__ out
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float m_old = m_mine[u], m_new = fmaxf(m_old, most[u]), corr = m_old == -INFINITY ? 0.f : exp2f(m_old - m_new);
-        p[u] = sum[u] = x[u] == -INFINITY ? 0.f : exp2f(x[u] - m_new);
+        p[u] = x[u] == -INFINITY ? 0.f : exp2f(x[u] - m_new);
+        if (bad_s && p[u] == 0.f && x[u] != -INFINITY) p[u] = 1.4e-45f;  // (the smallest number: whoever sees a value that is not finite gets it)
+        sum[u] = p[u];
         m_mine[u] = m_new;
         l_mine[u] *= corr;
         if (lane == 0) corr_s[warp * 4 + u] = corr;
