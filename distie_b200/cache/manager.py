@@ -227,16 +227,20 @@ class KvGroup:
                 self._uploaded = torch.cuda.Event()
             self._uploaded.record()
 
-    def move_rows(self, seat: int, sources: list[int], targets: list[int]) -> None:
-        """The rows of places ``sources`` of a seat, in every slot, to ``targets`` (all are read before any is written)."""
-        if self.device_table is None:
-            return
-        place = np.asarray([sources, targets], dtype=np.int64)
+    def rows_at(self, seat: int, places: list[int]) -> np.ndarray:
+        """[page, row in it] of the places of a seat, all of which it has to hold."""
+        place = np.asarray(places, dtype=np.int64)
         pages = self.host_table[seat, place // self.page_size].astype(np.int64)
         if bool((pages < 0).any()):
-            raise ValueError(f"seat {seat} holds no page for some of the places {sources} and {targets}")
-        index = torch.from_numpy(np.stack([pages, place % self.page_size])).to(self.device_table.device)
-        (from_page, to_page), (from_row, to_row) = index[0], index[1]
+            raise ValueError(f"seat {seat} holds no page for some of the places {places}")
+        return np.stack([pages, place % self.page_size])
+
+    def move_rows(self, sources: np.ndarray, targets: np.ndarray) -> None:
+        """The rows ``sources`` (of :meth:`rows_at`), in every slot, to ``targets`` (all are read before any is written)."""
+        if self.device_table is None:
+            return
+        index = torch.from_numpy(np.stack([sources, targets])).to(self.device_table.device)
+        (from_page, from_row), (to_page, to_row) = index[0], index[1]
         held = [self._keys] if self.need.values_in_keys else [self._keys, self._values]
         held = [t.view(torch.uint8) if t.dtype == E4M3 else t for t in held]  # (numbers of eight bits move as bytes)
         if self._scales is not None:
@@ -400,8 +404,10 @@ class CacheManager:
         if moved:
             if self.state_needs:
                 raise ValueError("layers with per-request state cannot take back some of a step's tokens")
-            for group in self.groups:
-                group.move_rows(seat, *map(list, zip(*moved)))
+            sources, targets = map(list, zip(*moved))
+            found = [(group.rows_at(seat, sources), group.rows_at(seat, targets)) for group in self.groups]  # (all, before any moves)
+            for group, rows in zip(self.groups, found):
+                group.move_rows(*rows)
         return cached + len(places)
 
     # -- what a step sees -----------------------------------------------------

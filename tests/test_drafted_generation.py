@@ -10,6 +10,9 @@ import test_fovudra as fovudra
 from ref_cached import RefCached
 from test_cached_engine import engine_for
 
+from distie_b200.cache import CacheManager
+from distie_b200.parts.base import CacheNeed
+
 NONE = lambda ids: ([], [])  # noqa: E731
 
 
@@ -77,3 +80,18 @@ def test_guesses_that_the_request_has_no_use_for_are_not_checked():
     seen = checked(engine)
     made = engine.generate_drafted(prompt, lambda ids: ([answer[len(ids) - len(prompt)]] * 300, [-1] * 300), 2, eos_id=None)
     assert made.token_ids == answer[:2] and seen == [0] and made.drafted == 0
+
+
+def test_a_refused_path_moves_nothing():
+    """A group whose window has given a place's page back refuses the path; no other group has moved its rows then."""
+    needs = {0: CacheNeed(1, 8), 1: CacheNeed(1, 8, window=4)}
+    cache = CacheManager(needs, num_pages=8, page_size=2, max_seats=1, max_tokens_per_request=16, dtype=torch.float32, device="cpu")
+    seat = cache.open_seat()
+    assert cache.grow(seat, 12)
+    for slot in (0, 1):
+        cache.kv_slot(slot).k.copy_(torch.arange(cache.kv_slot(slot).k.numel()).reshape(cache.kv_slot(slot).k.shape))
+    cache.trim(seat, 12)  # (as if all twelve had been kept)
+    before = [cache.kv_slot(slot).k.clone() for slot in (0, 1)]
+    with pytest.raises(ValueError, match="holds no page"):
+        cache.keep_places(seat, 4, [1, 3])
+    assert all(torch.equal(cache.kv_slot(slot).k, old) for slot, old in zip((0, 1), before))
